@@ -398,7 +398,7 @@ def _exact_8_bits(x, random):
     top = x.view(-1, BLOCK).abs().amax(1)
     part, power = torch.frexp(top)  # top = part * 2^power, part in [0.5, 1); 448 = 0.875 * 2^9
     scale = torch.ldexp(torch.ones_like(top), torch.where(part > 0.875, power - 8, power - 9))
-    scale = scale.clamp(min=2.0 ** -126)
+    scale = torch.where(top > 0, scale, 0.0).clamp(min=2.0 ** -126)
     y = x.abs() / scale.repeat_interleave(BLOCK)
     step = torch.ldexp(torch.ones_like(y), (torch.frexp(y).exponent - 1).clamp(min=-6) - 3)
     q = torch.floor(y / step + (random.double() + 0.5) / 65536) * step
