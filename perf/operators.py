@@ -194,7 +194,7 @@ def run(s):
 
 def _own(s, case):
     import arboretum_b200
-    pooled = case["per_bag"] > 1
+    pooled = case.get("per_bag", 1) > 1
     if case["op"] == "lookup":
         return arboretum_b200.embedding(s["tokens"] if pooled else s["tokens"].view(-1), s["table"], scale=_scale(case), pooled=pooled)
     if case["op"] == "grad":
