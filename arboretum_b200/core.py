@@ -35,7 +35,9 @@ def _load_lib():
                  "ACreateFromBinnedMatrix", "ASetThresholds", "AQuantize", "AGetTrainY",
                  "AGetLevelStats", "AGetLevelStatsOf", "AGetGradientStep", "APeerWaitProbe", "ASetProfile", "AGetTimings", "ABuildHistogram",
                  "ABuildHistogramFromParents", "ANcclUniqueId", "AInitNccl", "AThresholdsNoAlloc", "ASharedAtomicPeak",
-                 "AReleaseCachedMemory"):
+                 "AReleaseCachedMemory", "AEmbedding", "ATokenOrderBytes", "ATokenOrder", "AEmbeddingGradBytes",
+                 "AEmbeddingGrad", "AAdamWBytes", "AAdamWCreate", "AAdamWSetStep", "AAdamWGetStep", "AAdamWStep",
+                 "AFreeAdamW"):
         getattr(lib, name).restype = ctypes.c_char_p
     lib.ADumpModel.argtypes = [ctypes.POINTER(ctypes.c_char_p), ctypes.c_void_p]
     lib.AFreeDMatrix.argtypes = [ctypes.c_void_p]
@@ -77,6 +79,18 @@ def _load_lib():
                                        ctypes.c_void_p, ctypes.c_void_p]
     lib.ANcclUniqueId.argtypes = [ctypes.c_void_p]
     lib.AInitNccl.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
+    ptr, i32, i64, f64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
+    lib.AEmbedding.argtypes = [ptr, i32, i64, i64, i64, ptr, i32, i64, i64, i64, i64, f64, ptr, i32, i64, i32, ptr]
+    lib.ATokenOrderBytes.argtypes = [i64, i64, ptr, ptr]
+    lib.ATokenOrder.argtypes = [ptr, i32, i64, i64, i64, i64, i64, ptr, ptr, i32, ptr]
+    lib.AEmbeddingGradBytes.argtypes = [i64, i64, i64, ptr]
+    lib.AEmbeddingGrad.argtypes = [ptr, i32, i64, i64, i64, ptr, i64, i64, f64, ptr, i32, i64, i32, ptr, i32, ptr]
+    lib.AAdamWBytes.argtypes = [ptr, i32, ptr, ptr]
+    lib.AAdamWCreate.argtypes = [ptr, i32, ptr, ptr, i32, ptr]
+    lib.AAdamWSetStep.argtypes = [ptr, i64, ptr]
+    lib.AAdamWGetStep.argtypes = [ptr, ptr, ptr]
+    lib.AAdamWStep.argtypes = [ptr, ptr, i32, i32, f64, ptr, ptr, ptr]
+    lib.AFreeAdamW.argtypes = [ptr]
     return lib
 
 

@@ -9,14 +9,15 @@
 #include <mutex>
 
 #include "../../include/arboretum_b200.h"
+#include "abi.h"
 #include "exchange.h"
 #include "garden.h"
 
 using namespace arb;
 
-namespace {
+namespace arb {
 
-thread_local std::string g_error;
+static thread_local std::string g_error;
 
 const char *fail(const std::exception &e) {
   g_error = e.what();
@@ -27,13 +28,9 @@ const char *fail(const char *msg) {
   return g_error.c_str();
 }
 
-#define ARB_TRY try {
-#define ARB_CATCH                                 \
-  return nullptr;                                 \
-  }                                               \
-  catch (const std::exception &e) { return fail(e); } \
-  catch (const char *e) { return fail(e); }       \
-  catch (...) { return fail("unknown error"); }
+}  // namespace arb
+
+namespace {
 
 // ---- NCCL through dlopen: the library has no link-time dependency on it -------
 struct NcclApi {

@@ -1,0 +1,105 @@
+// Operators on tables of learned rows (leaf values, embeddings): lookup, its gradient by sorted
+// tokens, and the AdamW step over many tensors.  All launchers enqueue on the given stream, never
+// synchronise and never allocate: outputs and scratch memory come from the caller, so that a call
+// can be captured into a CUDA graph.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <vector>
+
+#include "common.cuh"
+
+namespace arb {
+
+enum ElemType { kF32 = 0, kBF16 = 1, kF16 = 2 };
+inline size_t elem_size(int t) { return t == kF32 ? 4 : 2; }
+
+// Tokens of `bags` bags of `per_bag` each: token t of bag b is at[b * bag_stride + t * token_stride]
+// (strides in elements, int32 or int64).  A token outside [0, rows) is an empty slot.
+struct TokenView {
+  const void *at;
+  int bytes;  // 4 or 8
+  int64_t bags, per_bag, bag_stride, token_stride;
+  int64_t count() const { return bags * per_bag; }
+};
+
+struct LookupLaunch {
+  const void *table;
+  int type;
+  int64_t rows, dim, row_stride;
+  TokenView tokens;
+  float scale;
+  void *out;
+  int out_type;
+  int64_t out_stride;
+};
+void launch_lookup(const LookupLaunch &a, cudaStream_t s);
+
+// The tokens' order, in memory of the caller: for every row v of the table, the bags that name it
+// are bag[begin[v] .. begin[v + 1]), in a fixed order that only the tokens decide.
+struct TokenOrder {
+  unsigned *bag;    // count
+  unsigned *begin;  // rows + 1
+  int64_t count, rows;
+  TokenOrder(void *mem, int64_t count, int64_t rows);
+  static size_t bytes(int64_t count, int64_t rows);
+};
+size_t token_order_scratch(int64_t count, int64_t rows);
+void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, cudaStream_t s);
+
+struct LookupGradLaunch {
+  const void *grad;  // [bags][dim], rows grad_stride apart (0: the same row for every bag)
+  int type;
+  int64_t dim, grad_stride;
+  float scale;
+  void *out;  // [rows][dim]
+  int out_type;
+  int64_t out_stride;
+  bool accumulate;
+};
+size_t lookup_grad_scratch(int64_t count, int64_t rows, int64_t dim);
+void launch_lookup_grad(const LookupGradLaunch &a, const TokenOrder &o, void *scratch, cudaStream_t s);
+
+// ---- AdamW ---------------------------------------------------------------------------------
+constexpr int kMomentBlock = 128;  // elements of an 8-bit block; tensors' slots are padded to it
+constexpr int kAdamWChunk = 4096;  // elements a CTA takes at a time
+
+struct AdamWTensor {  // device table, one record a tensor
+  void *param;
+  long long n;
+  long long slot;  // first element in the flat moment buffers, a multiple of kMomentBlock
+  int type;
+  int vec;         // the parameter is 16-byte aligned
+};
+struct AdamWChunk {
+  int tensor;
+  int index;  // elements index * kAdamWChunk ..
+};
+struct AdamWState {  // device: the step count and the powers of the betas, advanced by the kernel
+  double beta1_t, beta2_t;
+  long long step;
+  unsigned done;   // CTAs of the running step that have finished
+  unsigned pad;
+};
+struct AdamWLaunch {
+  const AdamWTensor *tensors;
+  const AdamWChunk *chunks;
+  AdamWState *state;
+  void *moment1, *moment2;  // float, or e4m3 codes when bits == 8
+  float *scale1, *scale2;   // one a block, bits == 8
+  float *master;            // single-precision copy of the parameters in the slots' layout, or nullptr
+  int bits;
+  double beta1, beta2;
+  float eps;
+  double decay, lr;
+  const float *lr_device;    // takes lr's place when not nullptr
+  const float *grad_scale;   // device factor on every gradient, or nullptr
+  unsigned seed;
+  bool grad_f32;             // all gradients are fp32; else each has its parameter's type
+};
+// grads[i] belongs to tensor first_tensor + i (nullptr: that tensor is left as it is)
+void launch_adamw(const AdamWLaunch &a, const void *const *grads, const std::vector<int> &first_chunk,
+                  int n_tensors, cudaStream_t s);
+
+}  // namespace arb

@@ -157,6 +157,84 @@ const char *AReleaseCachedMemory(void);
  * thousand steps run for a millisecond. */
 const char *ASharedAtomicPeak(int steps, double *pair_updates_per_s);
 
+/* ---- operators on tables of learned rows (no counterpart in the reference) ------------------
+ * A forest of T trees with L leaves is a table of T * L rows, a row of the data set a bag of T
+ * tokens (ALeafTokens) and its prediction the sum of the rows they name.  The operators take
+ * tables of any width: lookup, its gradient, and the AdamW step on what is learned.
+ *
+ * All pointers below are device memory of `device` (an ordinal) unless said otherwise, `stream`
+ * is a cudaStream_t of that device (NULL = its default stream).  The calls only enqueue: no
+ * synchronisation, no allocation, so they can be captured into a CUDA graph; outputs and scratch
+ * memory belong to the caller and must live until the work is done.  Two calls that may overlap
+ * need scratch of their own.  Strides are in elements.
+ * Element types: 0 = fp32, 1 = bf16, 2 = fp16; an output has the input's type or fp32.
+ * Tokens are int32 (token_bytes 4) or int64 (8): token t of bag b is
+ * tokens[b * bag_stride + t * token_stride].  A token outside [0, rows) is an empty slot: it adds
+ * nothing and gets no gradient.  bags * per_bag and rows must be below 2^31 - 1. */
+
+/* out[b][:] = scale * sum over t of table[token(b, t)][:], summed in fp32, rounded once */
+const char *AEmbedding(const void *table, int type, int64_t rows, int64_t dim, int64_t row_stride,
+                       const void *tokens, int token_bytes, int64_t bags, int64_t per_bag,
+                       int64_t bag_stride, int64_t token_stride, double scale, void *out, int out_type,
+                       int64_t out_stride, int device, void *stream);
+/* Bytes that ATokenOrder needs for `count` = bags * per_bag tokens: the order itself (kept as long
+ * as it is used) and scratch (free after the call).  Both 256-byte aligned. */
+const char *ATokenOrderBytes(int64_t count, int64_t rows, int64_t *order_bytes, int64_t *scratch_bytes);
+/* Sorts the bags by the tokens that name them, for AEmbeddingGrad: stable, so equal tokens give
+ * equal orders. */
+const char *ATokenOrder(const void *tokens, int token_bytes, int64_t bags, int64_t per_bag, int64_t bag_stride,
+                        int64_t token_stride, int64_t rows, void *order, void *scratch, int device, void *stream);
+const char *AEmbeddingGradBytes(int64_t count, int64_t rows, int64_t dim, int64_t *scratch_bytes);
+/* out[v][:] = scale * sum of grad[b][:] over all (b, t) whose token is v (accumulate: added to out,
+ * rows no token names stay untouched; else they become zero).  `order` of the same count and rows.
+ * Summed in fp32 in a fixed order: the same inputs give the same bits.  grad_stride 0: one row for
+ * all bags. */
+const char *AEmbeddingGrad(const void *grad, int type, int64_t bags, int64_t dim, int64_t grad_stride,
+                           const void *order, int64_t count, int64_t rows, double scale, void *out, int out_type,
+                           int64_t out_stride, int accumulate, void *scratch, int device, void *stream);
+
+/* AdamW over many tensors in one launch.  Element i of tensor k has its moments at element
+ * slot[k] + i of the flat moment buffers; slots start at multiples of 128 in the order of the
+ * tensors: slot[0] = 0, slot[k + 1] = slot[k] + (size[k] rounded up to 128).  `length` is the end
+ * of the last slot.
+ *   state_bits 32: moment1, moment2 = fp32 first and second moment.
+ *   state_bits 8:  moment1, moment2 = e4m3 codes, scale1, scale2 = one fp32 power of two for every
+ *                  128 elements; moment2 holds the SQUARE ROOT of the second moment.  Rounded with
+ *                  a dither keyed by (element, step, seed).
+ * master: fp32 copy of the parameters in the slots' layout, or NULL; with it a step updates the
+ * copy and stores it rounded to each parameter's type. */
+typedef struct {
+  void *param;   /* contiguous */
+  int64_t size;  /* elements, may be 0 */
+  int type;      /* element type */
+} AAdamWParam;
+typedef struct {
+  double beta1, beta2, eps, weight_decay;
+  int state_bits;
+  unsigned seed;
+  void *moment1, *moment2;
+  float *scale1, *scale2;
+  float *master;
+} AAdamWConfig;
+/* params is host memory.  *length: elements of the moment buffers; *workspace_bytes: what the
+ * optimizer keeps beside them in device memory of the caller. */
+const char *AAdamWBytes(const AAdamWParam *params, int count, int64_t *length, int64_t *workspace_bytes);
+/* params and config are host memory and copied; the buffers they name and the workspace must
+ * outlive the handle.  Waits for the upload of the workspace.  The moments are taken as they are. */
+const char *AAdamWCreate(const AAdamWParam *params, int count, const AAdamWConfig *config, void *workspace,
+                         int device, VoidPointer *out);
+/* The step count, which lives in device memory (a captured step counts every replay): set, or
+ * read back after waiting for `stream`. */
+const char *AAdamWSetStep(VoidPointer optimizer, int64_t step, void *stream);
+const char *AAdamWGetStep(VoidPointer optimizer, int64_t *step, void *stream);
+/* One step.  grads: host array of `count` device pointers, contiguous gradients (NULL: that tensor
+ * and its moments stay as they are); all fp32 (grads_fp32 != 0) or each of its parameter's type.
+ * lr_device (fp32, NULL: lr) and grad_scale (fp32 factor on all gradients, NULL: 1) are read by the
+ * kernel.  Steps of one optimizer must be ordered on the device. */
+const char *AAdamWStep(VoidPointer optimizer, const void *const *grads, int count, int grads_fp32, double lr,
+                       const float *lr_device, const float *grad_scale, void *stream);
+const char *AFreeAdamW(VoidPointer optimizer);
+
 #ifdef __cplusplus
 }
 #endif

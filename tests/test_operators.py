@@ -1,0 +1,128 @@
+"""CPU-side checks of the operators on learned tables (lookup, its gradient, AdamW): every
+argument that a kernel would index with is refused before the device is touched, by the C entry
+points as an error string and by the Python functions as an exception."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import arboretum_b200 as arb
+
+LIB = arb.lib()
+P = ctypes.c_void_p(1 << 20)  # an address that is never followed: the checks come first
+
+
+def _message(e):
+    assert e is not None
+    return e.decode()
+
+
+def _embedding(**change):
+    a = dict(table=P, type=0, rows=10, dim=4, row_stride=4, tokens=P, token_bytes=4, bags=3, per_bag=2, bag_stride=2,
+             token_stride=1, scale=1.0, out=P, out_type=0, out_stride=4, device=0, stream=None)
+    a.update(change)
+    return LIB.AEmbedding(*a.values())
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(token_bytes=2), "int32 or int64"), (dict(bags=-1), "negative"), (dict(per_bag=-1), "negative"),
+    (dict(bags=1 << 20, per_bag=1 << 11), "2^31 - 2 tokens"), (dict(bags=1 << 62, per_bag=1 << 62), "2^31 - 2 tokens"),
+    (dict(rows=(1 << 31) - 1), "rows"), (dict(rows=-1), "rows"),
+    (dict(tokens=None), "tokens is NULL"), (dict(tokens=ctypes.c_void_p((1 << 20) + 2)), "aligned"),
+    (dict(table=None), "table is NULL"), (dict(table=ctypes.c_void_p((1 << 20) + 2)), "aligned"),
+    (dict(type=3), "element type"), (dict(type=-1), "element type"), (dict(out_type=1), "input's type or fp32"),
+    (dict(type=1, out_type=2), "input's type or fp32"), (dict(out=None), "out is NULL"),
+    (dict(out_stride=3), "overlap"), (dict(row_stride=-4), "stride"), (dict(row_stride=1 << 45), "stride"),
+    (dict(dim=-1), "width"), (dict(token_stride=1 << 60), "stride"),
+])
+def test_embedding_refuses(change, words):
+    assert words in _message(_embedding(**change))
+
+
+def test_nothing_to_do_touches_no_device():
+    assert _embedding(bags=0, tokens=None, out=None) is None
+    assert _embedding(dim=0, table=None, out=None) is None
+
+
+def test_order_and_gradient_refuse():
+    a, b = ctypes.c_int64(0), ctypes.c_int64(0)
+    assert LIB.ATokenOrderBytes(100, 10, ctypes.byref(a), ctypes.byref(b)) is None
+    assert a.value >= 4 * (100 + 11) and b.value > 0 and a.value % 256 == 0
+    assert "2^31 - 2 tokens" in _message(LIB.ATokenOrderBytes(1 << 31, 10, ctypes.byref(a), ctypes.byref(b)))
+    assert "NULL" in _message(LIB.ATokenOrderBytes(1, 10, None, ctypes.byref(b)))
+    assert "NULL" in _message(LIB.ATokenOrder(P, 4, 3, 1, 1, 0, 10, None, P, 0, None))
+    assert "aligned" in _message(LIB.ATokenOrder(P, 4, 3, 1, 1, 0, 10, ctypes.c_void_p(8), P, 0, None))
+    assert "rows" in _message(LIB.ATokenOrder(P, 4, 3, 1, 1, 0, 1 << 31, P, P, 0, None))
+
+    def grad(**change):
+        g = dict(grad=P, type=0, bags=3, dim=4, grad_stride=4, order=P, count=3, rows=10, scale=1.0, out=P, out_type=0,
+                 out_stride=4, accumulate=0, scratch=P, device=0, stream=None)
+        g.update(change)
+        return LIB.AEmbeddingGrad(*g.values())
+    for change, words in ((dict(order=None), "order is NULL"), (dict(grad=None), "grad is NULL"), (dict(out=None), "out is NULL"),
+                          (dict(out_stride=2), "overlap"), (dict(type=2, out_type=1), "input's type"), (dict(rows=-1), "rows"),
+                          (dict(count=-1), "negative"), (dict(grad_stride=-1), "stride"), (dict(scratch=ctypes.c_void_p(3)), "aligned"),
+                          (dict(bags=1 << 40), "bag count")):
+        assert words in _message(grad(**change)), change
+    assert grad(rows=0, out=None) is None and grad(dim=0, grad=None, out=None) is None
+
+
+def test_adamw_refuses():
+    from arboretum_b200.adamw import _Config, _Param
+    params = (_Param * 2)(_Param(1 << 20, 5, 0), _Param(1 << 21, 300, 1))
+    n, w = ctypes.c_int64(0), ctypes.c_int64(0)
+    assert LIB.AAdamWBytes(params, 2, ctypes.byref(n), ctypes.byref(w)) is None
+    assert n.value == 128 + 384 and w.value > 0
+    bad = (_Param * 1)(_Param(1 << 20, -5, 0))
+    assert "size" in _message(LIB.AAdamWBytes(bad, 1, ctypes.byref(n), ctypes.byref(w)))
+    assert "NULL" in _message(LIB.AAdamWBytes(None, 1, ctypes.byref(n), ctypes.byref(w)))
+    h = ctypes.c_void_p()
+
+    def create(table=params, count=2, workspace=P, **change):
+        c = dict(beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, state_bits=32, seed=0, moment1=1 << 20, moment2=1 << 20,
+                 scale1=None, scale2=None, master=None)
+        c.update(change)
+        return LIB.AAdamWCreate(table, count, ctypes.byref(_Config(*c.values())), workspace, 0, ctypes.byref(h))
+    for words, kw in (("state_bits", dict(state_bits=16)), ("betas", dict(beta1=1.0)), ("betas", dict(beta2=-0.1)),
+                      ("betas", dict(beta2=float("nan"))), ("eps", dict(eps=float("inf"))), ("eps", dict(weight_decay=-1.0)),
+                      ("moment", dict(moment1=None)), ("scale", dict(state_bits=8)), ("aligned", dict(moment2=(1 << 20) + 4)),
+                      ("NULL", dict(workspace=None)), ("aligned", dict(workspace=ctypes.c_void_p(16))),
+                      ("element type", dict(table=(_Param * 1)(_Param(1 << 20, 5, 7)), count=1)),
+                      ("NULL", dict(table=(_Param * 1)(_Param(None, 5, 0)), count=1)),
+                      ("aligned", dict(table=(_Param * 1)(_Param((1 << 20) + 2, 5, 0)), count=1))):
+        assert words in _message(create(**kw)), kw
+    assert "NULL" in _message(LIB.AAdamWStep(None, None, 0, 0, 1e-3, None, None, None))
+    assert "NULL" in _message(LIB.AAdamWSetStep(None, 0, None))
+    assert LIB.AFreeAdamW(None) is None
+
+
+def test_python_refusals():
+    t = torch.zeros(5, 4)
+    i = torch.zeros(3, dtype=torch.int64)
+    for error, words, call in (
+            (TypeError, "torch tensor", lambda: arb.embedding(i, np.zeros((5, 4), np.float32))),
+            (TypeError, "torch tensor", lambda: arb.embedding([1, 2], t)),
+            (TypeError, "float32", lambda: arb.embedding(i, t.double())),
+            (TypeError, "int32 or int64", lambda: arb.embedding(i.float(), t)),
+            (ValueError, "two dimensions", lambda: arb.embedding(i, t[0])),
+            (ValueError, "contiguous", lambda: arb.embedding(i, torch.zeros(4, 5).t())),
+            (ValueError, "bags x tokens", lambda: arb.embedding(i, t, pooled=True)),
+            (ValueError, "requires grad", lambda: arb.embedding(i, t.clone().requires_grad_())),
+            (ValueError, "CUDA", lambda: arb.embedding(i, t)),
+            (ValueError, "must have shape", lambda: arb.embedding_grad(torch.zeros(4, 4), i, 5)),
+            (ValueError, "must have shape", lambda: arb.embedding_grad(torch.zeros(3, 2, 4), i.view(3, 1), 5, pooled=True)),
+            (ValueError, "accumulate", lambda: arb.embedding_grad(torch.zeros(3, 4), i, 5, accumulate=True)),
+            (arb.ArboretumError, "rows", lambda: arb.embedding_grad(torch.zeros(3, 4), i, 1 << 31)),
+            (ValueError, "CUDA", lambda: arb.embedding_grad(torch.zeros(3, 4), i, 5)),
+            (arb.ArboretumError, "rows", lambda: arb.token_order(i, -1)),
+            (ValueError, "CUDA", lambda: arb.token_order(i, 5)),
+            (ValueError, "empty", lambda: arb.AdamW([])),
+            (ValueError, "not contiguous", lambda: arb.AdamW([torch.zeros(4, 5).t()])),
+            (ValueError, "share memory", lambda: arb.AdamW([t, t[2:]])),
+            (ValueError, "state_bits", lambda: arb.AdamW([t], state_bits=4)),
+            (TypeError, "float32", lambda: arb.AdamW([i])),
+            (TypeError, "lr", lambda: arb.AdamW([t], lr=torch.zeros(2))),
+            (ValueError, "CUDA", lambda: arb.AdamW([t]))):
+        with pytest.raises(error, match=words):
+            call()
