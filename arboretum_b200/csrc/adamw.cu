@@ -79,76 +79,130 @@ __device__ __forceinline__ Scalars scalars_of(const AdamWLaunch &a) {
   return c;
 }
 
-__device__ __forceinline__ float load_as(const void *p, int type, long long i) {
-  if (type == kF32) return static_cast<const float *>(p)[i];
-  if (type == kBF16) return to_f32(static_cast<const __nv_bfloat16 *>(p)[i]);
-  return to_f32(static_cast<const __half *>(p)[i]);
+// Eight neighbouring elements of a tensor of type T.  `vec`: the tensor starts on a 16-byte
+// boundary; the last elements of a tensor, and tensors that start elsewhere, go one by one.
+constexpr int kEach = 8;
+template <typename T>
+__device__ __forceinline__ void load_each(const T *p, long long i, int left, bool vec, float (&v)[kEach]) {
+  if (vec && left >= kEach) {
+    load_vec<T, kEach>(p + i, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) v[j] = j < left ? to_f32(p[i + j]) : 0.0f;
+  }
 }
-__device__ __forceinline__ void store_as(void *p, int type, long long i, float v) {
-  if (type == kF32) static_cast<float *>(p)[i] = v;
-  else if (type == kBF16) from_f32(v, static_cast<__nv_bfloat16 *>(p)[i]);
-  else from_f32(v, static_cast<__half *>(p)[i]);
+template <typename T>
+__device__ __forceinline__ void store_each(T *p, long long i, int left, bool vec, const float (&v)[kEach]) {
+  if (vec && left >= kEach) {
+    store_vec<T, kEach>(p + i, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (j < left) from_f32(v[j], p[i + j]);
+  }
+}
+__device__ __forceinline__ void load_typed(const void *p, int type, long long i, int left, bool vec, float (&v)[kEach]) {
+  if (type == kF32) load_each(static_cast<const float *>(p), i, left, vec, v);
+  else if (type == kBF16) load_each(static_cast<const __nv_bfloat16 *>(p), i, left, vec, v);
+  else load_each(static_cast<const __half *>(p), i, left, vec, v);
+}
+__device__ __forceinline__ void store_typed(void *p, int type, long long i, int left, bool vec, const float (&v)[kEach]) {
+  if (type == kF32) store_each(static_cast<float *>(p), i, left, vec, v);
+  else if (type == kBF16) store_each(static_cast<__nv_bfloat16 *>(p), i, left, vec, v);
+  else store_each(static_cast<__half *>(p), i, left, vec, v);
 }
 
-constexpr int kThreads = 128;  // a CTA step covers one 8-bit block
+constexpr int kThreads = 256;
+constexpr int kLanes = kMomentBlock / kEach;  // lanes that hold an 8-bit block: half a warp
 
+// A thread takes eight neighbouring elements: 16 bytes of a half-precision tensor, two accesses of 16
+// of a float one, 8 bytes of codes; half a warp holds a block, so its largest magnitude is found with
+// shuffles.  All loads of an element are issued before the first is used: 128 bytes a thread in flight.
 template <int BITS>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(AdamWLaunch a, const __grid_constant__ GradPointers grads,
                                                          int first_tensor, int first_chunk, int n_chunks, bool last) {
-  __shared__ unsigned warp_m[4], warp_r[4];
-  const Scalars c = scalars_of(a);
+  __shared__ Scalars shared_scalars;
+  if (threadIdx.x == 0) shared_scalars = scalars_of(a);
+  __syncthreads();
+  const Scalars c = shared_scalars;
   for (int k = blockIdx.x; k < n_chunks; k += gridDim.x) {
     const AdamWChunk ch = a.chunks[first_chunk + k];
     const AdamWTensor t = a.tensors[ch.tensor];
     const void *grad = grads.at[ch.tensor - first_tensor];
     if (grad == nullptr) continue;
     const int grad_type = a.grad_f32 ? kF32 : t.type;
+    const bool grad_vec = reinterpret_cast<unsigned long long>(grad) % 16 == 0, vec = t.vec != 0;
     const long long i1 = min(t.n, (ch.index + 1ll) * kAdamWChunk);
-    for (long long i0 = (long long)ch.index * kAdamWChunk; i0 < i1; i0 += kThreads) {
-      const long long i = i0 + threadIdx.x, at = t.slot + i;
-      const bool in = i < i1;
-      float m = 0.0f, v = 0.0f, root = 0.0f;
-      if (in) {
-        const float g = load_as(grad, grad_type, i) * c.grad_scale;
-        float p = a.master ? a.master[at] : load_as(t.param, t.type, i);
-        if (BITS == 8) {
-          m = decode(static_cast<unsigned char *>(a.moment1)[at], a.scale1[at / kMomentBlock]);
-          const float r = decode(static_cast<unsigned char *>(a.moment2)[at], a.scale2[at / kMomentBlock]);
-          v = r * r;
-        } else {
-          m = static_cast<float *>(a.moment1)[at];
-          v = static_cast<float *>(a.moment2)[at];
-        }
-        m = m * c.beta1 + g * c.one_beta1;
-        v = v * c.beta2 + (g * g) * c.one_beta2;
-        root = sqrtf(v);
-        p = p * c.keep - (m / (root * c.inv_root_bc2 + c.eps)) * c.step_size;
-        store_as(t.param, t.type, i, p);
-        if (a.master) a.master[at] = p;
-        if (BITS == 32) {
-          static_cast<float *>(a.moment1)[at] = m;
-          static_cast<float *>(a.moment2)[at] = v;
+    for (long long i0 = (long long)ch.index * kAdamWChunk; i0 < i1; i0 += kThreads * kEach) {
+      const long long i = i0 + threadIdx.x * kEach, at = t.slot + i;
+      const int left = int(min((long long)kEach, i1 - i));  // <= 0: nothing here, the lane only takes part in the shuffles
+      if (BITS == 32 && left <= 0) continue;
+      float p[kEach], g[kEach], m[kEach], v[kEach];
+      load_typed(grad, grad_type, i, left, grad_vec, g);
+      if (a.master) load_each(a.master, at, left, true, p);
+      else load_typed(t.param, t.type, i, left, vec, p);
+      if (BITS == 32) {
+        load_each(static_cast<float *>(a.moment1), at, left, true, m);
+        load_each(static_cast<float *>(a.moment2), at, left, true, v);
+      } else if (left > 0) {  // slots are whole blocks: the codes behind a tensor's end are there
+        const uint2 cm = *reinterpret_cast<const uint2 *>(static_cast<unsigned char *>(a.moment1) + at);
+        const uint2 cr = *reinterpret_cast<const uint2 *>(static_cast<unsigned char *>(a.moment2) + at);
+        const float s1 = a.scale1[at / kMomentBlock], s2 = a.scale2[at / kMomentBlock];
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) {
+          m[j] = decode((j < 4 ? cm.x : cm.y) >> (j % 4 * 8) & 255u, s1);
+          const float r = decode((j < 4 ? cr.x : cr.y) >> (j % 4 * 8) & 255u, s2);
+          v[j] = r * r;
         }
       }
-      if (BITS == 8) {
-        const unsigned mm = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(m)));
-        const unsigned mr = __reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(root)));
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) warp_m[threadIdx.x >> 5] = mm, warp_r[threadIdx.x >> 5] = mr;
-        __syncthreads();
-        const unsigned fm = scale_field(max(max(warp_m[0], warp_m[1]), max(warp_m[2], warp_m[3])));
-        const unsigned fr = scale_field(max(max(warp_r[0], warp_r[1]), max(warp_r[2], warp_r[3])));
-        if (in) {
-          const unsigned h = hash_bits((unsigned long long)at, c.step, a.seed);
-          const unsigned cm = encode(m, inv_scale_of(fm), h & 0xffffu) | (m < 0.0f ? 128u : 0u);
-          unsigned cr = encode(root, inv_scale_of(fr), h >> 16);
-          if (root > 0.0f) cr = max(cr, 1u);
-          static_cast<unsigned char *>(a.moment1)[at] = (unsigned char)cm;
-          static_cast<unsigned char *>(a.moment2)[at] = (unsigned char)cr;
+      unsigned top_m = 0, top_r = 0;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const float gj = g[j] * c.grad_scale;
+        m[j] = m[j] * c.beta1 + gj * c.one_beta1;
+        v[j] = v[j] * c.beta2 + (gj * gj) * c.one_beta2;
+        const float root = sqrtf(v[j]);
+        p[j] = p[j] * c.keep - (m[j] / (root * c.inv_root_bc2 + c.eps)) * c.step_size;
+        if (BITS == 8) {
+          v[j] = root;
+          if (j < left) {
+            top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+            top_r = max(top_r, __float_as_uint(root) & 0x7FFFFFFFu);
+          }
         }
-        if (threadIdx.x == 0) {
-          a.scale1[at / kMomentBlock] = scale_of(fm);
-          a.scale2[at / kMomentBlock] = scale_of(fr);
+      }
+      store_typed(t.param, t.type, i, left, vec, p);
+      if (a.master) store_each(a.master, at, left, true, p);
+      if (BITS == 32) {
+        store_each(static_cast<float *>(a.moment1), at, left, true, m);
+        store_each(static_cast<float *>(a.moment2), at, left, true, v);
+      } else {
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) {
+          top_m = max(top_m, __shfl_xor_sync(0xffffffffu, top_m, o));
+          top_r = max(top_r, __shfl_xor_sync(0xffffffffu, top_r, o));
+        }
+        if (left > 0) {
+          const unsigned fm = scale_field(top_m), fr = scale_field(top_r);
+          const float im = inv_scale_of(fm), ir = inv_scale_of(fr);
+          uint2 cm = make_uint2(0u, 0u), cr = make_uint2(0u, 0u);
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) {
+            if (j < left) {
+              const unsigned h = hash_bits((unsigned long long)(at + j), c.step, a.seed);
+              const unsigned em = encode(m[j], im, h & 0xffffu) | (m[j] < 0.0f ? 128u : 0u);
+              unsigned er = encode(v[j], ir, h >> 16);
+              if (v[j] > 0.0f) er = max(er, 1u);
+              (j < 4 ? cm.x : cm.y) |= em << (j % 4 * 8);
+              (j < 4 ? cr.x : cr.y) |= er << (j % 4 * 8);
+            }
+          }
+          *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(a.moment1) + at) = cm;
+          *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(a.moment2) + at) = cr;
+          if (threadIdx.x % kLanes == 0) {
+            a.scale1[at / kMomentBlock] = scale_of(fm);
+            a.scale2[at / kMomentBlock] = scale_of(fr);
+          }
         }
       }
     }
@@ -177,7 +231,7 @@ void launch_adamw(const AdamWLaunch &a, const void *const *grads, const std::vec
     std::copy(grads + t0, grads + t1, g.at);
     const int chunks = first_chunk[t1] - first_chunk[t0];
     if (chunks > 0 || last) {  // a step without elements still counts
-      const int grid = std::max(1, std::min(chunks, device_sm_count() * 16));
+      const int grid = std::max(1, std::min(chunks, device_sm_count() * 8));
       if (a.bits == 8) adamw_kernel<8><<<grid, kThreads, 0, s>>>(a, g, t0, first_chunk[t0], chunks, last);
       else adamw_kernel<32><<<grid, kThreads, 0, s>>>(a, g, t0, first_chunk[t0], chunks, last);
       ARB_CUDA(cudaGetLastError());
