@@ -42,6 +42,11 @@ struct TokenOrder {
   unsigned *bag;    // count
   unsigned *begin;  // rows + 1
   int64_t count, rows;
+  // rows named by more than `piece` bags: (row, number of its first piece), and how many there are:
+  // the rows in the upper half of *counts, their pieces in the lower one
+  unsigned piece;
+  uint2 *frequent;
+  unsigned long long *counts;
   TokenOrder(void *mem, int64_t count, int64_t rows);
   static size_t bytes(int64_t count, int64_t rows);
 };
