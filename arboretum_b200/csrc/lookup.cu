@@ -6,6 +6,8 @@
 // Sums are held in fp32 and rounded once to the output's type.  No floating-point atomics: the
 // gradient of a row is summed by its owner over the sorted tokens, in an order that only the tokens
 // decide, so two calls on the same tokens give the same bits.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "operators.h"
@@ -38,7 +40,7 @@ struct LaneShape {
 constexpr int kLookupThreads = 256;
 template <typename T, typename O, int VEC, int U, int K>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupLaunch a, LaneShape sh, int vecs, int chunks) {
-  __shared__ float part[K > 1 ? kLookupThreads * U * VEC : 1];  // one token a bag: nothing to join
+  __shared__ float part[kLookupThreads * U * VEC];
   const int tx = 1 << sh.tx_bits, ly = 1 << sh.ly_bits;
   const int lane = threadIdx.x & (tx - 1), slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
   const int group = threadIdx.x >> (sh.tx_bits + sh.ly_bits), groups = kLookupThreads >> (sh.tx_bits + sh.ly_bits);
@@ -56,27 +58,21 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupLaunch a, 
         long long row[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) row[k] = k0 + k * ly < a.tokens.per_bag ? row_at(a.tokens, a.rows, b, k0 + k * ly) : -1;
-        float v[K][U][VEC];
+        Vec<T, VEC> v[K][U];
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            if (row[k] >= 0 && c0 + u * tx < vecs) {
-              load_vec<T, VEC>(table + row[k] * a.row_stride + (long long)(c0 + u * tx) * VEC, v[k][u]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) v[k][u][j] = 0.0f;
-            }
+            if (row[k] >= 0 && c0 + u * tx < vecs) v[k][u].load(table + row[k] * a.row_stride + (long long)(c0 + u * tx) * VEC);
+            else v[k][u].clear();
           }
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) sum[u][j] += v[k][u][j];
+          for (int u = 0; u < U; ++u) v[k][u].add_to(sum[u]);
       }
     }
-    if (K > 1 && ly > 1) {
+    if (ly > 1) {
       __syncthreads();
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -110,6 +106,96 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupLaunch a, 
   }
 }
 
+// One token a bag: a row is copied, scaled, from the table to the output.  A group of tx lanes takes a
+// run of tx * U vectors of one row.
+template <typename T, typename O, int VEC, int U>
+__global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunch a, int tx_bits, int vecs, int chunks) {
+  const int tx = 1 << tx_bits, lane = threadIdx.x & (tx - 1);
+  const long long b = blockIdx.x * (long long)(kLookupThreads >> tx_bits) + (threadIdx.x >> tx_bits);
+  if (b >= a.tokens.bags) return;
+  const long long row = row_at(a.tokens, a.rows, b, 0);
+  const T *from = static_cast<const T *>(a.table) + row * a.row_stride;
+  O *out = static_cast<O *>(a.out) + b * a.out_stride;
+  for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+    const int c0 = chunk * (tx * U) + lane;
+    Vec<T, VEC> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].clear();
+      if (row >= 0 && c0 + u * tx < vecs) v[u].load(from + (long long)(c0 + u * tx) * VEC);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[VEC];
+      v[u].get(x);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) x[j] *= a.scale;
+      if (c0 + u * tx < vecs) store_vec<O, VEC>(out + (long long)(c0 + u * tx) * VEC, x);
+    }
+  }
+}
+
+// Bags of many tokens over a narrow table that fits into shared memory (the leaf values of a forest):
+// every CTA holds the whole table and a thread the sums of two neighbouring bags, whose tokens lie
+// side by side in memory, tree after tree.  The tokens are all that is read from device memory; the
+// table's values come from shared memory, where 32 random words cost a few cycles and a gather
+// through the first-level cache one for every line it touches.
+constexpr int kTableThreads = 1024;
+template <typename T, typename O, typename I, int DIM>
+__global__ void __launch_bounds__(kTableThreads) lookup_table_kernel(LookupLaunch a, bool paired) {
+  extern __shared__ float values[];  // [rows][DIM], and a row of zeros for empty slots
+  const int rows = int(a.rows);
+  for (int i = threadIdx.x; i < (rows + 1) * DIM; i += kTableThreads) {
+    const int r = i / DIM, d = i - r * DIM;
+    values[i] = r < rows ? to_f32(static_cast<const T *>(a.table)[(long long)r * a.row_stride + d]) : 0.0f;
+  }
+  __syncthreads();
+  constexpr int K = 8;  // tokens of a bag in flight
+  const int per_bag = int(a.tokens.per_bag);
+  const long long step = a.tokens.token_stride;
+  for (long long b = (blockIdx.x * (long long)kTableThreads + threadIdx.x) * 2; b < a.tokens.bags;
+       b += (long long)gridDim.x * kTableThreads * 2) {
+    const bool two = b + 1 < a.tokens.bags;
+    const I *at = static_cast<const I *>(a.tokens.at) + b * a.tokens.bag_stride;
+    float sum[2][DIM];
+#pragma unroll
+    for (int d = 0; d < DIM; ++d) sum[0][d] = sum[1][d] = 0.0f;
+    for (int k0 = 0; k0 < per_bag; k0 += K) {
+      I tok[K][2];
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        tok[k][0] = tok[k][1] = -1;
+        if (k0 + k < per_bag) {
+          const I *p = at + (k0 + k) * step;
+          if (paired && two) {  // one access for both
+            struct alignas(2 * sizeof(I)) Both { I v[2]; };
+            const Both both = *reinterpret_cast<const Both *>(p);
+            tok[k][0] = both.v[0], tok[k][1] = both.v[1];
+          } else {
+            tok[k][0] = p[0];
+            if (two) tok[k][1] = p[a.tokens.bag_stride];
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = tok[k][e] >= 0 && tok[k][e] < a.rows ? int(tok[k][e]) : rows;
+#pragma unroll
+          for (int d = 0; d < DIM; ++d) sum[e][d] += values[r * DIM + d];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (e == 0 || two) {
+        O *out = static_cast<O *>(a.out) + (b + e) * a.out_stride;
+#pragma unroll
+        for (int d = 0; d < DIM; ++d) from_f32(sum[e][d] * a.scale, out[d]);
+      }
+  }
+}
+
 // ---- the sort --------------------------------------------------------------------------------
 // Least-significant-digit radix sort of (token, bag): every pass counts the digits of each tile,
 // turns the counts into positions (digit by digit, tile by tile) and moves the pairs, keeping the
@@ -130,21 +216,20 @@ struct SortPass {
   bool first, by_slot;     // by_slot: pairs are numbered slot after slot (neighbouring bags lie side by side)
 };
 
-template <typename I>
 __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsigned &key, unsigned &bag) {
   if (!p.first) {
     key = p.key_in[i];
     bag = p.bag_in[i];
     return;
   }
-  const long long b = p.by_slot ? i % p.tokens.bags : i / p.tokens.per_bag;
-  const long long k = p.by_slot ? i / p.tokens.bags : i - b * p.tokens.per_bag;
-  const long long tok = token_at<I>(p.tokens, b, k);
-  key = tok >= 0 && tok < p.rows ? unsigned(tok) : unsigned(p.rows);
+  const unsigned at = unsigned(i), by = unsigned(p.by_slot ? p.tokens.bags : p.tokens.per_bag);  // both below 2^31
+  const unsigned hi = by == 1 ? at : at / by, lo = at - hi * by;
+  const long long b = p.by_slot ? lo : hi, k = p.by_slot ? hi : lo;
+  const long long row = row_at(p.tokens, p.rows, b, k);
+  key = row >= 0 ? unsigned(row) : unsigned(p.rows);
   bag = unsigned(b);
 }
 
-template <typename I>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
   __shared__ unsigned cnt[kDigits];
   for (int i = threadIdx.x; i < kDigits; i += kSortThreads) cnt[i] = 0;
@@ -154,7 +239,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
     const long long i = t0 + j * kSortThreads + threadIdx.x;
     if (i < p.n) {
       unsigned key, bag;
-      sort_pair<I>(p, i, key, bag);
+      sort_pair(p, i, key, bag);
       atomicAdd(&cnt[(key >> p.shift) & (kDigits - 1)], 1u);
     }
   }
@@ -198,7 +283,6 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(SortPass p) {
   if (threadIdx.x == 0) p.totals[blockIdx.x] = run;
 }
 
-template <typename I>
 __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortPass p) {
   __shared__ unsigned warp_cnt[kSortWarps][kDigits];
   __shared__ unsigned base[kDigits];
@@ -218,7 +302,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortPass p) {
     const long long i = w0 + j * 32 + lane;
     const bool in = i < p.n;
     key[j] = bag[j] = rank[j] = 0;
-    if (in) sort_pair<I>(p, i, key[j], bag[j]);
+    if (in) sort_pair(p, i, key[j], bag[j]);
     const unsigned digit = in ? (key[j] >> p.shift) & (kDigits - 1) : kDigits;
     const unsigned same = __match_any_sync(0xffffffffu, digit);
     const unsigned below = __popc(same & ((1u << lane) - 1u));
@@ -294,6 +378,7 @@ struct GradLanes {
   int tx_bits;      // lanes across the columns
   int ly_row_bits;  // lanes along the bags of a row
   int ly_item_bits; // ... of a piece of a frequent row
+  int rows_per_group;
 };
 
 constexpr int kGradThreads = 256;
@@ -302,7 +387,7 @@ constexpr int kGradThreads = 256;
 template <typename T, int VEC, int U>
 __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsigned *__restrict__ bag, unsigned p0, unsigned p1,
                                          int slice, int ly, int tx, int c0, int vecs, float (&sum)[U][VEC]) {
-  constexpr int K = U * VEC >= 16 ? 2 : 4;  // bags whose loads are in flight together
+  constexpr int K = U > 1 ? 4 : 8;  // bags whose loads are in flight together
   const T *grad = static_cast<const T *>(a.grad);
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -312,24 +397,18 @@ __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsign
     long long row[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) row[k] = p + k * ly < p1 ? (long long)bag[p + k * ly] * a.grad_stride : -1;
-    float v[K][U][VEC];
+    Vec<T, VEC> v[K][U];
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (row[k] >= 0 && c0 + u * tx < vecs) {
-          load_vec<T, VEC>(grad + row[k] + (long long)(c0 + u * tx) * VEC, v[k][u]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) v[k][u][j] = 0.0f;
-        }
+        if (row[k] >= 0 && c0 + u * tx < vecs) v[k][u].load(grad + row[k] + (long long)(c0 + u * tx) * VEC);
+        else v[k][u].clear();
       }
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[u][j] += v[k][u][j];
+      for (int u = 0; u < U; ++u) v[k][u].add_to(sum[u]);
   }
   for (int o = tx; o < tx * ly; o <<= 1)  // the slices of a group are neighbouring lanes of a warp
 #pragma unroll
@@ -361,8 +440,7 @@ __device__ __forceinline__ void write_row(const LookupGradLaunch &a, long long r
 }
 
 // CTAs below item_blocks sum the pieces of frequent rows into `partial` [piece][dim]; the others
-// take the rows of the table in order: zeros where no bag names a row, else its sum.  (The sums
-// behind the loops are uniform over a warp: lanes without a row of their own go through them empty.)
+// take the rows of the table in order: zeros where no bag names a row, else its sum.  
 template <typename T, typename O, int VEC, int U>
 __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLaunch a, TokenOrder o, GradLanes sh, int vecs,
                                                                    int chunks, unsigned item_blocks, float *partial) {
@@ -404,18 +482,43 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
     }
     return;
   }
+  // A warp takes rows_per_warp rows a lane group, and reads where their bags begin in one access: it
+  // knows the untouched rows at once, and their zeros are stores that wait for nothing.
   const int ly = 1 << sh.ly_row_bits, slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
   const int bits = sh.tx_bits + sh.ly_row_bits;
-  const long long row = (blockIdx.x - item_blocks) * (long long)(kGradThreads >> bits) + (threadIdx.x >> bits);
-  unsigned p0 = 0, p1 = 0;
-  if (row < o.rows) p0 = o.begin[row], p1 = o.begin[row + 1];
-  const bool mine = row < o.rows && p1 - p0 <= o.piece && !(a.accumulate && p0 == p1);
-  if (!mine) p1 = p0;
+  const int groups = 32 >> bits, group = (threadIdx.x & 31) >> bits;  // of a warp
+  const long long warp = (blockIdx.x - item_blocks) * (long long)(kGradThreads / 32) + threadIdx.x / 32;
+  const int span = groups * sh.rows_per_group;  // at most 32
+  const long long row0 = warp * span;
+  unsigned my_begin = 0, my_end = 0;
+  if ((threadIdx.x & 31) < span && row0 + (threadIdx.x & 31) < o.rows) {
+    my_begin = o.begin[row0 + (threadIdx.x & 31)];
+    my_end = o.begin[row0 + (threadIdx.x & 31) + 1];
+  }
+  const unsigned touched = __ballot_sync(0xffffffffu, my_begin != my_end);
   for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
     const int c0 = chunk * (tx * U) + lane;
-    float sum[U][VEC];
-    sum_bags<T, VEC, U>(a, o.bag, p0, p1, slice, ly, tx, c0, vecs, sum);
-    if (mine && slice == 0) write_row<O, VEC, U>(a, row, c0, tx, vecs, sum);
+    if (!a.accumulate && slice == 0) {
+      float zero[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) zero[j] = 0.0f;
+      for (int r = group; r < span; r += groups) {
+        if ((touched >> r & 1u) || row0 + r >= o.rows) continue;
+        O *out = static_cast<O *>(a.out) + (row0 + r) * a.out_stride;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + u * tx < vecs) store_vec<O, VEC>(out + (long long)(c0 + u * tx) * VEC, zero);
+      }
+    }
+    for (int r0 = 0; r0 < span; r0 += groups) {
+      if ((touched >> r0 & ((groups == 32 ? 0u : 1u << groups) - 1u)) == 0) continue;  // the same for the whole warp
+      const int r = r0 + group;
+      const unsigned p0 = __shfl_sync(0xffffffffu, my_begin, r), p1 = __shfl_sync(0xffffffffu, my_end, r);
+      const bool mine = p0 != p1 && p1 - p0 <= o.piece;
+      float sum[U][VEC];
+      sum_bags<T, VEC, U>(a, o.bag, p0, mine ? p1 : p0, slice, ly, tx, c0, vecs, sum);
+      if (mine && slice == 0) write_row<O, VEC, U>(a, row0 + r, c0, tx, vecs, sum);
+    }
   }
 }
 
@@ -438,6 +541,169 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGr
         for (int j = 0; j < VEC; ++j) sum[0][j] += at[j];
       }
       write_row<O, VEC, 1>(a, f.x, c, 0, vecs, sum);
+    }
+  }
+}
+
+// ---- the sort of a batch in one launch -------------------------------------------------------
+// Up to 131072 tokens are sorted by one cluster of at most eight CTAs: the pairs stay in shared
+// memory, a pass exchanges digit counts and moves the pairs through distributed shared memory, and
+// the rows' first positions and the frequent rows come out of the same launch.  (The general sort
+// takes three launches a pass and leaves the device to a few tiles at these sizes: 16384 tokens over
+// 131072 rows took 109 us.)
+namespace cg = cooperative_groups;
+constexpr int kClusterThreads = 1024, kMostClusterBits = 9, kMostClusterDigits = 1 << kMostClusterBits;
+constexpr int kLongGaps = 512;
+
+struct ClusterSortMemory {
+  unsigned short warp_cnt[kClusterThreads / 32][kMostClusterDigits];
+  unsigned cta_cnt[kMostClusterDigits];
+  unsigned base[kMostClusterDigits];
+  unsigned warp_sum[kClusterThreads / 32];
+  unsigned n_long;
+  uint2 long_gap[kLongGaps];  // rows first .. last that begin at long_at
+  unsigned long_at[kLongGaps];
+  unsigned last_key;
+};
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass p, TokenOrder o, int digit_bits, int passes) {
+  extern __shared__ __align__(16) unsigned char raw[];
+  uint2 *pair = reinterpret_cast<uint2 *>(raw);
+  ClusterSortMemory &m = *reinterpret_cast<ClusterSortMemory *>(raw + sizeof(uint2) * kClusterThreads * ITEMS);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = int(cluster.block_rank()), ctas = int(cluster.num_blocks());
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  constexpr int kSpan = kClusterThreads * ITEMS;  // pairs of a CTA
+  const int digits = 1 << digit_bits;
+  const int at0 = w * (ITEMS * 32) + lane;  // this thread's pairs: at0, at0 + 32, ..
+  unsigned key[ITEMS], bag[ITEMS], rank_in[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const long long i = (long long)rank * kSpan + at0 + j * 32;
+    key[j] = 0xffffffffu;  // behind everything, empty slots included: it comes after them and digits are stable
+    bag[j] = 0;
+    if (i < p.n) sort_pair(p, i, key[j], bag[j]);
+  }
+  if (rank == 0 && tid == 0) *o.counts = 0;
+  if (tid == 0) m.n_long = 0;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * digit_bits;
+    for (int i = tid; i < (kClusterThreads / 32) * kMostClusterDigits / 2; i += kClusterThreads)
+      reinterpret_cast<unsigned *>(&m.warp_cnt[0][0])[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const unsigned digit = (key[j] >> shift) & (digits - 1);
+      const unsigned same = __match_any_sync(0xffffffffu, digit);
+      const unsigned below = __popc(same & ((1u << lane) - 1u));
+      rank_in[j] = m.warp_cnt[w][digit] + below;
+      __syncwarp();
+      if (below == 0) m.warp_cnt[w][digit] += (unsigned short)__popc(same);
+      __syncwarp();
+    }
+    __syncthreads();
+    if (tid < digits) {
+      unsigned run = 0;
+      for (int i = 0; i < kClusterThreads / 32; ++i) {
+        const unsigned c = m.warp_cnt[i][tid];
+        m.warp_cnt[i][tid] = (unsigned short)run;  // at most kSpan - 1 = 16383
+        run += c;
+      }
+      m.cta_cnt[tid] = run;
+    }
+    cluster.sync();  // the counts are there, and every CTA holds its pairs in registers
+    unsigned before = 0, total = 0;
+    if (tid < digits)
+      for (int r = 0; r < ctas; ++r) {
+        const unsigned c = cluster.map_shared_rank(m.cta_cnt, r)[tid];
+        if (r < rank) before += c;
+        total += c;
+      }
+    // exclusive sum of the digits' totals over the CTA's first warps
+    unsigned x = total;
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) m.warp_sum[w] = x;
+    __syncthreads();
+    unsigned ahead = 0;
+    for (int i = 0; i < w && i < kMostClusterDigits / 32; ++i) ahead += m.warp_sum[i];
+    if (tid < digits) m.base[tid] = ahead + x - total + before;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const unsigned digit = (key[j] >> shift) & (digits - 1);
+      const unsigned to = m.base[digit] + m.warp_cnt[w][digit] + rank_in[j];
+      cluster.map_shared_rank(pair, int(to / kSpan))[to % kSpan] = make_uint2(key[j], bag[j]);
+    }
+    cluster.sync();
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const uint2 v = pair[at0 + j * 32];
+      key[j] = v.x;
+      bag[j] = v.y;
+    }
+  }
+  if (tid == 0) m.last_key = pair[kSpan - 1].x;
+  cluster.sync();
+  // a position fills the rows behind its predecessor's token up to its own; gaps that would keep one
+  // warp busy for long are left to the whole cluster
+  const long long longest = max(256ll, p.rows / (kLongGaps / 2));
+  const unsigned first_prev = rank == 0 ? 0xffffffffu : *cluster.map_shared_rank(&m.last_key, rank - 1);
+  for (int j = 0; j < ITEMS; ++j) {
+    const int at = at0 + j * 32;
+    const long long q = (long long)rank * kSpan + at;
+    const uint2 mine = pair[at];
+    const unsigned k = mine.x, prev = at == 0 ? first_prev : pair[at - 1].x;
+    long long lo = 0, hi = -1, lo_end = 0, hi_end = -1;
+    if (q < p.n) {
+      o.bag[q] = mine.y;
+      lo = q == 0 ? 0 : (long long)prev + 1;
+      hi = k;
+      if (q == p.n - 1) lo_end = (long long)k + 1, hi_end = p.rows;
+    }
+    for (int part = 0; part < 2; ++part) {
+      const long long l0 = part ? lo_end : lo, h0 = part ? hi_end : hi;
+      bool wide = h0 - l0 >= longest;
+      if (wide) {
+        const unsigned slot = atomicAdd(&m.n_long, 1u);
+        if (slot < kLongGaps) {  // always: gaps are disjoint, so fewer than kLongGaps / 2 are that long
+          m.long_gap[slot] = make_uint2(unsigned(l0), unsigned(h0));
+          m.long_at[slot] = unsigned(q + part);
+        }
+      }
+      unsigned todo = __ballot_sync(0xffffffffu, l0 <= h0 && !wide);
+      while (todo) {
+        const int src = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const unsigned l = unsigned(__shfl_sync(0xffffffffu, l0, src)), h = unsigned(__shfl_sync(0xffffffffu, h0, src));
+        const unsigned value = unsigned(__shfl_sync(0xffffffffu, q, src)) + part;
+        for (unsigned v = l + lane; v <= h; v += 32) o.begin[v] = value;
+      }
+    }
+  }
+  cluster.sync();
+  for (int r = 0; r < ctas; ++r) {
+    const ClusterSortMemory &other = *cluster.map_shared_rank(&m, r);
+    const unsigned n_long = other.n_long;
+    for (unsigned g = 0; g < n_long; ++g) {
+      const uint2 gap = other.long_gap[g];
+      const unsigned value = other.long_at[g];
+      for (long long v = (long long)gap.x + rank * kClusterThreads + tid; v <= gap.y; v += ctas * kClusterThreads)
+        o.begin[v] = value;
+    }
+  }
+  __threadfence();
+  cluster.sync();  // begin is complete; nobody reads another CTA's shared memory after this
+  for (int j = 0; j < ITEMS; ++j) {
+    const int at = at0 + j * 32;
+    const long long q = (long long)rank * kSpan + at;
+    const unsigned k = pair[at].x, prev = at == 0 ? first_prev : pair[at - 1].x;
+    if (q < p.n && k < p.rows && (q == 0 || prev != k)) {
+      const unsigned len = __ldcg(o.begin + k + 1) - unsigned(q);
+      if (len > o.piece) add_frequent(o, k, len);
     }
   }
 }
@@ -494,10 +760,10 @@ int log2_floor(int64_t v) {
   return b;
 }
 
-// Elements a thread may move in one access: the widest of 16 bytes, 4 bytes and one element that
+// Elements a thread may move in one access: the widest of 16, 8 and 4 bytes and one element that
 // the columns, the distances of the rows and both starts allow.
 int vec_of(int type, int64_t dim, const void *p, int64_t stride, const void *q, int out_type, int64_t out_stride) {
-  const int widths[2] = {int(16 / elem_size(type)), int(4 / elem_size(type))};
+  const int widths[3] = {int(16 / elem_size(type)), int(8 / elem_size(type)), int(4 / elem_size(type))};
   for (int v : widths) {
     const auto fits = [&](const void *at, int t, int64_t st) {
       const size_t bytes = std::min<size_t>(16, v * elem_size(t));
@@ -512,15 +778,15 @@ template <typename T, typename O, int VEC>
 void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   const int64_t vecs = a.dim / VEC;
   ARB_CHECK(vecs <= (int64_t(1) << 30), "rows of more than 2^30 vectors");
-  const bool pooled = a.tokens.per_bag > 1;
+  const bool pooled = a.tokens.per_bag != 1;
   const int u = !pooled && vecs >= 256 ? 4 : 1;
   LaneShape sh;
-  // lanes across the columns: enough for the row, at most a CTA
+  // lanes across the columns: enough for the row, at most half a CTA
   sh.tx_bits = std::min(7, log2_floor(std::max<int64_t>(1, (vecs + u - 1) / u * 2 - 1)));
   // lanes along the tokens: where a bag's tokens lie side by side a narrow group reads them as one
   // line, and where the bags alone do not fill the device they share the loop
   const int64_t threads_wanted = int64_t(device_sm_count()) * 1024;
-  int64_t have = a.tokens.bags * ((vecs + u - 1) / u);
+  const int64_t have = a.tokens.bags * vecs;
   const bool side_by_side = std::abs(a.tokens.token_stride) < std::abs(a.tokens.bag_stride);
   sh.ly_bits = 0;
   while (pooled && sh.tx_bits + sh.ly_bits < 8 && (int64_t(4) << sh.ly_bits) < a.tokens.per_bag &&
@@ -529,9 +795,45 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   const int groups = kLookupThreads >> (sh.tx_bits + sh.ly_bits);
   const int chunks = int((vecs + (int64_t(u) << sh.tx_bits) - 1) / (int64_t(u) << sh.tx_bits));
   const dim3 grid(unsigned((a.tokens.bags + groups - 1) / groups), unsigned(std::min(chunks, 65535)));
-  if (pooled) lookup_kernel<T, O, VEC, 1, 4><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
-  else if (u == 4) lookup_kernel<T, O, VEC, 4, 1><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
-  else lookup_kernel<T, O, VEC, 1, 1><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  if (pooled) lookup_kernel<T, O, VEC, 1, 8><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  else if (u == 4) lookup_rows_kernel<T, O, VEC, 4><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
+  else lookup_rows_kernel<T, O, VEC, 1><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
+}
+
+constexpr size_t kMostTableBytes = 200 << 10;  // of shared memory, one CTA an SM
+
+template <typename T, typename O, typename I, int DIM>
+void lookup_table_with(const LookupLaunch &a, cudaStream_t s) {
+  static bool ready[kMaxDevices] = {};
+  const int dev = current_device();
+  if (!ready[dev]) {
+    ARB_CUDA(cudaFuncSetAttribute(lookup_table_kernel<T, O, I, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  int(kMostTableBytes)));
+    ready[dev] = true;
+  }
+  const size_t smem = size_t(a.rows + 1) * DIM * sizeof(float);
+  const bool paired = a.tokens.bag_stride == 1 && a.tokens.token_stride % 2 == 0 &&
+                      reinterpret_cast<uintptr_t>(a.tokens.at) % (2 * sizeof(I)) == 0;
+  lookup_table_kernel<T, O, I, DIM><<<device_sm_count(), kTableThreads, smem, s>>>(a, paired);
+}
+
+template <typename T, typename O>
+bool lookup_table(const LookupLaunch &a, cudaStream_t s) {
+  // Only where the bags of one slot lie next to one another, the table fits, and the lookups are
+  // many times the words every SM has to copy first.
+  const TokenView &t = a.tokens;
+  if (a.dim > 3 || t.per_bag < 2 || std::abs(t.bag_stride) >= std::abs(t.token_stride) ||
+      size_t(a.rows + 1) * size_t(a.dim) * sizeof(float) > kMostTableBytes ||
+      t.count() < 4 * a.rows * device_sm_count())
+    return false;
+#define ARB_DIM(D)                                                     \
+  if (a.dim == D) {                                                    \
+    if (t.bytes == 4) lookup_table_with<T, O, int32_t, D>(a, s);       \
+    else lookup_table_with<T, O, int64_t, D>(a, s);                    \
+  }
+  ARB_DIM(1) ARB_DIM(2) ARB_DIM(3)
+#undef ARB_DIM
+  return true;
 }
 
 }  // namespace
@@ -539,9 +841,11 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
 void launch_lookup(const LookupLaunch &a, cudaStream_t s) {
   if (a.tokens.bags == 0 || a.dim == 0) return;
   const int vec = vec_of(a.type, a.dim, a.table, a.row_stride, a.out, a.out_type, a.out_stride);
-#define ARB_CALL(T, O)                                              \
-  if (vec * sizeof(T) == 16) lookup_with<T, O, 16 / sizeof(T)>(a, s); \
-  else if (vec > 1) lookup_with<T, O, 4 / sizeof(T)>(a, s);         \
+#define ARB_CALL(T, O)                                                      \
+  if (lookup_table<T, O>(a, s)) {}                                          \
+  else if (vec * sizeof(T) == 16) lookup_with<T, O, 16 / sizeof(T)>(a, s);  \
+  else if (vec * sizeof(T) == 8) lookup_with<T, O, 8 / sizeof(T)>(a, s);    \
+  else if (vec > 1) lookup_with<T, O, 4 / sizeof(T)>(a, s);                 \
   else lookup_with<T, O, 1>(a, s)
   ARB_BY_TYPE(a.type, a.out_type, ARB_CALL);
 #undef ARB_CALL
@@ -575,8 +879,48 @@ TokenOrder::TokenOrder(void *mem, int64_t count_, int64_t rows_) : count(count_)
 
 size_t token_order_scratch(int64_t count, int64_t rows) { return SortScratch(nullptr, count, rows).bytes; }
 
+namespace {
+template <int ITEMS>
+void launch_cluster_order(const SortPass &p, const TokenOrder &o, cudaStream_t s) {
+  constexpr size_t smem = sizeof(uint2) * kClusterThreads * ITEMS + sizeof(ClusterSortMemory);
+  static bool ready[kMaxDevices] = {};  // setting it twice does no harm
+  const int dev = current_device();
+  if (!ready[dev]) {
+    ARB_CUDA(cudaFuncSetAttribute(order_cluster_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    ready[dev] = true;
+  }
+  int ctas = 1;
+  while (int64_t(ctas) * kClusterThreads * ITEMS < p.n) ctas *= 2;
+  const int bits = key_bits(o.rows), passes = (bits + kMostClusterBits - 1) / kMostClusterBits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(ctas);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ARB_CUDA(cudaLaunchKernelEx(&cfg, order_cluster_kernel<ITEMS>, p, o, (bits + passes - 1) / passes, passes));
+  count_launch();
+}
+}  // namespace
+
 void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, cudaStream_t s) {
   const int64_t n = t.count();
+  if (n > 0 && n <= int64_t(8) * kClusterThreads * 16) {
+    SortPass p = {};
+    p.tokens = t;
+    p.rows = o.rows;
+    p.n = n;
+    p.first = true;
+    p.by_slot = t.bag_stride < t.token_stride;
+    if (n <= int64_t(8) * kClusterThreads * 2) launch_cluster_order<2>(p, o, s);
+    else launch_cluster_order<16>(p, o, s);
+    return;
+  }
   const SortScratch sc(scratch, n, o.rows);
   const int passes = (key_bits(o.rows) + kDigitBits - 1) / kDigitBits;
   SortPass p;
@@ -594,11 +938,9 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
     p.bag_in = sc.bag[(i + 1) & 1];
     p.key_out = sc.key[i & 1];
     p.bag_out = i == passes - 1 ? o.bag : sc.bag[i & 1];
-    if (t.bytes == 4) sort_count_kernel<int32_t><<<p.tiles, kSortThreads, 0, s>>>(p);
-    else sort_count_kernel<int64_t><<<p.tiles, kSortThreads, 0, s>>>(p);
+    sort_count_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
     sort_scan_kernel<<<kDigits, 256, 0, s>>>(p);
-    if (t.bytes == 4) sort_move_kernel<int32_t><<<p.tiles, kSortThreads, 0, s>>>(p);
-    else sort_move_kernel<int64_t><<<p.tiles, kSortThreads, 0, s>>>(p);
+    sort_move_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
     ARB_CUDA(cudaGetLastError());
     count_launch(3);
   }
@@ -626,7 +968,13 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   sh.ly_row_bits = 0;
   while (sh.tx_bits + sh.ly_row_bits < 5 && (o.rows << sh.ly_row_bits) < o.count) ++sh.ly_row_bits;
   const int chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
-  const int64_t groups = kGradThreads >> (sh.tx_bits + sh.ly_row_bits);
+  // rows a warp: as many as leave the device four CTAs an SM, at most 32
+  const int warp_groups = 32 >> (sh.tx_bits + sh.ly_row_bits);
+  sh.rows_per_group = 1;
+  while (warp_groups * sh.rows_per_group < 32 &&
+         o.rows * chunks / (2 * warp_groups * sh.rows_per_group) >= int64_t(device_sm_count()) * 4 * (kGradThreads / 32))
+    sh.rows_per_group *= 2;
+  const int64_t groups = (kGradThreads / 32) * warp_groups * sh.rows_per_group;  // rows a CTA
   const int64_t item_groups = kGradThreads >> (sh.tx_bits + sh.ly_item_bits);
   unsigned item_blocks = 0;
   if (o.count > o.piece)
@@ -657,6 +1005,7 @@ void launch_lookup_grad(const LookupGradLaunch &a, const TokenOrder &o, void *sc
   float *partial = static_cast<float *>(scratch);
 #define ARB_CALL(T, O)                                                             \
   if (vec * sizeof(T) == 16) lookup_grad_vec<T, O, 16 / sizeof(T)>(a, o, partial, s); \
+  else if (vec * sizeof(T) == 8) lookup_grad_vec<T, O, 8 / sizeof(T)>(a, o, partial, s); \
   else if (vec > 1) lookup_grad_vec<T, O, 4 / sizeof(T)>(a, o, partial, s);         \
   else lookup_grad_vec<T, O, 1>(a, o, partial, s)
   ARB_BY_TYPE(a.type, a.out_type, ARB_CALL);
