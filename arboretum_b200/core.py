@@ -81,9 +81,9 @@ def _load_lib():
     lib.AInitNccl.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
     ptr, i32, i64, f64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
     lib.AEmbedding.argtypes = [ptr, i32, i64, i64, i64, ptr, i32, i64, i64, i64, i64, f64, ptr, i32, i64, i32, ptr]
-    lib.ATokenOrderBytes.argtypes = [i64, i64, ptr, ptr]
+    lib.ATokenOrderBytes.argtypes = [i64, i64, i64, ptr, ptr]
     lib.ATokenOrder.argtypes = [ptr, i32, i64, i64, i64, i64, i64, ptr, ptr, i32, ptr]
-    lib.AEmbeddingGradBytes.argtypes = [i64, i64, i64, ptr]
+    lib.AEmbeddingGradBytes.argtypes = [i64, i64, i64, i64, i32, ptr]
     lib.AEmbeddingGrad.argtypes = [ptr, i32, i64, i64, i64, ptr, i64, i64, f64, ptr, i32, i64, i32, ptr, i32, ptr]
     lib.AAdamWBytes.argtypes = [ptr, i32, ptr, ptr]
     lib.AAdamWCreate.argtypes = [ptr, i32, ptr, ptr, i32, ptr]

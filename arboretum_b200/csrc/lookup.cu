@@ -214,6 +214,8 @@ struct SortPass {
   long long n;
   int tiles, shift;
   bool first, by_slot;     // by_slot: pairs are numbered slot after slot (neighbouring bags lie side by side)
+  bool blocked;            // keys are (run of bags, token)
+  unsigned short *local_out;  // last pass of a blocked order: bags within their run
 };
 
 __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsigned &key, unsigned &bag) {
@@ -228,6 +230,7 @@ __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsign
   const long long row = row_at(p.tokens, p.rows, b, k);
   key = row >= 0 ? unsigned(row) : unsigned(p.rows);
   bag = unsigned(b);
+  if (p.blocked) key += (bag >> kBlockBits) * unsigned(p.rows + 1);
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
@@ -328,7 +331,8 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortPass p) {
       const unsigned digit = (key[j] >> p.shift) & (kDigits - 1);
       const unsigned to = base[digit] + warp_cnt[w][digit] + rank[j];
       p.key_out[to] = key[j];
-      p.bag_out[to] = bag[j];
+      if (p.local_out) p.local_out[to] = (unsigned short)(bag[j] & (kBlockBags - 1));
+      else p.bag_out[to] = bag[j];
     }
   }
 }
@@ -519,6 +523,134 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
       sum_bags<T, VEC, U>(a, o.bag, p0, mine ? p1 : p0, slice, ly, tx, c0, vecs, sum);
       if (mine && slice == 0) write_row<O, VEC, U>(a, row0 + r, c0, tx, vecs, sum);
     }
+  }
+}
+
+// ---- the gradient over a blocked order -------------------------------------------------------
+// Narrow rows: a CTA brings the gradients of one run of bags into shared memory and sums the rows of
+// its share of the table over them: 2 bytes a token are read from device memory, the gradient's
+// values from shared memory.  (Gathered through the second-level cache, 4 bytes of a 32-byte sector
+// each, the same sums of 128 M leaf tokens took 478 us, that cache's bandwidth.)
+constexpr int kNarrowThreads = 512, kNarrowLanes = 8;  // lanes a row
+constexpr unsigned kLongRow = 512;                     // tokens from which a warp takes a row together
+
+template <int DIM>
+__device__ __forceinline__ void add_narrow(const float *grads, const unsigned short *__restrict__ local, unsigned p0,
+                                           unsigned p1, int lane, int lanes, float (&sum)[DIM]) {
+  constexpr int K = 8;
+  for (unsigned p = p0 + lane; p < p1; p += lanes * K) {
+    unsigned at[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) at[k] = p + k * lanes < p1 ? local[p + k * lanes] : unsigned(kBlockBags);
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) sum[d] += grads[at[k] * DIM + d];
+  }
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradLaunch a, TokenOrder o, float *__restrict__ partial) {
+  extern __shared__ float grads[];  // [kBlockBags][DIM], and zeros for positions past a row's end
+  const long long bag0 = (long long)blockIdx.y * kBlockBags;
+  const int n = int(min((long long)kBlockBags, o.bags - bag0));
+  for (int i = threadIdx.x; i < n * DIM; i += kNarrowThreads) {
+    const int r = i / DIM, d = i - r * DIM;
+    grads[i] = to_f32(static_cast<const T *>(a.grad)[(bag0 + r) * a.grad_stride + d]);
+  }
+  if (threadIdx.x < DIM) grads[kBlockBags * DIM + threadIdx.x] = 0.0f;
+  __syncthreads();
+  const unsigned *begin = o.begin + size_t(blockIdx.y) * (o.rows + 1);
+  float *out = partial + size_t(blockIdx.y) * o.rows * DIM;
+  const int lane = threadIdx.x & 31, part = lane & (kNarrowLanes - 1);
+  constexpr int kRows = 32 / kNarrowLanes;  // rows of a warp at a time
+  const long long v_end = min((long long)o.rows, (blockIdx.x + 1ll) * a.rows_per_cta);
+  for (long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * kRows; v0 < v_end;
+       v0 += kNarrowThreads / 32 * kRows) {
+    const long long v = v0 + lane / kNarrowLanes;
+    unsigned p0 = 0, p1 = 0;
+    if (v < v_end) p0 = begin[v], p1 = begin[v + 1];
+    const bool is_long = p1 - p0 >= kLongRow;
+    float sum[DIM];
+#pragma unroll
+    for (int d = 0; d < DIM; ++d) sum[d] = 0.0f;
+    add_narrow<DIM>(grads, o.local, p0, is_long ? p0 : p1, part, kNarrowLanes, sum);
+#pragma unroll
+    for (int d = 0; d < DIM; ++d)
+      for (int s = 1; s < kNarrowLanes; s <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], s);
+    if (part == 0 && v < v_end && !is_long)
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) out[v * DIM + d] = sum[d];
+    unsigned todo = __ballot_sync(0xffffffffu, is_long && part == 0);
+    while (todo) {
+      const int src = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const unsigned q0 = __shfl_sync(0xffffffffu, p0, src), q1 = __shfl_sync(0xffffffffu, p1, src);
+      float all[DIM];
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) all[d] = 0.0f;
+      add_narrow<DIM>(grads, o.local, q0, q1, lane, 32, all);
+#pragma unroll
+      for (int d = 0; d < DIM; ++d)
+        for (int s = 1; s < 32; s <<= 1) all[d] += __shfl_xor_sync(0xffffffffu, all[d], s);
+      if (lane == 0)
+#pragma unroll
+        for (int d = 0; d < DIM; ++d) out[(v0 + src / kNarrowLanes) * DIM + d] = all[d];
+    }
+  }
+}
+
+// Wider rows over a blocked order: a group of tx lanes takes a row's columns over a share of the runs
+// (blockIdx.z of `splits`), from device memory.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLaunch a, TokenOrder o, int tx_bits, int vecs,
+                                                                    int chunks, int splits, float *__restrict__ partial) {
+  const int tx = 1 << tx_bits, lane = threadIdx.x & (tx - 1);
+  const long long v = blockIdx.x * (long long)(kGradThreads >> tx_bits) + (threadIdx.x >> tx_bits);
+  if (v >= o.rows) return;
+  const int k0 = int((long long)o.blocks * blockIdx.z / splits), k1 = int((long long)o.blocks * (blockIdx.z + 1) / splits);
+  for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+    const int c = chunk * tx + lane;
+    if (c >= vecs) continue;
+    const T *grad = static_cast<const T *>(a.grad) + (long long)c * VEC;
+    float sum[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+    for (int k = k0; k < k1; ++k) {
+      const unsigned *begin = o.begin + size_t(k) * (o.rows + 1) + v;
+      const long long bag0 = (long long)k * kBlockBags;
+      const unsigned p1 = begin[1];
+      constexpr int K = 8;
+      for (unsigned p = begin[0]; p < p1; p += K) {
+        Vec<T, VEC> x[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          x[i].clear();
+          if (p + i < p1) x[i].load(grad + (bag0 + o.local[p + i]) * a.grad_stride);
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i) x[i].add_to(sum);
+      }
+    }
+    float *out = partial + ((size_t(blockIdx.z) * o.rows + v) * vecs + c) * VEC;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) out[j] = sum[j];
+  }
+}
+
+// the shares' sums, joined in their order
+template <typename O>
+__global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLaunch a, long long rows, int splits,
+                                                                    const float *__restrict__ partial) {
+  const long long n = rows * a.dim;
+  for (long long i = blockIdx.x * (long long)kGradThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kGradThreads) {
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) sum += partial[size_t(k) * n + i];
+    sum *= a.scale;
+    O *at = static_cast<O *>(a.out) + i / a.dim * a.out_stride + i % a.dim;
+    if (!a.accumulate) from_f32(sum, *at);
+    else if (sum != 0.0f) from_f32(to_f32(*at) + sum, *at);  // a row without bags keeps its bits
   }
 }
 
@@ -722,8 +854,7 @@ int key_bits(int64_t rows) {  // keys are 0 .. rows
 struct SortScratch {
   unsigned *key[2], *bag[2], *counts, *totals;
   size_t bytes;
-  SortScratch(void *mem, int64_t n, int64_t rows) {
-    (void)rows;
+  SortScratch(void *mem, int64_t n) {
     const size_t pair = (size_t(n) * 4 + 255) / 256 * 256;
     const size_t tiles = size_t((n + kTile - 1) / kTile);
     char *p = static_cast<char *>(mem);
@@ -866,18 +997,40 @@ unsigned piece_of(int64_t count) {
 int64_t most_pieces(int64_t count) { return count / piece_of(count) * 2 + 1; }
 }  // namespace
 
-size_t TokenOrder::bytes(int64_t count, int64_t rows) {
-  return 256 + pad256(size_t(count) * 4) + pad256(size_t(rows + 1) * 4) + pad256(size_t(count / piece_of(count) + 1) * 8);
+namespace {
+constexpr int64_t kMostClusterTokens = int64_t(8) * kClusterThreads * 16;
+// An order is kept by runs of bags where a row has 32 bags a run or more, on average: then a run's
+// sums are worth more than the look at where its bags begin.
+int blocks_of(int64_t bags, int64_t per_bag, int64_t rows) {
+  const int64_t blocks = (bags + kBlockBags - 1) / kBlockBags;
+  const bool many = per_bag > 1 && bags * per_bag > kMostClusterTokens && bags * per_bag >= 32 * rows * blocks;
+  return many && blocks < 65536 && blocks * (rows + 1) < (int64_t(1) << 31) ? int(blocks) : 1;
 }
-TokenOrder::TokenOrder(void *mem, int64_t count_, int64_t rows_) : count(count_), rows(rows_), piece(piece_of(count_)) {
-  char *p = static_cast<char *>(mem);
-  counts = reinterpret_cast<unsigned long long *>(p);
-  bag = reinterpret_cast<unsigned *>(p + 256);
-  begin = reinterpret_cast<unsigned *>(p + 256 + pad256(size_t(count) * 4));
-  frequent = reinterpret_cast<uint2 *>(p + 256 + pad256(size_t(count) * 4) + pad256(size_t(rows + 1) * 4));
+}  // namespace
+
+TokenOrder::TokenOrder(void *mem, int64_t bags_, int64_t per_bag, int64_t rows_)
+    : bags(bags_), count(bags_ * per_bag), rows(rows_), blocks(blocks_of(bags_, per_bag, rows_)), piece(piece_of(count)) {
+  size_t at = 0;
+  auto take = [&](size_t b) {
+    char *q = static_cast<char *>(mem) + at;
+    at += pad256(b);
+    return static_cast<void *>(q);
+  };
+  counts = static_cast<unsigned long long *>(take(256));
+  begin = static_cast<unsigned *>(take(size_t(blocks) * size_t(rows + 1) * 4));
+  bag = nullptr, local = nullptr, frequent = nullptr;
+  if (blocks > 1) {
+    local = static_cast<unsigned short *>(take(size_t(count) * 2));
+  } else {
+    bag = static_cast<unsigned *>(take(size_t(count) * 4));
+    frequent = static_cast<uint2 *>(take(size_t(count / piece + 1) * 8));
+  }
+  bytes = at;
 }
 
-size_t token_order_scratch(int64_t count, int64_t rows) { return SortScratch(nullptr, count, rows).bytes; }
+size_t token_order_scratch(int64_t count) {
+  return count <= kMostClusterTokens ? 0 : SortScratch(nullptr, count).bytes;
+}
 
 namespace {
 template <int ITEMS>
@@ -910,50 +1063,108 @@ void launch_cluster_order(const SortPass &p, const TokenOrder &o, cudaStream_t s
 
 void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, cudaStream_t s) {
   const int64_t n = t.count();
-  if (n > 0 && n <= int64_t(8) * kClusterThreads * 16) {
-    SortPass p = {};
-    p.tokens = t;
-    p.rows = o.rows;
-    p.n = n;
-    p.first = true;
-    p.by_slot = t.bag_stride < t.token_stride;
+  SortPass p = {};
+  p.tokens = t;
+  p.rows = o.rows;
+  p.n = n;
+  p.first = true;
+  p.by_slot = std::abs(t.bag_stride) < std::abs(t.token_stride);
+  if (n > 0 && n <= kMostClusterTokens) {
     if (n <= int64_t(8) * kClusterThreads * 2) launch_cluster_order<2>(p, o, s);
     else launch_cluster_order<16>(p, o, s);
     return;
   }
-  const SortScratch sc(scratch, n, o.rows);
-  const int passes = (key_bits(o.rows) + kDigitBits - 1) / kDigitBits;
-  SortPass p;
-  p.tokens = t;
-  p.rows = o.rows;
-  p.n = n;
-  p.tiles = int((n + kTile - 1) / kTile);
-  p.counts = sc.counts;
-  p.totals = sc.totals;
-  p.by_slot = t.bag_stride < t.token_stride;
-  for (int i = 0; i < passes && n > 0; ++i) {
-    p.first = i == 0;
-    p.shift = i * kDigitBits;
-    p.key_in = sc.key[(i + 1) & 1];
-    p.bag_in = sc.bag[(i + 1) & 1];
-    p.key_out = sc.key[i & 1];
-    p.bag_out = i == passes - 1 ? o.bag : sc.bag[i & 1];
-    sort_count_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
-    sort_scan_kernel<<<kDigits, 256, 0, s>>>(p);
-    sort_move_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
-    ARB_CUDA(cudaGetLastError());
-    count_launch(3);
+  const int64_t keys = o.blocks * (o.rows + 1) - 1;  // the largest key
+  const unsigned *sorted = nullptr;
+  if (n > 0) {
+    const SortScratch sc(scratch, n);
+    const int passes = (key_bits(keys) + kDigitBits - 1) / kDigitBits;
+    p.tiles = int((n + kTile - 1) / kTile);
+    p.counts = sc.counts;
+    p.totals = sc.totals;
+    p.blocked = o.blocks > 1;
+    for (int i = 0; i < passes; ++i) {
+      const bool last = i == passes - 1;
+      p.first = i == 0;
+      p.shift = i * kDigitBits;
+      p.key_in = sc.key[(i + 1) & 1];
+      p.bag_in = sc.bag[(i + 1) & 1];
+      p.key_out = sc.key[i & 1];
+      p.bag_out = last ? o.bag : sc.bag[i & 1];
+      p.local_out = last ? o.local : nullptr;
+      sort_count_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
+      sort_scan_kernel<<<kDigits, 256, 0, s>>>(p);
+      sort_move_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
+      ARB_CUDA(cudaGetLastError());
+      count_launch(3);
+    }
+    sorted = sc.key[(passes - 1) & 1];
   }
-  order_begin_kernel<<<grid_of(n + 1, 256, 8), 256, 0, s>>>(sc.key[(passes - 1) & 1], n, o.rows, o.begin);
+  order_begin_kernel<<<grid_of(n + 1, 256, 8), 256, 0, s>>>(sorted, n, keys, o.begin);
   ARB_CUDA(cudaMemsetAsync(o.counts, 0, sizeof *o.counts, s));
-  order_plan_kernel<<<grid_of(o.rows, 256, 8), 256, 0, s>>>(o);
+  if (o.blocks == 1) order_plan_kernel<<<grid_of(o.rows, 256, 8), 256, 0, s>>>(o);
   ARB_CUDA(cudaGetLastError());
   count_launch(2);
 }
 
-size_t lookup_grad_scratch(int64_t count, int64_t rows, int64_t dim) {
-  (void)rows;
-  return count > piece_of(count) ? pad256(size_t(most_pieces(count)) * size_t(dim) * sizeof(float)) : 0;
+namespace {
+
+// shares a row's runs are divided into: one run a share where they fit shared memory, else as many
+// shares as it takes to fill the device
+int splits_of(const TokenOrder &o, int64_t dim) {
+  if (dim <= 3) return o.blocks;
+  const int64_t lanes = std::max<int64_t>(1, o.rows * ((dim + 7) / 8));
+  const int64_t want = (int64_t(device_sm_count()) * 2048 + lanes - 1) / lanes;
+  return int(std::max<int64_t>(1, std::min<int64_t>(o.blocks, want)));
+}
+
+template <typename T, int DIM>
+void narrow_grad_with(LookupGradLaunch a, const TokenOrder &o, float *partial, cudaStream_t s) {
+  static bool ready[kMaxDevices] = {};
+  const int dev = current_device();
+  constexpr int smem = (kBlockBags + 1) * DIM * int(sizeof(float));
+  if (!ready[dev]) {
+    ARB_CUDA(cudaFuncSetAttribute(narrow_grad_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ready[dev] = true;
+  }
+  // shares of the table a run: a few CTAs for every place on the device, so that the last ones fill it
+  const int places = device_sm_count() * (DIM == 1 ? 3 : 1);
+  const int64_t shares = std::max<int64_t>(1, (4 * int64_t(places) + o.blocks - 1) / o.blocks);
+  constexpr int kStep = kNarrowThreads / kNarrowLanes;  // rows a CTA takes at a time
+  a.rows_per_cta = int(std::max<int64_t>(kStep, ((o.rows + shares - 1) / shares + kStep - 1) / kStep * kStep));
+  const dim3 grid(unsigned((o.rows + a.rows_per_cta - 1) / a.rows_per_cta), unsigned(o.blocks));
+  narrow_grad_kernel<T, DIM><<<grid, kNarrowThreads, smem, s>>>(a, o, partial);
+}
+
+template <typename T, int VEC>
+void blocked_grad_with(const LookupGradLaunch &a, const TokenOrder &o, int splits, float *partial, cudaStream_t s) {
+  const int vecs = int(a.dim / VEC);
+  const int tx_bits = std::min(5, log2_floor(std::max(1, vecs * 2 - 1)));
+  const int chunks = (vecs + (1 << tx_bits) - 1) >> tx_bits;
+  const int64_t groups = kGradThreads >> tx_bits;
+  const dim3 grid(unsigned((o.rows + groups - 1) / groups), unsigned(std::min(chunks, 65535)), unsigned(splits));
+  blocked_grad_kernel<T, VEC><<<grid, kGradThreads, 0, s>>>(a, o, tx_bits, vecs, chunks, splits, partial);
+}
+
+template <typename T, typename O>
+void blocked_grad(const LookupGradLaunch &a, const TokenOrder &o, int vec, float *partial, cudaStream_t s) {
+  const int splits = splits_of(o, a.dim);
+  ARB_CHECK(a.dim / vec <= (int64_t(1) << 30), "rows of more than 2^30 vectors");
+  if (a.dim == 1) narrow_grad_with<T, 1>(a, o, partial, s);
+  else if (a.dim == 2) narrow_grad_with<T, 2>(a, o, partial, s);
+  else if (a.dim == 3) narrow_grad_with<T, 3>(a, o, partial, s);
+  else if (vec * sizeof(T) == 16) blocked_grad_with<T, 16 / sizeof(T)>(a, o, splits, partial, s);
+  else if (vec * sizeof(T) >= 4) blocked_grad_with<T, 4 / sizeof(T)>(a, o, splits, partial, s);
+  else blocked_grad_with<T, 1>(a, o, splits, partial, s);
+  blocked_join_kernel<O><<<grid_of(o.rows * a.dim, kGradThreads, 8), kGradThreads, 0, s>>>(a, o.rows, splits, partial);
+  count_launch();
+}
+
+}  // namespace
+
+size_t lookup_grad_scratch(const TokenOrder &o, int64_t dim) {
+  if (o.blocks > 1) return pad256(size_t(splits_of(o, dim)) * size_t(o.rows) * size_t(dim) * sizeof(float));
+  return o.count > o.piece ? pad256(size_t(most_pieces(o.count)) * size_t(dim) * sizeof(float)) : 0;
 }
 
 namespace {
@@ -1004,7 +1215,8 @@ void launch_lookup_grad(const LookupGradLaunch &a, const TokenOrder &o, void *sc
   const int vec = vec_of(a.type, a.dim, a.grad, a.grad_stride, a.out, a.out_type, a.out_stride);
   float *partial = static_cast<float *>(scratch);
 #define ARB_CALL(T, O)                                                             \
-  if (vec * sizeof(T) == 16) lookup_grad_vec<T, O, 16 / sizeof(T)>(a, o, partial, s); \
+  if (o.blocks > 1) blocked_grad<T, O>(a, o, vec, partial, s);                      \
+  else if (vec * sizeof(T) == 16) lookup_grad_vec<T, O, 16 / sizeof(T)>(a, o, partial, s); \
   else if (vec * sizeof(T) == 8) lookup_grad_vec<T, O, 8 / sizeof(T)>(a, o, partial, s); \
   else if (vec > 1) lookup_grad_vec<T, O, 4 / sizeof(T)>(a, o, partial, s);         \
   else lookup_grad_vec<T, O, 1>(a, o, partial, s)

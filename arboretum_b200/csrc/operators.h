@@ -36,21 +36,30 @@ struct LookupLaunch {
 };
 void launch_lookup(const LookupLaunch &a, cudaStream_t s);
 
-// The tokens' order, in memory of the caller: for every row v of the table, the bags that name it
-// are bag[begin[v] .. begin[v + 1]), in a fixed order that only the tokens decide.
+// The tokens' order, in memory of the caller: for every row v of the table, the bags that name it,
+// in a fixed order that only the tokens decide.
+//
+// blocks == 1: bag[begin[v] .. begin[v + 1]).
+// blocks > 1: many bags of several tokens over few rows (the leaves of a forest).  The order is kept
+// apart for every run of kBlockBags bags: within run k the bags of row v are
+// local[begin[k * (rows + 1) + v] .. begin[k * (rows + 1) + v + 1]), numbered from the run's first one
+// in 16 bits.  The gradients of a run fit into shared memory.
+constexpr int kBlockBits = 14, kBlockBags = 1 << kBlockBits;
 struct TokenOrder {
-  unsigned *bag;    // count
-  unsigned *begin;  // rows + 1
-  int64_t count, rows;
-  // rows named by more than `piece` bags: (row, number of its first piece), and how many there are:
-  // the rows in the upper half of *counts, their pieces in the lower one
+  int64_t bags, count, rows;
+  int blocks;
+  unsigned *bag;          // count
+  unsigned short *local;  // count
+  unsigned *begin;        // blocks * (rows + 1)
+  // rows named by more than `piece` bags (blocks == 1 only): (row, number of its first piece), and
+  // how many there are: the rows in the upper half of *counts, their pieces in the lower one
   unsigned piece;
   uint2 *frequent;
   unsigned long long *counts;
-  TokenOrder(void *mem, int64_t count, int64_t rows);
-  static size_t bytes(int64_t count, int64_t rows);
+  size_t bytes;
+  TokenOrder(void *mem, int64_t bags, int64_t per_bag, int64_t rows);
 };
-size_t token_order_scratch(int64_t count, int64_t rows);
+size_t token_order_scratch(int64_t count);
 void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, cudaStream_t s);
 
 struct LookupGradLaunch {
@@ -62,8 +71,9 @@ struct LookupGradLaunch {
   int out_type;
   int64_t out_stride;
   bool accumulate;
+  int rows_per_cta = 0;  // set by the launcher
 };
-size_t lookup_grad_scratch(int64_t count, int64_t rows, int64_t dim);
+size_t lookup_grad_scratch(const TokenOrder &o, int64_t dim);
 void launch_lookup_grad(const LookupGradLaunch &a, const TokenOrder &o, void *scratch, cudaStream_t s);
 
 // ---- AdamW ---------------------------------------------------------------------------------

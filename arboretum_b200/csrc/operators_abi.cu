@@ -50,13 +50,17 @@ void check_matrix(const void *p, int type, int64_t rows, int64_t dim, int64_t st
     throw std::runtime_error(std::string(what) + ": stride out of range");
 }
 
-TokenView check_tokens(const void *tokens, int bytes, int64_t bags, int64_t per_bag, int64_t bag_stride,
-                       int64_t token_stride, int64_t rows) {
-  ARB_CHECK(bytes == 4 || bytes == 8, "tokens are int32 or int64");
+void check_counts(int64_t bags, int64_t per_bag, int64_t rows) {
   ARB_CHECK(bags >= 0 && per_bag >= 0, "negative token count");
   ARB_CHECK(bags <= kMostTokens && per_bag <= kMostTokens && (per_bag == 0 || bags <= kMostTokens / per_bag),
             "more than 2^31 - 2 tokens in one call");
   ARB_CHECK(rows >= 0 && rows <= kMostRows, "a table has at most 2^31 - 2 rows");
+}
+
+TokenView check_tokens(const void *tokens, int bytes, int64_t bags, int64_t per_bag, int64_t bag_stride,
+                       int64_t token_stride, int64_t rows) {
+  ARB_CHECK(bytes == 4 || bytes == 8, "tokens are int32 or int64");
+  check_counts(bags, per_bag, rows);
   ARB_CHECK(std::abs(bag_stride) <= kMostElements && std::abs(token_stride) <= kMostElements, "token stride out of range");
   if (bags * per_bag > 0) {
     ARB_CHECK(tokens != nullptr, "tokens is NULL");
@@ -133,12 +137,12 @@ const char *AEmbedding(const void *table, int type, int64_t rows, int64_t dim, i
   ARB_CATCH
 }
 
-const char *ATokenOrderBytes(int64_t count, int64_t rows, int64_t *order_bytes, int64_t *scratch_bytes) {
+const char *ATokenOrderBytes(int64_t bags, int64_t per_bag, int64_t rows, int64_t *order_bytes, int64_t *scratch_bytes) {
   ARB_TRY
   ARB_CHECK(order_bytes && scratch_bytes, "NULL argument");
-  check_tokens(nullptr, 4, count, 0, 0, 0, rows);
-  *order_bytes = int64_t(TokenOrder::bytes(count, rows));
-  *scratch_bytes = int64_t(token_order_scratch(count, rows));
+  check_counts(bags, per_bag, rows);
+  *order_bytes = int64_t(TokenOrder(nullptr, bags, per_bag, rows).bytes);
+  *scratch_bytes = int64_t(token_order_scratch(bags * per_bag));
   ARB_CATCH
 }
 
@@ -146,29 +150,34 @@ const char *ATokenOrder(const void *tokens, int token_bytes, int64_t bags, int64
                         int64_t token_stride, int64_t rows, void *order, void *scratch, int device, void *stream) {
   ARB_TRY
   const TokenView t = check_tokens(tokens, token_bytes, bags, per_bag, bag_stride, token_stride, rows);
-  ARB_CHECK(order && scratch, "NULL argument");
+  ARB_CHECK(order && (scratch || token_order_scratch(t.count()) == 0), "NULL argument");
   check_aligned(order, 256, "order");
   check_aligned(scratch, 256, "scratch");
   DeviceScope scope(device);
-  launch_token_order(t, TokenOrder(order, t.count(), rows), scratch, static_cast<cudaStream_t>(stream));
+  launch_token_order(t, TokenOrder(order, bags, per_bag, rows), scratch, static_cast<cudaStream_t>(stream));
   ARB_CATCH
 }
 
-const char *AEmbeddingGradBytes(int64_t count, int64_t rows, int64_t dim, int64_t *scratch_bytes) {
+const char *AEmbeddingGradBytes(int64_t bags, int64_t per_bag, int64_t rows, int64_t dim, int device, int64_t *scratch_bytes) {
   ARB_TRY
   ARB_CHECK(scratch_bytes, "NULL argument");
-  check_tokens(nullptr, 4, count, 0, 0, 0, rows);
+  check_counts(bags, per_bag, rows);
   ARB_CHECK(dim >= 0 && dim <= kMostElements, "row width out of range");
-  *scratch_bytes = int64_t(lookup_grad_scratch(count, rows, dim));
+  const TokenOrder o(nullptr, bags, per_bag, rows);
+  if (o.blocks > 1) {  // goes by the device's size
+    DeviceScope scope(device);
+    *scratch_bytes = int64_t(lookup_grad_scratch(o, dim));
+  } else {
+    *scratch_bytes = int64_t(lookup_grad_scratch(o, dim));
+  }
   ARB_CATCH
 }
 
 const char *AEmbeddingGrad(const void *grad, int type, int64_t bags, int64_t dim, int64_t grad_stride,
-                           const void *order, int64_t count, int64_t rows, double scale, void *out, int out_type,
+                           const void *order, int64_t per_bag, int64_t rows, double scale, void *out, int out_type,
                            int64_t out_stride, int accumulate, void *scratch, int device, void *stream) {
   ARB_TRY
-  check_tokens(nullptr, 4, count, 0, 0, 0, rows);
-  ARB_CHECK(bags >= 0 && bags <= kMostTokens, "bag count out of range");
+  check_counts(bags, per_bag, rows);
   ARB_CHECK(dim >= 0 && dim <= kMostElements, "row width out of range");
   check_matrix(grad, type, bags, dim, grad_stride, "grad");
   check_out(type, out_type);
@@ -176,16 +185,17 @@ const char *AEmbeddingGrad(const void *grad, int type, int64_t bags, int64_t dim
   ARB_CHECK(rows < 2 || out_stride >= dim, "rows of out overlap");
   ARB_CHECK(order != nullptr, "order is NULL");
   check_aligned(order, 256, "order");
-  if (rows == 0 || dim == 0) return nullptr;
-  ARB_CHECK(scratch != nullptr || lookup_grad_scratch(count, rows, dim) == 0, "scratch is NULL");
   check_aligned(scratch, 256, "scratch");
+  if (rows == 0 || dim == 0) return nullptr;
+  const TokenOrder o(const_cast<void *>(order), bags, per_bag, rows);
+  DeviceScope scope(device);
+  ARB_CHECK(scratch != nullptr || lookup_grad_scratch(o, dim) == 0, "scratch is NULL");
   LookupGradLaunch a;
   a.grad = grad, a.type = type, a.dim = dim, a.grad_stride = grad_stride;
   a.scale = float(scale);
   a.out = out, a.out_type = out_type, a.out_stride = out_stride;
   a.accumulate = accumulate != 0;
-  DeviceScope scope(device);
-  launch_lookup_grad(a, TokenOrder(const_cast<void *>(order), count, rows), scratch, static_cast<cudaStream_t>(stream));
+  launch_lookup_grad(a, o, scratch, static_cast<cudaStream_t>(stream));
   ARB_CATCH
 }
 

@@ -140,16 +140,16 @@ def embedding(tokens, table, scale=1.0, pooled=False, out=None, out_dtype=None):
 
 
 @functools.lru_cache(maxsize=1024)
-def _order_bytes(count, rows):
+def _order_bytes(bags, per_bag, rows):
     order, scratch = ctypes.c_int64(0), ctypes.c_int64(0)
-    _call_and_throw_if_error(_LIB.ATokenOrderBytes(count, rows, ctypes.byref(order), ctypes.byref(scratch)))
+    _call_and_throw_if_error(_LIB.ATokenOrderBytes(bags, per_bag, rows, ctypes.byref(order), ctypes.byref(scratch)))
     return order.value, scratch.value
 
 
 @functools.lru_cache(maxsize=1024)
-def _grad_bytes(count, rows, dim):
+def _grad_bytes(bags, per_bag, rows, dim, device):
     scratch = ctypes.c_int64(0)
-    _call_and_throw_if_error(_LIB.AEmbeddingGradBytes(count, rows, dim, ctypes.byref(scratch)))
+    _call_and_throw_if_error(_LIB.AEmbeddingGradBytes(bags, per_bag, rows, dim, device, ctypes.byref(scratch)))
     return scratch.value
 
 
@@ -162,19 +162,18 @@ class TokenOrder(object):
     sorts anew in every call that is given tokens."""
 
     def __init__(self, tokens, rows, pooled=False):
-        flat, self.bags, per_bag, bag_stride, token_stride = _bags(tokens, pooled)
+        flat, self.bags, self.per_bag, bag_stride, token_stride = _bags(tokens, pooled)
         self.rows = int(rows)
         self.pooled = bool(pooled)
         self.shape = tuple(tokens.shape)
-        self.count = self.bags * per_bag
-        order_bytes, scratch_bytes = _order_bytes(self.count, self.rows)
+        order_bytes, scratch_bytes = _order_bytes(self.bags, self.per_bag, self.rows)
         device = _one_device(tokens)
         self.device = tokens.device
         self._stream = _stream(device)
         self._data = _memory(order_bytes, self.device)
         scratch = _memory(scratch_bytes, self.device)
         _call_and_throw_if_error(_LIB.ATokenOrder(
-            flat.data_ptr(), _TOKEN_BYTES[flat.dtype], self.bags, per_bag, bag_stride, token_stride, self.rows,
+            flat.data_ptr(), _TOKEN_BYTES[flat.dtype], self.bags, self.per_bag, bag_stride, token_stride, self.rows,
             self._data.data_ptr(), scratch.data_ptr(), device, self._stream))
 
     def _use(self, stream):
@@ -206,21 +205,20 @@ def embedding_grad(grad, tokens, rows, scale=1.0, pooled=False, out=None, out_dt
     order = tokens if isinstance(tokens, TokenOrder) else None
     if order is None:
         flat, bags, per_bag, bag_stride, token_stride = _bags(tokens, pooled)
-        shape, count = tuple(tokens.shape), bags * per_bag
+        shape = tuple(tokens.shape)
     else:
         if order.rows != rows:
             raise ValueError("the order was made for %d rows, not %d" % (order.rows, rows))
-        shape, count, bags, pooled = order.shape, order.count, order.bags, order.pooled
+        shape, per_bag, bags, pooled = order.shape, order.per_bag, order.bags, order.pooled
     if grad.dim() < 1 or tuple(grad.shape[:-1]) != ((bags,) if pooled else shape):
         raise ValueError("grad must have shape %s x columns, not %s" % ((bags,) if pooled else shape, tuple(grad.shape)))
     dim = grad.shape[-1]
     if accumulate and out is None:
         raise ValueError("accumulate needs the gradient to add to: out")
     # bytes first: a size out of range is refused before anything is allocated
-    scratch_bytes = _grad_bytes(count, rows, dim)
-    if order is None:
-        order_bytes, sort_bytes = _order_bytes(count, rows)
+    order_bytes, sort_bytes = _order_bytes(bags, per_bag, rows)
     device = _one_device(grad, tokens=tokens, out=out)
+    scratch_bytes = _grad_bytes(bags, per_bag, rows, dim, device)
     if grad.dim() != 2:
         grad = grad.reshape(-1, dim) if grad.numel() else grad.reshape(bags, dim)
     if grad.numel() and dim > 1 and grad.stride(1) != 1:
@@ -243,6 +241,6 @@ def embedding_grad(grad, tokens, rows, scale=1.0, pooled=False, out=None, out_dt
         memory = _memory(scratch_bytes, grad.device)
         order_at, scratch_at = order._use(stream), memory.data_ptr()
     _call_and_throw_if_error(_LIB.AEmbeddingGrad(
-        grad.data_ptr(), kind, bags, dim, grad.stride(0), order_at, count, rows, scale, matrix.data_ptr(),
+        grad.data_ptr(), kind, bags, dim, grad.stride(0), order_at, per_bag, rows, scale, matrix.data_ptr(),
         _TYPE[matrix.dtype], matrix.stride(0), int(accumulate), scratch_at, device, stream))
     return out

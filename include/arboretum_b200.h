@@ -177,20 +177,21 @@ const char *AEmbedding(const void *table, int type, int64_t rows, int64_t dim, i
                        const void *tokens, int token_bytes, int64_t bags, int64_t per_bag,
                        int64_t bag_stride, int64_t token_stride, double scale, void *out, int out_type,
                        int64_t out_stride, int device, void *stream);
-/* Bytes that ATokenOrder needs for `count` = bags * per_bag tokens: the order itself (kept as long
- * as it is used) and scratch (free after the call).  Both 256-byte aligned. */
-const char *ATokenOrderBytes(int64_t count, int64_t rows, int64_t *order_bytes, int64_t *scratch_bytes);
+/* Bytes that ATokenOrder needs: the order itself (kept as long as it is used) and scratch (free
+ * after the call; may be 0).  Both 256-byte aligned. */
+const char *ATokenOrderBytes(int64_t bags, int64_t per_bag, int64_t rows, int64_t *order_bytes, int64_t *scratch_bytes);
 /* Sorts the bags by the tokens that name them, for AEmbeddingGrad: stable, so equal tokens give
  * equal orders. */
 const char *ATokenOrder(const void *tokens, int token_bytes, int64_t bags, int64_t per_bag, int64_t bag_stride,
                         int64_t token_stride, int64_t rows, void *order, void *scratch, int device, void *stream);
-const char *AEmbeddingGradBytes(int64_t count, int64_t rows, int64_t dim, int64_t *scratch_bytes);
+const char *AEmbeddingGradBytes(int64_t bags, int64_t per_bag, int64_t rows, int64_t dim, int device,
+                                int64_t *scratch_bytes);
 /* out[v][:] = scale * sum of grad[b][:] over all (b, t) whose token is v (accumulate: added to out,
- * rows no token names stay untouched; else they become zero).  `order` of the same count and rows.
- * Summed in fp32 in a fixed order: the same inputs give the same bits.  grad_stride 0: one row for
- * all bags. */
+ * rows no token names stay untouched; else they become zero).  `order` of the same bags, tokens a
+ * bag and rows.  Summed in fp32 in a fixed order: the same inputs give the same bits on the same
+ * device.  grad_stride 0: one row for all bags. */
 const char *AEmbeddingGrad(const void *grad, int type, int64_t bags, int64_t dim, int64_t grad_stride,
-                           const void *order, int64_t count, int64_t rows, double scale, void *out, int out_type,
+                           const void *order, int64_t per_bag, int64_t rows, double scale, void *out, int out_type,
                            int64_t out_stride, int accumulate, void *scratch, int device, void *stream);
 
 /* AdamW over many tensors in one launch.  Element i of tensor k has its moments at element

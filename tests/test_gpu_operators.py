@@ -181,6 +181,33 @@ def test_forest_layout(bags, per_bag, leaves, dim):
     _near(arb.embedding_grad(grad.cuda(), order, rows, scale=0.1), want, size, count, F32)
 
 
+@pytest.mark.parametrize("bags,per_bag,rows,dim", [
+    (40001, 9, 90, 1), (40000, 9, 90, 3), (16384 * 2 + 1, 17, 33, 2), (70001, 5, 7, 5), (50000, 6, 20, 64), (33000, 8, 3, 1),
+    (20000, 40, 500, 2), (65536, 4, 2, 8), (300007, 2, 600, 33)])
+def test_many_bags_over_few_rows(bags, per_bag, rows, dim):
+    """Where the lookup holds the table in shared memory and the order is kept by runs of bags."""
+    gen = _rng(bags, per_bag, rows, dim)
+    for index, by_slot in ((torch.int32, True), (torch.int64, False), (torch.int64, True)):
+        tok = _tokens(bags, per_bag, rows, index, gen, empty=0.1)
+        tok[:, 0] = rows - 1  # a row that every bag names
+        tok = tok.t().contiguous().t() if by_slot else tok
+        dev = tok.cuda().t().contiguous().t() if by_slot else tok.cuda()
+        for dtype, out_dtype in ((F32, F32), (BF16, F32), (F16, F16)):
+            table = torch.randn(rows, dim, generator=gen).to(dtype)
+            want, size = _plain_lookup(tok, table, 0.3)
+            _near(arb.embedding(dev, table.cuda(), scale=0.3, pooled=True, out_dtype=out_dtype), want, size, per_bag, out_dtype)
+            grad = (torch.randn(bags, dim, generator=gen) * 0.01).to(dtype)
+            want, size, count = _plain_grad(grad, tok, rows, 0.3)
+            got = arb.embedding_grad(grad.cuda(), dev, rows, scale=0.3, pooled=True, out_dtype=out_dtype)
+            _near(got, want, size, count, out_dtype)
+            assert torch.equal(got, arb.embedding_grad(grad.cuda(), arb.token_order(dev, rows, pooled=True), rows, scale=0.3, out_dtype=out_dtype))
+            before = torch.randn(rows, dim, generator=gen).to(out_dtype)
+            out = before.cuda()
+            arb.embedding_grad(grad.cuda(), dev, rows, scale=0.3, pooled=True, out=out, accumulate=True)
+            assert torch.equal(out.cpu()[(count == 0).expand(rows, dim)], before[(count == 0).expand(rows, dim)])
+            _near(out, want + before.double(), size + before.double().abs(), count + 1, out_dtype)
+
+
 def test_gradient_of_broadcast_inputs():
     tok = torch.randint(0, 30, (6, 50), generator=_rng(5))
     row = torch.randn(40, generator=_rng(6)).cuda()

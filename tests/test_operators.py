@@ -47,23 +47,24 @@ def test_nothing_to_do_touches_no_device():
 
 def test_order_and_gradient_refuse():
     a, b = ctypes.c_int64(0), ctypes.c_int64(0)
-    assert LIB.ATokenOrderBytes(100, 10, ctypes.byref(a), ctypes.byref(b)) is None
-    assert a.value >= 4 * (100 + 11) and b.value > 0 and a.value % 256 == 0
-    assert "2^31 - 2 tokens" in _message(LIB.ATokenOrderBytes(1 << 31, 10, ctypes.byref(a), ctypes.byref(b)))
-    assert "NULL" in _message(LIB.ATokenOrderBytes(1, 10, None, ctypes.byref(b)))
+    for bags, per_bag, rows in ((50, 2, 10), (200000, 1, 10), (200000, 100, 6400)):
+        assert LIB.ATokenOrderBytes(bags, per_bag, rows, ctypes.byref(a), ctypes.byref(b)) is None
+        assert a.value >= 2 * bags * per_bag + 4 * (rows + 1) and b.value >= 0 and a.value % 256 == 0 and b.value % 256 == 0
+    assert "2^31 - 2 tokens" in _message(LIB.ATokenOrderBytes(1 << 30, 2, 10, ctypes.byref(a), ctypes.byref(b)))
+    assert "NULL" in _message(LIB.ATokenOrderBytes(1, 1, 10, None, ctypes.byref(b)))
     assert "NULL" in _message(LIB.ATokenOrder(P, 4, 3, 1, 1, 0, 10, None, P, 0, None))
     assert "aligned" in _message(LIB.ATokenOrder(P, 4, 3, 1, 1, 0, 10, ctypes.c_void_p(8), P, 0, None))
     assert "rows" in _message(LIB.ATokenOrder(P, 4, 3, 1, 1, 0, 1 << 31, P, P, 0, None))
 
     def grad(**change):
-        g = dict(grad=P, type=0, bags=3, dim=4, grad_stride=4, order=P, count=3, rows=10, scale=1.0, out=P, out_type=0,
+        g = dict(grad=P, type=0, bags=3, dim=4, grad_stride=4, order=P, per_bag=1, rows=10, scale=1.0, out=P, out_type=0,
                  out_stride=4, accumulate=0, scratch=P, device=0, stream=None)
         g.update(change)
         return LIB.AEmbeddingGrad(*g.values())
     for change, words in ((dict(order=None), "order is NULL"), (dict(grad=None), "grad is NULL"), (dict(out=None), "out is NULL"),
                           (dict(out_stride=2), "overlap"), (dict(type=2, out_type=1), "input's type"), (dict(rows=-1), "rows"),
-                          (dict(count=-1), "negative"), (dict(grad_stride=-1), "stride"), (dict(scratch=ctypes.c_void_p(3)), "aligned"),
-                          (dict(bags=1 << 40), "bag count")):
+                          (dict(per_bag=-1), "negative"), (dict(grad_stride=-1), "stride"), (dict(scratch=ctypes.c_void_p(3)), "aligned"),
+                          (dict(bags=1 << 40), "2^31 - 2 tokens")):
         assert words in _message(grad(**change)), change
     assert grad(rows=0, out=None) is None and grad(dim=0, grad=None, out=None) is None
 
