@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "operators.h"
 #include "vec.cuh"
@@ -38,70 +39,90 @@ struct LaneShape {
 // it adds the first, so that enough bytes are in flight.  With few bags the tokens of a bag are
 // split over ly lanes, which join their sums through shared memory in a fixed order.
 constexpr int kLookupThreads = 256;
-template <typename T, typename O, int VEC, int U, int K>
+
+// A thread's vector of the sum over the tokens k0, k0 + ly, .. of bag b, K rows in flight.
+// TOGETHER: the lanes of a group (at least eight) fetch a token each and hand them around, so that a
+// bag's tokens cost one access and empty slots cost nothing.
+template <typename T, int VEC, int K, bool TOGETHER>
+__device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, int slice, int ly, int tx, int c, int vecs,
+                                           float (&sum)[VEC]) {
+  const T *table = static_cast<const T *>(a.table) + (long long)c * VEC;
+  const long long per_bag = b < a.tokens.bags ? a.tokens.per_bag : 0;
+  if (TOGETHER) {
+    const int width = min(tx, 32), lane = threadIdx.x & 31, group0 = lane & ~(width - 1);
+    // every lane of the warp makes as many rounds as a whole bag needs: the shuffles want them all
+    for (long long k0 = 0; k0 < a.tokens.per_bag; k0 += (long long)ly * width) {
+      const long long k = k0 + slice + (long long)(lane - group0) * ly;
+      const long long row = k < per_bag ? row_at(a.tokens, a.rows, b, k) : -1;
+      const int index = int(row);  // rows fit 31 bits
+      unsigned todo = (__ballot_sync(0xffffffffu, row >= 0) >> group0) & (width == 32 ? 0xffffffffu : (1u << width) - 1u);
+      while (__any_sync(0xffffffffu, todo != 0)) {
+        Vec<T, VEC> v[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+          const int src = todo ? __ffs(todo) - 1 : 0;
+          const int r = __shfl_sync(0xffffffffu, index, group0 + src);
+          v[i].clear();
+          if (todo && c < vecs) v[i].load(table + (long long)r * a.row_stride);
+          todo &= todo - 1;
+        }
+#pragma unroll
+        for (int i = 0; i < K; ++i) v[i].add_to(sum);
+      }
+    }
+  } else {
+    for (long long k0 = slice; k0 < per_bag; k0 += (long long)ly * K) {
+      long long row[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) row[i] = k0 + i * ly < per_bag ? row_at(a.tokens, a.rows, b, k0 + i * ly) : -1;
+      Vec<T, VEC> v[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        v[i].clear();
+        if (row[i] >= 0 && c < vecs) v[i].load(table + row[i] * a.row_stride);
+      }
+#pragma unroll
+      for (int i = 0; i < K; ++i) v[i].add_to(sum);
+    }
+  }
+}
+
+// Bags of several tokens.  A unit is a bag and a run of tx vectors of VEC columns.  Memory bound: the
+// rows are read once and the result written once; a thread has the loads of K rows in flight before it
+// adds the first.  With few bags the tokens of a bag are split over ly groups of lanes, which join
+// their sums through shared memory in a fixed order.
+template <typename T, typename O, int VEC, bool TOGETHER>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupLaunch a, LaneShape sh, int vecs, int chunks) {
-  __shared__ float part[kLookupThreads * U * VEC];
+  __shared__ float part[kLookupThreads * VEC];
   const int tx = 1 << sh.tx_bits, ly = 1 << sh.ly_bits;
   const int lane = threadIdx.x & (tx - 1), slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
   const int group = threadIdx.x >> (sh.tx_bits + sh.ly_bits), groups = kLookupThreads >> (sh.tx_bits + sh.ly_bits);
-  const T *table = static_cast<const T *>(a.table);
   const long long b = blockIdx.x * (long long)groups + group;
   for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
-    const int c0 = chunk * (tx * U) + lane;
-    float sum[U][VEC];
+    const int c = chunk * tx + lane;
+    float sum[VEC];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[u][j] = 0.0f;
-    if (b < a.tokens.bags) {
-      for (long long k0 = slice; k0 < a.tokens.per_bag; k0 += ly * K) {
-        long long row[K];
-#pragma unroll
-        for (int k = 0; k < K; ++k) row[k] = k0 + k * ly < a.tokens.per_bag ? row_at(a.tokens, a.rows, b, k0 + k * ly) : -1;
-        Vec<T, VEC> v[K][U];
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            if (row[k] >= 0 && c0 + u * tx < vecs) v[k][u].load(table + row[k] * a.row_stride + (long long)(c0 + u * tx) * VEC);
-            else v[k][u].clear();
-          }
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int u = 0; u < U; ++u) v[k][u].add_to(sum[u]);
-      }
-    }
+    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+    sum_tokens<T, VEC, 8, TOGETHER>(a, b, slice, ly, tx, c, vecs, sum);
     if (ly > 1) {
       __syncthreads();
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) part[(u * VEC + j) * kLookupThreads + threadIdx.x] = sum[u][j];
+      for (int j = 0; j < VEC; ++j) part[j * kLookupThreads + threadIdx.x] = sum[j];
       for (int half = ly >> 1; half > 0; half >>= 1) {
         __syncthreads();
         if (slice < half) {
 #pragma unroll
-          for (int i = 0; i < U * VEC; ++i)
-            part[i * kLookupThreads + threadIdx.x] += part[i * kLookupThreads + threadIdx.x + half * tx];
+          for (int j = 0; j < VEC; ++j)
+            part[j * kLookupThreads + threadIdx.x] += part[j * kLookupThreads + threadIdx.x + half * tx];
         }
       }
-      if (slice != 0) continue;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[u][j] = part[(u * VEC + j) * kLookupThreads + threadIdx.x];
+      for (int j = 0; j < VEC; ++j) sum[j] = part[j * kLookupThreads + threadIdx.x];
     }
-    if (b < a.tokens.bags) {
-      O *out = static_cast<O *>(a.out) + b * a.out_stride;
+    if (b < a.tokens.bags && slice == 0 && c < vecs) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (c0 + u * tx < vecs) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sum[u][j] *= a.scale;
-          store_vec<O, VEC>(out + (long long)(c0 + u * tx) * VEC, sum[u]);
-        }
-      }
+      for (int j = 0; j < VEC; ++j) sum[j] *= a.scale;
+      store_vec<O, VEC>(static_cast<O *>(a.out) + b * a.out_stride + (long long)c * VEC, sum);
     }
   }
 }
@@ -141,12 +162,38 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunc
 // table's values come from shared memory, where 32 random words cost a few cycles and a gather
 // through the first-level cache one for every line it touches.
 constexpr int kTableThreads = 1024;
+template <typename I, int DIM, int K>
+__device__ __forceinline__ void add_table(const float *values, unsigned rows, const I *p, long long step, long long other,
+                                          bool paired, float (&sum)[2][DIM]) {
+  struct alignas(2 * sizeof(I)) Both { I v[2]; };
+  Both tok[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (paired) {  // one access for both bags
+      tok[k] = *reinterpret_cast<const Both *>(p);
+    } else {
+      tok[k].v[0] = p[0];
+      tok[k].v[1] = p[other];
+    }
+    p += step;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      using U = typename std::make_unsigned<I>::type;
+      const unsigned r = U(tok[k].v[e]) < U(rows) ? unsigned(tok[k].v[e]) : rows;
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) sum[e][d] += values[r * DIM + d];
+    }
+}
+
 template <typename T, typename O, typename I, int DIM>
 __global__ void __launch_bounds__(kTableThreads) lookup_table_kernel(LookupLaunch a, bool paired) {
   extern __shared__ float values[];  // [rows][DIM], and a row of zeros for empty slots
-  const int rows = int(a.rows);
-  for (int i = threadIdx.x; i < (rows + 1) * DIM; i += kTableThreads) {
-    const int r = i / DIM, d = i - r * DIM;
+  const unsigned rows = unsigned(a.rows);
+  for (unsigned i = threadIdx.x; i < (rows + 1) * DIM; i += kTableThreads) {
+    const unsigned r = i / DIM, d = i - r * DIM;
     values[i] = r < rows ? to_f32(static_cast<const T *>(a.table)[(long long)r * a.row_stride + d]) : 0.0f;
   }
   __syncthreads();
@@ -156,36 +203,15 @@ __global__ void __launch_bounds__(kTableThreads) lookup_table_kernel(LookupLaunc
   for (long long b = (blockIdx.x * (long long)kTableThreads + threadIdx.x) * 2; b < a.tokens.bags;
        b += (long long)gridDim.x * kTableThreads * 2) {
     const bool two = b + 1 < a.tokens.bags;
-    const I *at = static_cast<const I *>(a.tokens.at) + b * a.tokens.bag_stride;
+    const long long other = two ? a.tokens.bag_stride : 0;  // a last bag alone is summed twice
+    const bool both = paired && two;
+    const I *p = static_cast<const I *>(a.tokens.at) + b * a.tokens.bag_stride;
     float sum[2][DIM];
 #pragma unroll
     for (int d = 0; d < DIM; ++d) sum[0][d] = sum[1][d] = 0.0f;
-    for (int k0 = 0; k0 < per_bag; k0 += K) {
-      I tok[K][2];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        tok[k][0] = tok[k][1] = -1;
-        if (k0 + k < per_bag) {
-          const I *p = at + (k0 + k) * step;
-          if (paired && two) {  // one access for both
-            struct alignas(2 * sizeof(I)) Both { I v[2]; };
-            const Both both = *reinterpret_cast<const Both *>(p);
-            tok[k][0] = both.v[0], tok[k][1] = both.v[1];
-          } else {
-            tok[k][0] = p[0];
-            if (two) tok[k][1] = p[a.tokens.bag_stride];
-          }
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = tok[k][e] >= 0 && tok[k][e] < a.rows ? int(tok[k][e]) : rows;
-#pragma unroll
-          for (int d = 0; d < DIM; ++d) sum[e][d] += values[r * DIM + d];
-        }
-    }
+    int k = 0;
+    for (; k + K <= per_bag; k += K, p += K * step) add_table<I, DIM, K>(values, rows, p, step, other, both, sum);
+    for (; k < per_bag; ++k, p += step) add_table<I, DIM, 1>(values, rows, p, step, other, both, sum);
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (e == 0 || two) {
@@ -360,29 +386,71 @@ __global__ void order_begin_kernel(const unsigned *__restrict__ key, long long n
   }
 }
 
-// ---- rows named by many bags -----------------------------------------------------------------
-// A row named by more than `piece` bags is cut into pieces of that many, so that the sum of a
-// frequent token is shared by many warps.  Which slot a row's pieces get depends on the order of
-// arrival here; no value does: a row's pieces are joined in their own order.
-__device__ __forceinline__ void add_frequent(const TokenOrder &o, unsigned row, unsigned len) {
-  const unsigned pieces = (len + o.piece - 1) / o.piece;
-  const unsigned long long at = atomicAdd(o.counts, (1ull << 32) | pieces);
-  o.frequent[at >> 32] = make_uint2(row, unsigned(at));  // ascending in the first piece's number
+// ---- items of work -----------------------------------------------------------------------------
+// The bags of a row, in pieces: a frequent token's sum is shared by many warps.  The order of the list
+// depends on the order of arrival here; no value does: where a row is cut follows from the sorted
+// positions alone, and its pieces are joined in their own order.
+// Called by whole warps; `at(i)` is the token at sorted position i, `row` that of position q.
+template <typename At>
+__device__ __forceinline__ void add_item(const TokenOrder &o, bool valid, unsigned q, unsigned row, const At &at) {
+  const unsigned n = unsigned(o.count), piece = o.piece;
+  const bool first = valid && (q == 0 || at(q - 1) != row);
+  // q a multiple: is it inside the row, and with it another multiple before or behind?
+  const auto cut_at = [&](unsigned p) {
+    return (p >= piece && at(p - piece) == row) || (p + piece < n && at(p + piece) == row);
+  };
+  const bool item = first || (valid && (q & (piece - 1)) == 0 && cut_at(q));
+  const unsigned items = __ballot_sync(0xffffffffu, item);
+  if (items == 0) return;
+  const int lane = threadIdx.x & 31, leader = __ffs(items) - 1;
+  unsigned slot = 0;
+  if (lane == leader) slot = atomicAdd(&o.counts[0], unsigned(__popc(items)));
+  slot = __shfl_sync(0xffffffffu, slot, leader) + __popc(items & ((1u << lane) - 1u));
+  if (!item) return;
+  // first position behind q, below `most`, of another row
+  const auto end_of = [&](unsigned most) {
+    unsigned lo = q, hi = most;  // at(lo) is the row's, hi is not or is the end
+    while (hi - lo > 1) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (at(mid) == row) lo = mid;
+      else hi = mid;
+    }
+    return hi;
+  };
+  const unsigned next = (q / piece + 1) * piece;  // the next multiple; within the row it cuts if it is one of two
+  unsigned end;
+  bool whole = first;
+  if (next < n && at(next) == row && cut_at(next)) {
+    end = next;
+    if (first) o.frequent[atomicAdd(&o.counts[1], 1u)] = make_uint4(q, end_of(n), row, 0u);
+    whole = false;
+  } else {
+    end = end_of(n - q > 2 * piece ? q + 2 * piece : n);
+  }
+  o.item[slot] = make_uint4(q, end, row, whole ? 1u : 0u);
+  if (first) o.named[row] = 1;
 }
 
-__global__ void order_plan_kernel(TokenOrder o) {
-  for (long long v = blockIdx.x * (long long)blockDim.x + threadIdx.x; v < o.rows; v += (long long)gridDim.x * blockDim.x) {
-    const unsigned len = o.begin[v + 1] - o.begin[v];
-    if (len > o.piece) add_frequent(o, unsigned(v), len);
+__global__ void order_items_kernel(TokenOrder o, const unsigned *__restrict__ key) {
+  const long long step = (long long)gridDim.x * blockDim.x;
+  for (long long q0 = blockIdx.x * (long long)blockDim.x + (threadIdx.x & ~31u); q0 < o.count; q0 += step) {
+    const long long q = q0 + (threadIdx.x & 31);
+    const unsigned row = q < o.count ? key[q] : 0xffffffffu;
+    add_item(o, q < o.count && row < o.rows, unsigned(q), row, [&](unsigned i) { return key[i]; });
   }
+}
+
+// Where the sum of the piece that begins at position q goes.  Of the pieces that begin within one run of
+// `piece` positions at most two belong to cut rows: one that begins with the run, and the first one of a
+// row that ends beyond it.
+__device__ __forceinline__ size_t slot_of(unsigned q, unsigned piece) {
+  return size_t(q / piece) * 2 + ((q & (piece - 1)) != 0 ? 1 : 0);
 }
 
 // ---- the gradient ----------------------------------------------------------------------------
 struct GradLanes {
-  int tx_bits;      // lanes across the columns
-  int ly_row_bits;  // lanes along the bags of a row
-  int ly_item_bits; // ... of a piece of a frequent row
-  int rows_per_group;
+  int tx_bits, ly_bits;  // of a sum: lanes across the columns, lanes along the bags
+  int zero_bits;         // lanes across the columns of an untouched row
 };
 
 constexpr int kGradThreads = 256;
@@ -443,85 +511,108 @@ __device__ __forceinline__ void write_row(const LookupGradLaunch &a, long long r
   }
 }
 
-// CTAs below item_blocks sum the pieces of frequent rows into `partial` [piece][dim]; the others
-// take the rows of the table in order: zeros where no bag names a row, else its sum.  
+// CTAs below item_blocks sum the items' bags: a whole row is written at once, a piece of a frequent one
+// goes to `partial`.  The other CTAs write the zeros of the rows that no bag names, kZeroRows rows a
+// group of lanes: the marks of all of them are read at once, and the stores wait for nothing else.
+constexpr int kZeroRows = 8;
 template <typename T, typename O, int VEC, int U>
 __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLaunch a, TokenOrder o, GradLanes sh, int vecs,
                                                                    int chunks, unsigned item_blocks, float *partial) {
-  const int tx = 1 << sh.tx_bits, lane = threadIdx.x & (tx - 1);
+  overlap_release();
+  overlap_wait();
   if (blockIdx.x < item_blocks) {
-    const int ly = 1 << sh.ly_item_bits, slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
-    const int bits = sh.tx_bits + sh.ly_item_bits;
-    const unsigned group = threadIdx.x >> bits, groups = kGradThreads >> bits;
-    const unsigned long long counts = *o.counts;
-    const unsigned items = unsigned(counts), n_frequent = unsigned(counts >> 32);
-    for (unsigned i0 = blockIdx.x * groups; i0 < items; i0 += item_blocks * groups) {
-      const unsigned i = i0 + group;
-      unsigned p0 = 0, p1 = 0;
-      if (i < items) {  // the last frequent row whose pieces start at or below i
-        unsigned lo = 0, hi = n_frequent;
-        while (hi - lo > 1) {
-          const unsigned mid = (lo + hi) / 2;
-          if (o.frequent[mid].y <= i) lo = mid;
-          else hi = mid;
-        }
-        const uint2 f = o.frequent[lo];
-        const unsigned end = o.begin[f.x + 1];
-        p0 = o.begin[f.x] + (i - f.y) * o.piece;
-        p1 = end - p0 > o.piece ? p0 + o.piece : end;
-      }
-      for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
-        const int c0 = chunk * (tx * U) + lane;
-        float sum[U][VEC];
-        sum_bags<T, VEC, U>(a, o.bag, p0, p1, slice, ly, tx, c0, vecs, sum);
-        if (slice == 0 && i < items) {
+    const int tx = 1 << sh.tx_bits, lane = threadIdx.x & (tx - 1);
+    const int ly = 1 << sh.ly_bits, slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
+    const int bits = sh.tx_bits + sh.ly_bits;
+    const unsigned groups = kGradThreads >> bits;
+    const long long items = (long long)o.counts[0] * chunks;
+    for (long long i0 = (long long)blockIdx.x * groups; i0 < items; i0 += (long long)item_blocks * groups) {
+      const long long i = i0 + (threadIdx.x >> bits);
+      // neighbouring groups take the chunks of one row
+      const long long n = chunks == 1 ? i : items >> 32 ? i / chunks : unsigned(i) / unsigned(chunks);
+      const uint4 it = i < items ? o.item[n] : make_uint4(0, 0, 0, 0);
+      const int c0 = int(i - n * chunks) * (tx * U) + lane;
+      float sum[U][VEC];
+      sum_bags<T, VEC, U>(a, o.bag, it.x, it.y, slice, ly, tx, c0, vecs, sum);
+      if (i < items && slice == 0) {
+        if (it.w) {
+          write_row<O, VEC, U>(a, it.z, c0, tx, vecs, sum);
+        } else {
+          float *to = partial + slot_of(it.x, o.piece) * size_t(a.dim);
 #pragma unroll
           for (int u = 0; u < U; ++u)
             if (c0 + u * tx < vecs) {
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) partial[(size_t(i) * vecs + (c0 + u * tx)) * VEC + j] = sum[u][j];
+              for (int j = 0; j < VEC; ++j) to[(long long)(c0 + u * tx) * VEC + j] = sum[u][j];
             }
         }
       }
     }
     return;
   }
-  // A warp takes rows_per_warp rows a lane group, and reads where their bags begin in one access: it
-  // knows the untouched rows at once, and their zeros are stores that wait for nothing.
-  const int ly = 1 << sh.ly_row_bits, slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
-  const int bits = sh.tx_bits + sh.ly_row_bits;
-  const int groups = 32 >> bits, group = (threadIdx.x & 31) >> bits;  // of a warp
-  const long long warp = (blockIdx.x - item_blocks) * (long long)(kGradThreads / 32) + threadIdx.x / 32;
-  const int span = groups * sh.rows_per_group;  // at most 32
-  const long long row0 = warp * span;
-  unsigned my_begin = 0, my_end = 0;
-  if ((threadIdx.x & 31) < span && row0 + (threadIdx.x & 31) < o.rows) {
-    my_begin = o.begin[row0 + (threadIdx.x & 31)];
-    my_end = o.begin[row0 + (threadIdx.x & 31) + 1];
+  const int tx = 1 << sh.zero_bits, groups = kGradThreads >> sh.zero_bits;
+  const long long row0 = (blockIdx.x - item_blocks) * (long long)(groups * kZeroRows) + (threadIdx.x >> sh.zero_bits);
+  unsigned char named[kZeroRows];
+#pragma unroll
+  for (int r = 0; r < kZeroRows; ++r) named[r] = row0 + r * groups < o.rows ? o.named[row0 + r * groups] : 1;
+  float zero[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) zero[j] = 0.0f;
+#pragma unroll
+  for (int r = 0; r < kZeroRows; ++r) {
+    if (named[r]) continue;
+    O *out = static_cast<O *>(a.out) + (row0 + r * groups) * a.out_stride;
+    for (int c = threadIdx.x & (tx - 1); c < vecs; c += tx) store_vec<O, VEC>(out + (long long)c * VEC, zero);
   }
-  const unsigned touched = __ballot_sync(0xffffffffu, my_begin != my_end);
-  for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
-    const int c0 = chunk * (tx * U) + lane;
-    if (!a.accumulate && slice == 0) {
-      float zero[VEC];
+}
+
+// The pieces of a frequent row, joined in their order: eight groups of 32 lanes take every eighth piece
+// of 32 vectors of columns, and the groups' sums are added one after another.
+template <typename O, int VEC>
+__global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGradLaunch a, TokenOrder o, int vecs, int chunks,
+                                                                        const float *__restrict__ partial) {
+  __shared__ float part[kGradThreads * VEC];
+  constexpr int kSlices = kGradThreads / 32, K = 4;
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
+  overlap_release();
+  overlap_wait();
+  const unsigned frequent = o.counts[1];
+  for (unsigned h = blockIdx.x; h < frequent; h += gridDim.x) {
+    const uint4 f = o.frequent[h];
+    const unsigned second = (f.x / o.piece + 1) * o.piece;  // pieces: the first, then one at every multiple
+    const unsigned pieces = 1 + (f.y - second + o.piece - 1) / o.piece;
+    for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+      const int c = chunk * 32 + lane;
+      float sum[1][VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) zero[j] = 0.0f;
-      for (int r = group; r < span; r += groups) {
-        if ((touched >> r & 1u) || row0 + r >= o.rows) continue;
-        O *out = static_cast<O *>(a.out) + (row0 + r) * a.out_stride;
+      for (int j = 0; j < VEC; ++j) sum[0][j] = 0.0f;
+      for (unsigned k0 = slice; k0 < pieces; k0 += kSlices * K) {
+        float v[K][VEC];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (c0 + u * tx < vecs) store_vec<O, VEC>(out + (long long)(c0 + u * tx) * VEC, zero);
+        for (int k = 0; k < K; ++k) {
+          const unsigned n = k0 + k * kSlices;
+          const bool in = n < pieces && c < vecs;
+          const unsigned q = n == 0 ? f.x : second + (n - 1) * o.piece;
+          const float *at = partial + slot_of(q, o.piece) * size_t(a.dim) + (long long)c * VEC;
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) v[k][j] = in ? at[j] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) sum[0][j] += v[k][j];
       }
-    }
-    for (int r0 = 0; r0 < span; r0 += groups) {
-      if ((touched >> r0 & ((groups == 32 ? 0u : 1u << groups) - 1u)) == 0) continue;  // the same for the whole warp
-      const int r = r0 + group;
-      const unsigned p0 = __shfl_sync(0xffffffffu, my_begin, r), p1 = __shfl_sync(0xffffffffu, my_end, r);
-      const bool mine = p0 != p1 && p1 - p0 <= o.piece;
-      float sum[U][VEC];
-      sum_bags<T, VEC, U>(a, o.bag, p0, mine ? p1 : p0, slice, ly, tx, c0, vecs, sum);
-      if (mine && slice == 0) write_row<O, VEC, U>(a, row0 + r, c0, tx, vecs, sum);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) part[j * kGradThreads + threadIdx.x] = sum[0][j];
+      __syncthreads();
+      if (slice == 0 && c < vecs) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          for (int g = 1; g < kSlices; ++g) sum[0][j] += part[j * kGradThreads + g * 32 + lane];
+        }
+        write_row<O, VEC, 1>(a, f.z, c, 0, vecs, sum);
+      }
     }
   }
 }
@@ -654,49 +745,35 @@ __global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLa
   }
 }
 
-// the pieces of a frequent row, joined in their order
-template <typename O, int VEC>
-__global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGradLaunch a, TokenOrder o, int vecs,
-                                                                        const float *__restrict__ partial) {
-  const unsigned n_frequent = unsigned(*o.counts >> 32);
-  for (unsigned h = blockIdx.x; h < n_frequent; h += gridDim.x) {
-    const uint2 f = o.frequent[h];
-    const unsigned pieces = (o.begin[f.x + 1] - o.begin[f.x] + o.piece - 1) / o.piece;
-    for (int c = blockIdx.y * kGradThreads + threadIdx.x; c < vecs; c += gridDim.y * kGradThreads) {
-      float sum[1][VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[0][j] = 0.0f;
-#pragma unroll 4
-      for (unsigned k = 0; k < pieces; ++k) {
-        const float *at = partial + (size_t(f.y + k) * vecs + c) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[0][j] += at[j];
-      }
-      write_row<O, VEC, 1>(a, f.x, c, 0, vecs, sum);
-    }
-  }
-}
-
 // ---- the sort of a batch in one launch -------------------------------------------------------
 // Up to 131072 tokens are sorted by one cluster of at most eight CTAs: the pairs stay in shared
 // memory, a pass exchanges digit counts and moves the pairs through distributed shared memory, and
-// the rows' first positions and the frequent rows come out of the same launch.  (The general sort
-// takes three launches a pass and leaves the device to a few tiles at these sizes: 16384 tokens over
-// 131072 rows took 109 us.)
+// the rows' first positions and the items come out of the same launch.  Bound by latency: barriers and
+// dependent accesses.  (The general sort takes three launches a pass and leaves the device to a few
+// tiles at these sizes: 16384 tokens over 131072 rows took 109 us.)
 namespace cg = cooperative_groups;
-constexpr int kClusterThreads = 1024, kMostClusterBits = 9, kMostClusterDigits = 1 << kMostClusterBits;
-constexpr int kLongGaps = 512;
+constexpr int kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
+constexpr int kMostClusterBits = 9, kMostClusterDigits = 1 << kMostClusterBits;
+static_assert(kMostClusterDigits == kClusterThreads, "a thread takes a digit");
+constexpr int kMostClusterItems = 32;
 
 struct ClusterSortMemory {
-  unsigned short warp_cnt[kClusterThreads / 32][kMostClusterDigits];
+  unsigned short warp_cnt[kClusterWarps][kMostClusterDigits];
   unsigned cta_cnt[kMostClusterDigits];
   unsigned base[kMostClusterDigits];
-  unsigned warp_sum[kClusterThreads / 32];
-  unsigned n_long;
-  uint2 long_gap[kLongGaps];  // rows first .. last that begin at long_at
-  unsigned long_at[kLongGaps];
-  unsigned last_key;
+  unsigned warp_sum[kClusterWarps];
 };
+
+// lanes of the warp with the same digit: a ballot a bit (the match instruction takes its time with many
+// different values)
+__device__ __forceinline__ unsigned lanes_with(unsigned digit, int bits) {
+  unsigned same = 0xffffffffu;
+  for (int i = 0; i < bits; ++i) {
+    const unsigned set = __ballot_sync(0xffffffffu, digit >> i & 1u);
+    same &= digit >> i & 1u ? set : ~set;
+  }
+  return same;
+}
 
 template <int ITEMS>
 __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass p, TokenOrder o, int digit_bits, int passes) {
@@ -717,17 +794,18 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
     bag[j] = 0;
     if (i < p.n) sort_pair(p, i, key[j], bag[j]);
   }
-  if (rank == 0 && tid == 0) *o.counts = 0;
-  if (tid == 0) m.n_long = 0;
+  if (rank == 0 && tid < 2) o.counts[tid] = 0;
+  for (long long i = (long long)rank * kClusterThreads + tid; i < (p.rows + 15) / 16; i += ctas * kClusterThreads)
+    reinterpret_cast<uint4 *>(o.named)[i] = make_uint4(0u, 0u, 0u, 0u);  // padded to 256 bytes
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
-    for (int i = tid; i < (kClusterThreads / 32) * kMostClusterDigits / 2; i += kClusterThreads)
+    for (int i = tid; i < kClusterWarps * kMostClusterDigits / 2; i += kClusterThreads)
       reinterpret_cast<unsigned *>(&m.warp_cnt[0][0])[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
       const unsigned digit = (key[j] >> shift) & (digits - 1);
-      const unsigned same = __match_any_sync(0xffffffffu, digit);
+      const unsigned same = lanes_with(digit, digit_bits);
       const unsigned below = __popc(same & ((1u << lane) - 1u));
       rank_in[j] = m.warp_cnt[w][digit] + below;
       __syncwarp();
@@ -736,23 +814,29 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
     }
     __syncthreads();
     if (tid < digits) {
-      unsigned run = 0;
-      for (int i = 0; i < kClusterThreads / 32; ++i) {
-        const unsigned c = m.warp_cnt[i][tid];
-        m.warp_cnt[i][tid] = (unsigned short)run;  // at most kSpan - 1 = 16383
-        run += c;
+      unsigned c[kClusterWarps], run = 0;
+#pragma unroll
+      for (int i = 0; i < kClusterWarps; ++i) c[i] = m.warp_cnt[i][tid];
+#pragma unroll
+      for (int i = 0; i < kClusterWarps; ++i) {
+        m.warp_cnt[i][tid] = (unsigned short)run;  // below kSpan, at most 16384
+        run += c[i];
       }
       m.cta_cnt[tid] = run;
     }
     cluster.sync();  // the counts are there, and every CTA holds its pairs in registers
     unsigned before = 0, total = 0;
-    if (tid < digits)
-      for (int r = 0; r < ctas; ++r) {
-        const unsigned c = cluster.map_shared_rank(m.cta_cnt, r)[tid];
-        if (r < rank) before += c;
-        total += c;
+    if (tid < digits) {
+      unsigned c[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) c[r] = r < ctas ? cluster.map_shared_rank(m.cta_cnt, r)[tid] : 0u;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if (r < rank) before += c[r];
+        total += c[r];
       }
-    // exclusive sum of the digits' totals over the CTA's first warps
+    }
+    // exclusive sum of the digits' totals
     unsigned x = total;
     for (int d = 1; d < 32; d <<= 1) {
       const unsigned y = __shfl_up_sync(0xffffffffu, x, d);
@@ -761,8 +845,9 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
     if (lane == 31) m.warp_sum[w] = x;
     __syncthreads();
     unsigned ahead = 0;
-    for (int i = 0; i < w && i < kMostClusterDigits / 32; ++i) ahead += m.warp_sum[i];
-    if (tid < digits) m.base[tid] = ahead + x - total + before;
+#pragma unroll
+    for (int i = 0; i < kClusterWarps; ++i) ahead += i < w ? m.warp_sum[i] : 0u;
+    m.base[tid] = ahead + x - total + before;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
@@ -778,66 +863,17 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
       bag[j] = v.y;
     }
   }
-  if (tid == 0) m.last_key = pair[kSpan - 1].x;
-  cluster.sync();
-  // a position fills the rows behind its predecessor's token up to its own; gaps that would keep one
-  // warp busy for long are left to the whole cluster
-  const long long longest = max(256ll, p.rows / (kLongGaps / 2));
-  const unsigned first_prev = rank == 0 ? 0xffffffffu : *cluster.map_shared_rank(&m.last_key, rank - 1);
   for (int j = 0; j < ITEMS; ++j) {
     const int at = at0 + j * 32;
     const long long q = (long long)rank * kSpan + at;
+    if (q - lane >= p.n) break;  // the same for the whole warp
     const uint2 mine = pair[at];
-    const unsigned k = mine.x, prev = at == 0 ? first_prev : pair[at - 1].x;
-    long long lo = 0, hi = -1, lo_end = 0, hi_end = -1;
-    if (q < p.n) {
-      o.bag[q] = mine.y;
-      lo = q == 0 ? 0 : (long long)prev + 1;
-      hi = k;
-      if (q == p.n - 1) lo_end = (long long)k + 1, hi_end = p.rows;
-    }
-    for (int part = 0; part < 2; ++part) {
-      const long long l0 = part ? lo_end : lo, h0 = part ? hi_end : hi;
-      bool wide = h0 - l0 >= longest;
-      if (wide) {
-        const unsigned slot = atomicAdd(&m.n_long, 1u);
-        if (slot < kLongGaps) {  // always: gaps are disjoint, so fewer than kLongGaps / 2 are that long
-          m.long_gap[slot] = make_uint2(unsigned(l0), unsigned(h0));
-          m.long_at[slot] = unsigned(q + part);
-        }
-      }
-      unsigned todo = __ballot_sync(0xffffffffu, l0 <= h0 && !wide);
-      while (todo) {
-        const int src = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const unsigned l = unsigned(__shfl_sync(0xffffffffu, l0, src)), h = unsigned(__shfl_sync(0xffffffffu, h0, src));
-        const unsigned value = unsigned(__shfl_sync(0xffffffffu, q, src)) + part;
-        for (unsigned v = l + lane; v <= h; v += 32) o.begin[v] = value;
-      }
-    }
+    if (q < p.n) o.bag[q] = mine.y;
+    add_item(o, q < p.n && mine.x < p.rows, unsigned(q), mine.x, [&](unsigned i) {
+      return int(i / kSpan) == rank ? pair[i % kSpan].x : cluster.map_shared_rank(pair, int(i / kSpan))[i % kSpan].x;
+    });
   }
-  cluster.sync();
-  for (int r = 0; r < ctas; ++r) {
-    const ClusterSortMemory &other = *cluster.map_shared_rank(&m, r);
-    const unsigned n_long = other.n_long;
-    for (unsigned g = 0; g < n_long; ++g) {
-      const uint2 gap = other.long_gap[g];
-      const unsigned value = other.long_at[g];
-      for (long long v = (long long)gap.x + rank * kClusterThreads + tid; v <= gap.y; v += ctas * kClusterThreads)
-        o.begin[v] = value;
-    }
-  }
-  __threadfence();
-  cluster.sync();  // begin is complete; nobody reads another CTA's shared memory after this
-  for (int j = 0; j < ITEMS; ++j) {
-    const int at = at0 + j * 32;
-    const long long q = (long long)rank * kSpan + at;
-    const unsigned k = pair[at].x, prev = at == 0 ? first_prev : pair[at - 1].x;
-    if (q < p.n && k < p.rows && (q == 0 || prev != k)) {
-      const unsigned len = __ldcg(o.begin + k + 1) - unsigned(q);
-      if (len > o.piece) add_frequent(o, k, len);
-    }
-  }
+  cluster.sync();  // no CTA's memory goes while another may look at it
 }
 
 inline int grid_of(long long n, int threads, int per_sm) {
@@ -926,7 +962,8 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   const int groups = kLookupThreads >> (sh.tx_bits + sh.ly_bits);
   const int chunks = int((vecs + (int64_t(u) << sh.tx_bits) - 1) / (int64_t(u) << sh.tx_bits));
   const dim3 grid(unsigned((a.tokens.bags + groups - 1) / groups), unsigned(std::min(chunks, 65535)));
-  if (pooled) lookup_kernel<T, O, VEC, 1, 8><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  if (pooled && sh.tx_bits >= 3) lookup_kernel<T, O, VEC, true><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  else if (pooled) lookup_kernel<T, O, VEC, false><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
   else if (u == 4) lookup_rows_kernel<T, O, VEC, 4><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
   else lookup_rows_kernel<T, O, VEC, 1><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
 }
@@ -993,12 +1030,10 @@ unsigned piece_of(int64_t count) {
   while (p < 4096 && int64_t(p) * 8192 < count) p *= 2;
   return p;
 }
-// a frequent row has more than `piece` bags, so its pieces are fewer than two for every `piece` bags
-int64_t most_pieces(int64_t count) { return count / piece_of(count) * 2 + 1; }
 }  // namespace
 
 namespace {
-constexpr int64_t kMostClusterTokens = int64_t(8) * kClusterThreads * 16;
+constexpr int64_t kMostClusterTokens = int64_t(8) * kClusterThreads * kMostClusterItems;
 // An order is kept by runs of bags where a row has 32 bags a run or more, on average: then a run's
 // sums are worth more than the look at where its bags begin.
 int blocks_of(int64_t bags, int64_t per_bag, int64_t rows) {
@@ -1016,14 +1051,16 @@ TokenOrder::TokenOrder(void *mem, int64_t bags_, int64_t per_bag, int64_t rows_)
     at += pad256(b);
     return static_cast<void *>(q);
   };
-  counts = static_cast<unsigned long long *>(take(256));
-  begin = static_cast<unsigned *>(take(size_t(blocks) * size_t(rows + 1) * 4));
-  bag = nullptr, local = nullptr, frequent = nullptr;
+  counts = static_cast<unsigned *>(take(256));
+  bag = nullptr, local = nullptr, begin = nullptr, frequent = item = nullptr, named = nullptr;
   if (blocks > 1) {
+    begin = static_cast<unsigned *>(take(size_t(blocks) * size_t(rows + 1) * 4));
     local = static_cast<unsigned short *>(take(size_t(count) * 2));
   } else {
+    named = static_cast<unsigned char *>(take(size_t(rows)));
     bag = static_cast<unsigned *>(take(size_t(count) * 4));
-    frequent = static_cast<uint2 *>(take(size_t(count / piece + 1) * 8));
+    item = static_cast<uint4 *>(take(size_t(most_items()) * 16));
+    frequent = static_cast<uint4 *>(take(size_t(count / piece + 1) * 16));
   }
   bytes = at;
 }
@@ -1070,8 +1107,8 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
   p.first = true;
   p.by_slot = std::abs(t.bag_stride) < std::abs(t.token_stride);
   if (n > 0 && n <= kMostClusterTokens) {
-    if (n <= int64_t(8) * kClusterThreads * 2) launch_cluster_order<2>(p, o, s);
-    else launch_cluster_order<16>(p, o, s);
+    if (n <= int64_t(8) * kClusterThreads * 4) launch_cluster_order<4>(p, o, s);
+    else launch_cluster_order<kMostClusterItems>(p, o, s);
     return;
   }
   const int64_t keys = o.blocks * (o.rows + 1) - 1;  // the largest key
@@ -1100,11 +1137,18 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
     }
     sorted = sc.key[(passes - 1) & 1];
   }
-  order_begin_kernel<<<grid_of(n + 1, 256, 8), 256, 0, s>>>(sorted, n, keys, o.begin);
-  ARB_CUDA(cudaMemsetAsync(o.counts, 0, sizeof *o.counts, s));
-  if (o.blocks == 1) order_plan_kernel<<<grid_of(o.rows, 256, 8), 256, 0, s>>>(o);
+  if (o.blocks > 1) {
+    order_begin_kernel<<<grid_of(n + 1, 256, 8), 256, 0, s>>>(sorted, n, keys, o.begin);
+    count_launch();
+  } else {
+    ARB_CUDA(cudaMemsetAsync(o.counts, 0, 2 * sizeof *o.counts, s));
+    if (o.rows > 0) ARB_CUDA(cudaMemsetAsync(o.named, 0, size_t(o.rows), s));
+    if (n > 0) {
+      order_items_kernel<<<grid_of(n, 256, 8), 256, 0, s>>>(o, sorted);
+      count_launch();
+    }
+  }
   ARB_CUDA(cudaGetLastError());
-  count_launch(2);
 }
 
 namespace {
@@ -1164,7 +1208,7 @@ void blocked_grad(const LookupGradLaunch &a, const TokenOrder &o, int vec, float
 
 size_t lookup_grad_scratch(const TokenOrder &o, int64_t dim) {
   if (o.blocks > 1) return pad256(size_t(splits_of(o, dim)) * size_t(o.rows) * size_t(dim) * sizeof(float));
-  return o.count > o.piece ? pad256(size_t(most_pieces(o.count)) * size_t(dim) * sizeof(float)) : 0;
+  return o.count > o.piece ? pad256((size_t(o.count / o.piece) + 1) * 2 * size_t(dim) * sizeof(float)) : 0;
 }
 
 namespace {
@@ -1174,28 +1218,24 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   const int vecs = int(a.dim / VEC);
   GradLanes sh;
   sh.tx_bits = std::min(5, log2_floor(std::max(1, (vecs + U - 1) / U * 2 - 1)));
-  sh.ly_item_bits = 5 - sh.tx_bits;
-  // a row is named by count / rows bags: that many lanes share it
-  sh.ly_row_bits = 0;
-  while (sh.tx_bits + sh.ly_row_bits < 5 && (o.rows << sh.ly_row_bits) < o.count) ++sh.ly_row_bits;
+  // a row has count / rows bags, a piece no more than `piece`: that many lanes share them
+  const int64_t length = std::min<int64_t>(o.piece, o.count / std::max<int64_t>(1, std::min(o.count, o.rows)));
+  sh.ly_bits = 0;
+  while (sh.tx_bits + sh.ly_bits < 5 && (int64_t(1) << sh.ly_bits) < length) ++sh.ly_bits;
+  sh.zero_bits = std::min(8, log2_floor(std::max(1, vecs * 2 - 1)));
   const int chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
-  // rows a warp: as many as leave the device four CTAs an SM, at most 32
-  const int warp_groups = 32 >> (sh.tx_bits + sh.ly_row_bits);
-  sh.rows_per_group = 1;
-  while (warp_groups * sh.rows_per_group < 32 &&
-         o.rows * chunks / (2 * warp_groups * sh.rows_per_group) >= int64_t(device_sm_count()) * 4 * (kGradThreads / 32))
-    sh.rows_per_group *= 2;
-  const int64_t groups = (kGradThreads / 32) * warp_groups * sh.rows_per_group;  // rows a CTA
-  const int64_t item_groups = kGradThreads >> (sh.tx_bits + sh.ly_item_bits);
-  unsigned item_blocks = 0;
-  if (o.count > o.piece)
-    item_blocks = unsigned(std::min<int64_t>((most_pieces(o.count) + item_groups - 1) / item_groups, device_sm_count() * 16));
-  const dim3 grid(unsigned((o.rows + groups - 1) / groups) + item_blocks, unsigned(std::min(chunks, 65535)));
-  lookup_grad_kernel<T, O, VEC, U><<<grid, kGradThreads, 0, s>>>(a, o, sh, vecs, chunks, item_blocks, partial);
-  if (item_blocks) {
-    const dim3 join(unsigned(std::min<int64_t>(o.count / o.piece, device_sm_count() * 8)),
-                    unsigned(std::min<int64_t>((vecs + kGradThreads - 1) / kGradThreads, 65535)));
-    lookup_grad_join_kernel<O, VEC><<<join, kGradThreads, 0, s>>>(a, o, vecs, partial);
+  const int64_t groups = kGradThreads >> (sh.tx_bits + sh.ly_bits);
+  const int64_t item_blocks = std::min<int64_t>((o.most_items() * chunks + groups - 1) / groups, int64_t(device_sm_count()) * 64);
+  const int64_t zero_groups = kGradThreads >> sh.zero_bits;
+  const int64_t zero_blocks = a.accumulate ? 0 : (o.rows + zero_groups * kZeroRows - 1) / (zero_groups * kZeroRows);
+  if (item_blocks + zero_blocks == 0) return;
+  launch_overlapped(lookup_grad_kernel<T, O, VEC, U>, dim3(unsigned(item_blocks + zero_blocks)), dim3(kGradThreads), 0, s,
+                    a, o, sh, vecs, chunks, unsigned(item_blocks), partial);
+  if (o.count > o.piece) {
+    const int join_chunks = (vecs + 31) / 32;
+    const dim3 join(unsigned(std::min<int64_t>(o.count / o.piece, device_sm_count() * 2)), unsigned(std::min(join_chunks, 65535)));
+    launch_overlapped(lookup_grad_join_kernel<O, VEC>, join, dim3(kGradThreads), 0, s, a, o, vecs, join_chunks,
+                      static_cast<const float *>(partial));
     count_launch();
   }
 }

@@ -5,6 +5,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <vector>
 
@@ -39,7 +40,7 @@ void launch_lookup(const LookupLaunch &a, cudaStream_t s);
 // The tokens' order, in memory of the caller: for every row v of the table, the bags that name it,
 // in a fixed order that only the tokens decide.
 //
-// blocks == 1: bag[begin[v] .. begin[v + 1]).
+// blocks == 1: the bags sorted by token, and the sorted positions cut into items of work.
 // blocks > 1: many bags of several tokens over few rows (the leaves of a forest).  The order is kept
 // apart for every run of kBlockBags bags: within run k the bags of row v are
 // local[begin[k * (rows + 1) + v] .. begin[k * (rows + 1) + v + 1]), numbered from the run's first one
@@ -48,14 +49,17 @@ constexpr int kBlockBits = 14, kBlockBags = 1 << kBlockBits;
 struct TokenOrder {
   int64_t bags, count, rows;
   int blocks;
-  unsigned *bag;          // count
-  unsigned short *local;  // count
-  unsigned *begin;        // blocks * (rows + 1)
-  // rows named by more than `piece` bags (blocks == 1 only): (row, number of its first piece), and
-  // how many there are: the rows in the upper half of *counts, their pieces in the lower one
+  unsigned short *local;  // blocks > 1: count
+  unsigned *begin;        // blocks > 1: blocks * (rows + 1)
+  unsigned *bag;          // blocks == 1, and the rest: count
+  // The bags of a row are cut at multiples of `piece` (a power of two) where two of these lie inside
+  // them, so an item has fewer than 2 * piece bags.
   unsigned piece;
-  uint2 *frequent;
-  unsigned long long *counts;
+  uint4 *item;           // first position, end, row, 1 if these are all the row's bags
+  uint4 *frequent;       // the same of a whole row that is cut
+  unsigned char *named;  // per row: a bag names it
+  unsigned *counts;      // items, cut rows
+  int64_t most_items() const { return count / piece + (count < rows ? count : rows) + 1; }
   size_t bytes;
   TokenOrder(void *mem, int64_t bags, int64_t per_bag, int64_t rows);
 };
@@ -78,7 +82,7 @@ void launch_lookup_grad(const LookupGradLaunch &a, const TokenOrder &o, void *sc
 
 // ---- AdamW ---------------------------------------------------------------------------------
 constexpr int kMomentBlock = 128;  // elements of an 8-bit block; tensors' slots are padded to it
-constexpr int kAdamWChunk = 4096;  // elements a CTA takes at a time
+constexpr int kAdamWChunk = 8192;  // elements a CTA takes at a time
 
 struct AdamWTensor {  // device table, one record a tensor
   void *param;
@@ -91,11 +95,22 @@ struct AdamWChunk {
   int tensor;
   int index;  // elements index * kAdamWChunk ..
 };
-struct AdamWState {  // device: the step count and the powers of the betas, advanced by the kernel
-  double beta1_t, beta2_t;
-  long long step;
-  unsigned done;   // CTAs of the running step that have finished
-  unsigned pad;
+struct AdamWState {  // device: the step count and what follows from it, advanced by the kernel
+  double beta1_t, beta2_t;  // powers of the betas for the coming step
+  double inv_bc1;           // 1 / (1 - beta1_t)
+  float inv_root_bc2;       // 1 / sqrt(1 - beta2_t)
+  unsigned done;            // CTAs of the running step that have finished
+  long long step;           // steps taken
+  __host__ __device__ void derive() {
+    inv_bc1 = 1.0 / (1.0 - beta1_t);
+    inv_root_bc2 = float(1.0 / sqrt(1.0 - beta2_t));
+  }
+  __host__ __device__ void advance(double beta1, double beta2) {
+    beta1_t *= beta1;
+    beta2_t *= beta2;
+    step += 1;
+    derive();
+  }
 };
 struct AdamWLaunch {
   const AdamWTensor *tensors;

@@ -104,10 +104,11 @@ struct AdamWLayout {
 
 void put_step(AdamW *o, int64_t step, cudaStream_t s) {
   AdamWState st;
-  st.beta1_t = std::pow(o->launch.beta1, double(step));
-  st.beta2_t = std::pow(o->launch.beta2, double(step));
+  st.beta1_t = std::pow(o->launch.beta1, double(step) + 1);
+  st.beta2_t = std::pow(o->launch.beta2, double(step) + 1);
   st.step = step;
-  st.done = st.pad = 0;
+  st.done = 0;
+  st.derive();
   ARB_CUDA(cudaMemcpyAsync(o->launch.state, &st, sizeof st, cudaMemcpyHostToDevice, s));
   ARB_CUDA(cudaStreamSynchronize(s));
 }
