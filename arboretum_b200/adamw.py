@@ -5,9 +5,11 @@ import ctypes
 import torch
 
 from .core import _LIB, _call_and_throw_if_error
-from .lookup import _TYPE, _extent, _float_type, _memory, _one_device, _stream, _tensor
+from .lookup import _tensors
 
 __all__ = ["AdamW"]
+
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class _Param(ctypes.Structure):
@@ -49,15 +51,16 @@ class AdamW(object):
         if not params:
             raise ValueError("params is empty")
         for p in params:
-            _float_type(_tensor(p, "a parameter"), "a parameter")
+            if not isinstance(p, torch.Tensor) or p.dtype not in _TYPE:
+                raise TypeError("a parameter must be a float32, bfloat16 or float16 tensor")
             if not p.is_contiguous():
                 raise ValueError("a parameter is not contiguous")
-        extents = sorted(_extent(p) for p in params if p.numel())
+        extents = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
         for a, b in zip(extents, extents[1:]):
             if b[0] < a[1]:
                 raise ValueError("two parameters share memory")
-        self._config = _Config(float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(state_bits),
-                               int(seed) & 0xFFFFFFFF)
+        config = _Config(float(betas[0]), float(betas[1]), float(eps), float(weight_decay), int(state_bits),
+                         int(seed) & 0xFFFFFFFF)
         if state_bits not in (8, 32):
             raise ValueError("state_bits must be 8 or 32")
         self.lr = self._rate(lr)
@@ -70,11 +73,12 @@ class AdamW(object):
         length, size = ctypes.c_int64(0), ctypes.c_int64(0)
         _call_and_throw_if_error(_LIB.AAdamWBytes(table, len(params), ctypes.byref(length), ctypes.byref(size)))
         assert length.value == end
-        index = None
         for p in params:
-            index = _one_device(params[0], parameter=p)
+            if p.device.type != "cuda":
+                raise ValueError("the parameters must be CUDA tensors")
+            if p.device != params[0].device:
+                raise ValueError("a parameter is on %s, the others are on %s" % (p.device, params[0].device))
         self.device = params[0].device
-        self._index = index
         state = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
         zeros = lambda n, t: torch.zeros(n, dtype=t, device=self.device)  # noqa: E731
         self.moment1, self.moment2 = zeros(end, state), zeros(end, state)
@@ -85,24 +89,10 @@ class AdamW(object):
             self.master = zeros(end, torch.float32)
             for p, at in zip(params, self.slots):
                 self.master[at:at + p.numel()].copy_(p.detach().reshape(-1))
-        self._grads = None if grads is None else self._pointers(grads)
-        self._bound = None if grads is None else list(grads)
-        self._versions = [p for p in params if p.requires_grad]
-        self._stream = _stream(index)
-        self._workspace = _memory(size.value, self.device)
-        for name in ("moment1", "moment2", "scale1", "scale2", "master"):
-            buf = getattr(self, name)
-            setattr(self._config, name, None if buf is None else buf.data_ptr())
+        workspace = zeros(size.value, torch.uint8)
         torch.cuda.current_stream(self.device).synchronize()  # the library uploads its table on its own
-        self._handle = ctypes.c_void_p()
-        _call_and_throw_if_error(_LIB.AAdamWCreate(table, len(params), ctypes.byref(self._config),
-                                                   self._workspace.data_ptr(), index, ctypes.byref(self._handle)))
-
-    def __del__(self):
-        handle = getattr(self, "_handle", None)
-        if handle is not None and _LIB is not None:
-            _LIB.AFreeAdamW(handle)
-            self._handle = None
+        self._optimizer = _tensors.adamw(params, bytes(config), (self.moment1, self.moment2, self.scale1, self.scale2,
+                                                                 self.master, workspace), grads)
 
     @staticmethod
     def _rate(lr):
@@ -112,70 +102,17 @@ class AdamW(object):
             return lr
         return float(lr)
 
-    def _pointers(self, grads):
-        """(address array, all float32?) of one gradient, or None, for every parameter."""
-        if len(grads) != len(self.params):
-            raise ValueError("%d gradients for %d parameters" % (len(grads), len(self.params)))
-        same, single, at = True, True, []
-        for g, p in zip(grads, self.params):
-            if g is None:
-                at.append(None)
-                continue
-            if not isinstance(g, torch.Tensor) or g.shape != p.shape or not g.is_contiguous():
-                raise ValueError("a gradient must be a contiguous tensor of its parameter's shape")
-            if g.device != p.device:
-                raise ValueError("a gradient is on %s, its parameter on %s" % (g.device, p.device))
-            if g.dtype != torch.float32:
-                single = False
-            if g.dtype != p.dtype:
-                same = False
-            at.append(g.data_ptr())
-        if not same and not single:
-            raise TypeError("gradients must have their parameters' types, or all be float32")
-        return (ctypes.c_void_p * len(at))(*at), not same
-
     def step(self, grads=None, lr=None, grad_scale=None):
         """One step.  grads: one tensor, or None (that parameter and its moments stay as they are),
         for every parameter; by default the tensors given at construction.  lr: a number or a
         float32 CUDA tensor of one element, by default the constructor's.  grad_scale: a float32
         CUDA tensor of one element that multiplies every gradient (clipping, loss scaling)."""
-        if grads is None:
-            if self._grads is None:
-                raise ValueError("no gradients: pass grads to step() or to the constructor")
-            pointers, single = self._grads
-        else:
-            pointers, single = self._pointers(grads)
-        lr = self.lr if lr is None else self._rate(lr)
-        lr_at = scale_at = None
-        if isinstance(lr, torch.Tensor):
-            _one_device(self.params[0], lr=lr)
-            lr, lr_at = 0.0, lr.data_ptr()
-        if grad_scale is not None:
-            if not isinstance(grad_scale, torch.Tensor) or grad_scale.dtype != torch.float32 or grad_scale.numel() != 1:
-                raise TypeError("grad_scale must be a float32 tensor of one element")
-            _one_device(self.params[0], grad_scale=grad_scale)
-            scale_at = grad_scale.data_ptr()
-        stream = _stream(self._index)
-        if stream != self._stream:
-            self._on_another_stream()
-        _call_and_throw_if_error(_LIB.AAdamWStep(self._handle, pointers, len(self.params), int(single), lr, lr_at,
-                                                 scale_at, stream))
-        if self._versions:  # autograd sees that they changed
-            torch.autograd.graph.increment_version(self._versions)
-
-    def _on_another_stream(self):
-        """The optimizer's memory must not be handed out again before that stream is done with it."""
-        current = torch.cuda.current_stream(self.device)
-        for x in (self.moment1, self.moment2, self.scale1, self.scale2, self.master, self._workspace):
-            if x is not None:
-                x.record_stream(current)
+        _tensors.adamw_step(self._optimizer, grads, self.lr if lr is None else lr, grad_scale)
 
     @property
     def steps(self):
         """Steps taken so far (waits for the current stream)."""
-        n = ctypes.c_int64(0)
-        _call_and_throw_if_error(_LIB.AAdamWGetStep(self._handle, ctypes.byref(n), _stream(self._index)))
-        return n.value
+        return _tensors.adamw_count(self._optimizer, None)
 
     def state_dict(self):
         """The step count and the buffers themselves (no copies)."""
@@ -197,7 +134,7 @@ class AdamW(object):
                 raise ValueError("%s must be %d elements of %s" % (k, x.numel(), x.dtype))
         for k in mine:
             getattr(self, k).copy_(state[k])
-        _call_and_throw_if_error(_LIB.AAdamWSetStep(self._handle, int(state["step"]), _stream(self._index)))
+        _tensors.adamw_count(self._optimizer, int(state["step"]))
 
     def moments(self, k):
         """First and second moment of parameter ``k`` as float32 tensors of its shape."""

@@ -18,6 +18,7 @@ SOURCES = ["abi.cu", "garden.cu", "hist.cu", "split.cu", "partition.cu", "object
            "lookup.cu", "adamw.cu", "operators_abi.cu"]
 HEADERS = ["common.cuh", "config.h", "gain.cuh", "garden.h", "json.h", "kernels.cuh", "exchange.h", "abi.h", "operators.h",
            "vec.cuh"]
+BINDINGS = os.path.join(HERE, "_tensors.so")  # the operators on torch tensors
 NVCC = os.environ.get("NVCC", "nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "--fmad=false", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "-ccbin", "/usr/bin/g++"]
@@ -45,6 +46,27 @@ def _compile(src):
     return obj, r.stdout
 
 
+def _bindings():
+    """The Python module of the operators on torch tensors: g++ against torch's headers, linked to
+    the library beside it."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "bindings.cpp")
+    if not _stale(BINDINGS, [src, os.path.join(HERE, "..", "include", "arboretum_b200.h")]):
+        return
+    include = cpp_extension.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    cmd = ["/usr/bin/g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    cmd += [x for d in include for x in ("-isystem", d)]
+    cmd += [src, "-o", BINDINGS, "-L" + HERE, "-l:libarboretum.so", "-Wl,-rpath,$ORIGIN", "-L" + lib,
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed for bindings.cpp:\n" + r.stdout)
+
+
 def build(force=False, verbose=False):
     os.makedirs(BUILD, exist_ok=True)
     if force:
@@ -62,6 +84,7 @@ def build(force=False, verbose=False):
         r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout)
+    _bindings()
     return LIB
 
 
