@@ -37,7 +37,7 @@ def _load_lib():
                  "ABuildHistogramFromParents", "ANcclUniqueId", "AInitNccl", "AThresholdsNoAlloc", "ASharedAtomicPeak",
                  "AReleaseCachedMemory", "AEmbedding", "ATokenOrderBytes", "ATokenOrder", "AEmbeddingGradBytes",
                  "AEmbeddingGrad", "AAdamWBytes", "AAdamWCreate", "AAdamWSetStep", "AAdamWGetStep", "AAdamWStep",
-                 "AFreeAdamW"):
+                 "AFreeAdamW", "ATreeCount", "ALeafTokens", "ARefineLeaves"):
         getattr(lib, name).restype = ctypes.c_char_p
     lib.ADumpModel.argtypes = [ctypes.POINTER(ctypes.c_char_p), ctypes.c_void_p]
     lib.AFreeDMatrix.argtypes = [ctypes.c_void_p]
@@ -91,6 +91,9 @@ def _load_lib():
     lib.AAdamWGetStep.argtypes = [ptr, ptr, ptr]
     lib.AAdamWStep.argtypes = [ptr, ptr, i32, i32, f64, ptr, ptr, ptr]
     lib.AFreeAdamW.argtypes = [ptr]
+    lib.ATreeCount.argtypes = [ptr, ptr]
+    lib.ALeafTokens.argtypes = [ptr, ptr, i32, ptr]
+    lib.ARefineLeaves.argtypes = [ptr, ptr, i32, f64, f64, f64, f64, f64, i32]
     return lib
 
 
@@ -347,6 +350,35 @@ class Garden(object):
         g, h = ctypes.c_double(0), ctypes.c_double(0)
         _call_and_throw_if_error(_LIB.AGetGradientStep(self.handle, ctypes.byref(g), ctypes.byref(h)))
         return g.value, h.value
+
+    def leaf_tokens(self, data, n_rounds=-1, out=None):
+        """The leaf every row reaches in each of the first ``n_rounds`` trees (-1: all), as tokens of
+        the table of all leaves: ``tree * leaves + leaf``, int32 [rows][trees], stored tree after tree.
+        ``out``: a contiguous int32 CUDA tensor [trees][rows] to fill; its transpose is returned."""
+        self._ensure_init()
+        count = ctypes.c_int(0)
+        _call_and_throw_if_error(_LIB.ATreeCount(self.handle, ctypes.byref(count)))
+        use = count.value if n_rounds == -1 else min(int(n_rounds), count.value)
+        if out is None:
+            res = np.empty((max(0, use), int(data.rows)), dtype=np.int32)
+            _call_and_throw_if_error(_LIB.ALeafTokens(self.handle, data.handle, int(n_rounds), _ptr(res)))
+            return res.T
+        import torch
+        if out.dtype != torch.int32 or tuple(out.shape) != (use, data.rows) or not out.is_contiguous() \
+                or out.device.type != 'cuda':
+            raise ValueError("out must be a contiguous int32 CUDA tensor of %d trees x %d rows" % (use, data.rows))
+        torch.cuda.current_stream(out.device).synchronize()  # the library fills it on a stream of its own
+        _call_and_throw_if_error(_LIB.ALeafTokens(self.handle, data.handle, int(n_rounds),
+                                                  ctypes.c_void_p(out.data_ptr())))
+        return out.t()
+
+    def refine_leaves(self, data, steps, lr=0.01, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, state_bits=32):
+        """Gradient steps on the leaf values of all trees together: ``steps`` AdamW steps on the mean
+        loss of ``data`` (its ``y`` or ``labels``, this model's objective).  The trees' tests stay as
+        they are; ``predict``, ``dump`` and further ``grow_tree`` calls see the new values."""
+        self._ensure_init()
+        _call_and_throw_if_error(_LIB.ARefineLeaves(self.handle, data.handle, int(steps), float(lr), float(betas[0]),
+                                                    float(betas[1]), float(eps), float(weight_decay), int(state_bits)))
 
     def set_profile(self, on=True):
         self._ensure_init()

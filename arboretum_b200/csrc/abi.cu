@@ -5,6 +5,7 @@
 #include <nccl.h>
 
 #include <climits>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -340,6 +341,46 @@ const char *APredict(VoidPointer garden, VoidPointer data, const float **out, co
   static_cast<Garden *>(garden)->Predict(static_cast<DataMatrix *>(data), result,
                                          n_rounds == -1 ? INT_MAX : n_rounds);
   if (const char *e = to_new_array(result, out)) return e;
+  ARB_CATCH
+}
+
+const char *ATreeCount(VoidPointer garden, int *count) {
+  ARB_TRY
+  ARB_CHECK(garden && count, "NULL argument");
+  *count = int(static_cast<Garden *>(garden)->trees.size());
+  ARB_CATCH
+}
+
+const char *ALeafTokens(VoidPointer garden, VoidPointer data, int n_rounds, int *out) {
+  ARB_TRY
+  ARB_CHECK(garden && data && out, "NULL argument");
+  Garden *g = static_cast<Garden *>(garden);
+  DataMatrix *d = static_cast<DataMatrix *>(data);
+  ARB_CHECK(n_rounds >= -1, "n_rounds must be -1 or a number of trees");
+  const size_t use = n_rounds == -1 ? g->trees.size() : std::min<size_t>(size_t(n_rounds), g->trees.size());
+  const size_t bytes = use * size_t(d->rows) * sizeof(int);
+  if (bytes == 0) return nullptr;
+  if (is_device_pointer(out)) {
+    g->LeafTokens(d, int(use), 1, out, size_t(d->rows));
+  } else {
+    g->EnsureStream();
+    DevBuf tokens;
+    tokens.alloc(bytes);
+    g->LeafTokens(d, int(use), 1, tokens.as<int>(), size_t(d->rows));
+    ARB_CUDA(cudaMemcpy(out, tokens.p, bytes, cudaMemcpyDeviceToHost));
+  }
+  ARB_CATCH
+}
+
+const char *ARefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2, double eps,
+                          double weight_decay, int state_bits) {
+  ARB_TRY
+  ARB_CHECK(garden && data, "NULL argument");
+  ARB_CHECK(steps >= 0, "negative step count");
+  ARB_CHECK(state_bits == 8 || state_bits == 32, "state_bits must be 8 or 32");
+  ARB_CHECK(std::isfinite(lr), "lr is not finite");
+  static_cast<Garden *>(garden)->RefineLeaves(
+      static_cast<DataMatrix *>(data), Garden::Refinement{steps, lr, beta1, beta2, eps, weight_decay, state_bits});
   ARB_CATCH
 }
 

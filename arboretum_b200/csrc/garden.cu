@@ -5,8 +5,10 @@
 // memory, and the host reads the finished tree back once per tree.
 #include <mutex>
 
+#include "../../include/arboretum_b200.h"
 #include "garden.h"
 #include "exchange.h"
+#include "operators.h"
 
 #include <algorithm>
 #include <chrono>
@@ -576,6 +578,8 @@ class Builder {
   void UpdateGrad();
   void GrowTree(int label, Tree *tree);
   void Resume();
+  void Predict();
+  void Repredict();
   DataMatrix *data;
 
  private:
@@ -1105,6 +1109,13 @@ void Builder::UpdateGrad() {  // objective.cu:28-56
 // trees here.  (The reference restores the trees only: a builder made after `load` starts
 // from initial_y, garden.cu:585-606,659-677.)
 void Builder::Resume() {
+  Predict();
+  for (size_t t = 0; t < g_->trees.size(); ++t) SampleFeatures();
+  round_ = unsigned(g_->trees.size() / size_t(K_));
+}
+
+// adds what the existing trees give on this matrix's raw values to the predictions
+void Builder::Predict() {
   Garden *g = g_;
   cudaStream_t s = g->stream;
   ARB_CHECK(g->max_fid < data->cols(), "the model tests a feature the matrix does not have");
@@ -1119,8 +1130,12 @@ void Builder::Resume() {
                    d_yhat_.as<float>() + first, s, n_, feed.categories(first), data->cols_cat);
     ARB_CUDA(cudaStreamSynchronize(s));
   }
-  for (size_t t = 0; t < g->trees.size(); ++t) SampleFeatures();
-  round_ = unsigned(g->trees.size() / size_t(K_));
+}
+
+// the trees' values have changed: the predictions that the next round's gradients start from follow
+void Builder::Repredict() {
+  launch_fill(d_yhat_.as<float>(), n_ * size_t(K_), g_->InternalInitialY(), g_->stream);
+  Predict();
 }
 
 // Feature sampling of one tree (garden.cu:126-165,252-253 of the reference): the same
@@ -1732,6 +1747,138 @@ void Garden::Predict(DataMatrix *data, std::vector<float> &out, int n_rounds) {
                              cudaMemcpyDeviceToHost, stream));
     ARB_CUDA(cudaStreamSynchronize(stream));
   }
+}
+
+void Garden::LeafTokens(DataMatrix *data, int use, int group, int *out, size_t stride) {
+  const size_t n = size_t(data->rows);
+  ARB_CHECK(max_fid < data->cols(), "the model tests a feature the matrix does not have");
+  SyncForest();
+  RowFeeder feed(data);
+  const PackedTree pt{d_fid.as<int>(), d_thr.as<float>(), d_w.as<float>(), d_label.as<int>(),
+                      d_category.as<unsigned>()};
+  for (size_t first = 0; first < n; first += feed.chunk) {
+    const size_t count = std::min(feed.chunk, n - first);
+    const float *X = feed.load(first, count, stream);
+    launch_leaf_tokens(X, count, data->cols_dense, pt, 0, use, group, int(cfg.tree.depth), out + first, stride, stream,
+                       feed.categories(first), data->cols_cat);
+    ARB_CUDA(cudaStreamSynchronize(stream));
+  }
+}
+
+// The forest as a table of leaf values: a row's prediction is the sum of the values its tokens name
+// (one for each tree), the loss's gradient sums by token into the values' gradient, and an AdamW step
+// over one tensor a tree moves them all.  The tokens do not change, so they are sorted once.
+void Garden::RefineLeaves(DataMatrix *data, const Refinement &r) {
+  const size_t n = size_t(data->rows), T = trees.size(), K = std::max<size_t>(1, cfg.tree.labels_count);
+  ARB_CHECK(T > 0, "no tree has been grown yet");
+  ARB_CHECK(T % K == 0, "the number of trees is not a multiple of labels_count");
+  for (size_t t = 0; t < T; ++t) ARB_CHECK(size_t(trees[t].label) == t % K, "the trees are not in the order of their classes");
+  ARB_CHECK(shards.world == 1, "leaf refinement does not work on row shards");
+  const bool softmax = cfg.objective == kSoftMaxOneVsAll;
+  ARB_CHECK(softmax ? data->has_labels() : data->has_y(), "the matrix has no targets");
+  const int64_t per_class = int64_t(T / K);
+  ARB_CHECK(int64_t(n) <= ((int64_t(1) << 31) - 2) / per_class, "more than 2^31 - 2 leaf tokens of a class");
+  const int64_t leaves = int64_t(1) << (cfg.tree.depth - 1), rows = per_class * leaves;
+  ARB_CHECK(rows < (int64_t(1) << 31) - 1, "too many leaves");
+  EnsureStream();
+
+  DevBuf d_tokens, d_y, d_labels, d_w, d_grad_w, d_yhat, d_grad;
+  d_tokens.alloc(T * n * sizeof(int));
+  LeafTokens(data, int(T), int(K), d_tokens.as<int>(), n);
+  const float *y = data->d_y.as<float>();
+  const unsigned char *labels = data->d_labels.as<unsigned char>();
+  if (softmax) {
+    std::vector<unsigned char> host(n);
+    if (labels) ARB_CUDA(cudaMemcpy(host.data(), labels, n, cudaMemcpyDeviceToHost));
+    else host = data->labels;
+    for (unsigned char l : host) ARB_CHECK(l < K, "a label is not below labels_count");
+    if (!labels) {
+      d_labels.alloc(n);
+      ARB_CUDA(cudaMemcpy(d_labels.p, host.data(), n, cudaMemcpyHostToDevice));
+      labels = d_labels.as<unsigned char>();
+    }
+  } else if (!y) {
+    d_y.alloc(n * sizeof(float));
+    ARB_CUDA(cudaMemcpy(d_y.p, data->y.data(), d_y.bytes, cudaMemcpyHostToDevice));
+    y = d_y.as<float>();
+  }
+  // leaf values, class after class, tree after tree: tree t of class k begins at (k * per_class + t) * leaves
+  std::vector<float> w(T * size_t(leaves));
+  const auto values = [&](size_t t) { return w.begin() + (t % K * size_t(per_class) + t / K) * size_t(leaves); };
+  for (size_t t = 0; t < T; ++t) std::copy(trees[t].weights.begin(), trees[t].weights.end(), values(t));
+  d_w.alloc(w.size() * sizeof(float));
+  d_grad_w.alloc(d_w.bytes);
+  ARB_CUDA(cudaMemcpy(d_w.p, w.data(), d_w.bytes, cudaMemcpyHostToDevice));
+  d_yhat.alloc(n * K * sizeof(float));
+  d_grad.alloc(d_yhat.bytes);
+
+  // one order a class; the scratch of the sort and of the gradient is shared, they run one after another
+  std::vector<TokenView> views;
+  std::vector<TokenOrder> orders;
+  const TokenOrder shape(nullptr, int64_t(n), per_class, rows);
+  DevBuf d_orders, d_scratch;
+  d_orders.alloc(shape.bytes * K);
+  d_scratch.alloc(std::max<size_t>(256, std::max(token_order_scratch(shape.count), lookup_grad_scratch(shape, 1))));
+  for (size_t k = 0; k < K; ++k) {
+    views.push_back(TokenView{d_tokens.as<int>() + k * n, 4, int64_t(n), per_class, 1, int64_t(K * n)});
+    orders.push_back(TokenOrder(d_orders.as<char>() + k * shape.bytes, int64_t(n), per_class, rows));
+    launch_token_order(views[k], orders[k], d_scratch.p, stream);
+  }
+
+  struct Check {  // the C entry points' message as an exception
+    void operator()(const char *e) const {
+      if (e) throw std::runtime_error(e);
+    }
+  } check;
+  std::vector<AAdamWParam> params;
+  std::vector<const void *> grads;
+  for (size_t t = 0; t < T; ++t) {
+    params.push_back(AAdamWParam{d_w.as<float>() + t * size_t(leaves), leaves, kF32});
+    grads.push_back(d_grad_w.as<float>() + t * size_t(leaves));
+  }
+  int64_t length = 0, workspace = 0;
+  check(AAdamWBytes(params.data(), int(T), &length, &workspace));
+  DevBuf d_m, d_v, d_s1, d_s2, d_work;
+  d_m.alloc(size_t(length) * (r.state_bits == 8 ? 1 : 4));
+  d_v.alloc(d_m.bytes);
+  ARB_CUDA(cudaMemset(d_m.p, 0, d_m.bytes));
+  ARB_CUDA(cudaMemset(d_v.p, 0, d_v.bytes));
+  if (r.state_bits == 8) {
+    d_s1.alloc(size_t(length) / 128 * sizeof(float));
+    d_s2.alloc(d_s1.bytes);
+    ARB_CUDA(cudaMemset(d_s1.p, 0, d_s1.bytes));
+    ARB_CUDA(cudaMemset(d_s2.p, 0, d_s2.bytes));
+  }
+  d_work.alloc(size_t(workspace));
+  const AAdamWConfig config{r.beta1, r.beta2, r.eps, r.weight_decay, r.state_bits, 0u, d_m.p, d_v.p, d_s1.as<float>(),
+                            d_s2.as<float>(), nullptr};
+  struct Optimizer {
+    VoidPointer handle = nullptr;
+    ~Optimizer() { AFreeAdamW(handle); }
+  } optimizer;
+  check(AAdamWCreate(params.data(), int(T), &config, d_work.p, current_device(), &optimizer.handle));
+  ARB_CUDA(cudaDeviceSynchronize());  // the copies and clears above went to the default stream
+
+  for (int step = 0; step < r.steps; ++step) {
+    for (size_t k = 0; k < K; ++k)
+      launch_lookup(LookupLaunch{d_w.as<float>() + k * size_t(rows), kF32, rows, 1, 1, views[k], 1.0f,
+                                 d_yhat.as<float>() + k * n, kF32, 1}, stream);
+    launch_loss_gradient(cfg.objective, int(K), n, y, labels, d_yhat.as<float>(), InternalInitialY(), d_grad.as<float>(), stream);
+    for (size_t k = 0; k < K; ++k) {
+      LookupGradLaunch g;
+      g.grad = d_grad.as<float>() + k * n, g.type = kF32, g.dim = 1, g.grad_stride = 1;
+      g.scale = 1.0f;
+      g.out = d_grad_w.as<float>() + k * size_t(rows), g.out_type = kF32, g.out_stride = 1;
+      g.accumulate = false;
+      launch_lookup_grad(g, orders[k], d_scratch.p, stream);
+    }
+    check(AAdamWStep(optimizer.handle, grads.data(), int(T), 1, r.lr, nullptr, nullptr, stream));
+  }
+  ARB_CUDA(cudaMemcpyAsync(w.data(), d_w.p, d_w.bytes, cudaMemcpyDeviceToHost, stream));
+  ARB_CUDA(cudaStreamSynchronize(stream));
+  for (size_t t = 0; t < T; ++t) std::copy(values(t), values(t) + leaves, trees[t].weights.begin());
+  forest_trees_on_device = 0;  // the device copy of the forest holds the old values
+  if (builder) builder->Repredict();
 }
 
 // Garden::UpdateByLastTree garden.cu:627-635: add the last round's trees to the

@@ -165,6 +165,15 @@ class Garden {
   void Predict(DataMatrix *data, std::vector<float> &out, int n_rounds);
   void UpdateByLastTree(DataMatrix *data);
   void GetY(DataMatrix *data, std::vector<float> &out);
+  // tokens of the first `trees` trees: out (device) [k][stride], see launch_leaf_tokens
+  void LeafTokens(DataMatrix *data, int trees, int group, int *out, size_t stride);
+  // gradient steps on the leaf values of all trees together, against `data`'s targets
+  struct Refinement {
+    int steps;
+    double lr, beta1, beta2, eps, weight_decay;
+    int state_bits;
+  };
+  void RefineLeaves(DataMatrix *data, const Refinement &r);
   std::string GetModel() const;
   void Restore(const char *json_model);
   float InternalInitialY() const;

@@ -252,6 +252,14 @@ struct PackedTree {  // device arrays of one forest
 void launch_predict(const float *X, size_t n, int F, PackedTree t, int first_tree, int n_trees,
                     int depth, float *out /*[K][plane_stride]*/, cudaStream_t s, size_t plane_stride = 0,
                     const unsigned *cat = nullptr, int ccol = 0);
+// the leaf every row reaches in trees first_tree .. first_tree + n_trees, as tokens of a table of
+// leaf values: out[k * out_stride + row] = (k / group) * leaves + leaf for the k-th of them
+void launch_leaf_tokens(const float *X, size_t n, int F, PackedTree t, int first_tree, int n_trees, int group, int depth,
+                        int *out, size_t out_stride, cudaStream_t s, const unsigned *cat = nullptr, int ccol = 0);
+// gradient of the mean loss with respect to the internal predictions: yhat [K][n] holds the trees' sums
+// without the initial prediction; grad [K][n]
+void launch_loss_gradient(int objective, int K, size_t n, const float *y, const unsigned char *label, const float *yhat,
+                          float initial, float *grad, cudaStream_t s);
 void launch_fill(float *dst, size_t n, float value, cudaStream_t s);
 void launch_fill_u32(unsigned *dst, size_t n, unsigned value, cudaStream_t s);
 void launch_link(int objective, int K, size_t n, const float *internal /*[K][n]*/,

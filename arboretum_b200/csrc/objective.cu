@@ -292,32 +292,67 @@ __global__ void leaf_weights_kernel(LeafLaunch a) {
                                           a.lambda, a.alpha, a.mlw) * a.eta;
 }
 
+// The leaf that row i reaches in tree k, 0 .. 2^(depth - 1) - 1.  garden.h:79-84: dense features go
+// left below the threshold, categorical ones when the value is the node's category.
+__device__ __forceinline__ int leaf_of(const float *__restrict__ X, size_t i, int F, const PackedTree &t, int k, int depth,
+                                       const unsigned *__restrict__ cat, int ccol) {
+  const int nodes = (1 << depth) - 1;
+  const float *row = X + i * F;
+  const int *fid = t.fid + size_t(k) * nodes;
+  const float *thr = t.thr + size_t(k) * nodes;
+  int node = 0;
+  for (int j = 1; j < depth; ++j) {
+    const int f = fid[node];
+    const bool left = f < F ? row[f] < thr[node]
+                            : (cat != nullptr && f - F < ccol &&
+                               cat[i * size_t(ccol) + (f - F)] == t.category[size_t(k) * nodes + node]);
+    node = left ? 2 * node + 1 : 2 * node + 2;
+  }
+  return node - ((1 << (depth - 1)) - 1);
+}
+
 // RegTree::Predict garden.h:70-90 (dense features): x < threshold goes left, so
 // NaN goes right; trees are added in order, in float, like the reference's loop
 // in Garden::Predict garden.cu:643-657.
 __global__ void predict_kernel(const float *__restrict__ X, size_t n, int F, PackedTree t,
                                int first_tree, int n_trees, int depth, float *__restrict__ out,
                                size_t plane_stride, const unsigned *__restrict__ cat, int ccol) {
-  const int nodes = (1 << depth) - 1;
   const int leaves = 1 << (depth - 1);
-  const int offset = leaves - 1;
   for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
        i += size_t(gridDim.x) * blockDim.x) {
-    const float *row = X + i * F;
-    for (int k = first_tree; k < first_tree + n_trees; ++k) {
-      const int *fid = t.fid + size_t(k) * nodes;
-      const float *thr = t.thr + size_t(k) * nodes;
-      int node = 0;
-      for (int j = 1; j < depth; ++j) {
-        const int f = fid[node];
-        // garden.h:79-84: dense features go left below the threshold, categorical ones when
-        // the value is the node's category
-        const bool left = f < F ? row[f] < thr[node]
-                                : (cat != nullptr && f - F < ccol &&
-                                   cat[i * size_t(ccol) + (f - F)] == t.category[size_t(k) * nodes + node]);
-        node = left ? 2 * node + 1 : 2 * node + 2;
+    for (int k = first_tree; k < first_tree + n_trees; ++k)
+      out[size_t(t.label[k]) * plane_stride + i] +=
+          t.weights[size_t(k) * leaves + leaf_of(X, i, F, t, k, depth, cat, ccol)];
+  }
+}
+
+__global__ void leaf_tokens_kernel(const float *__restrict__ X, size_t n, int F, PackedTree t, int first_tree,
+                                   int n_trees, int group, int depth, int *__restrict__ out, size_t out_stride,
+                                   const unsigned *__restrict__ cat, int ccol) {
+  const int leaves = 1 << (depth - 1);
+  for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
+       i += size_t(gridDim.x) * blockDim.x) {
+    for (int k = 0; k < n_trees; ++k)
+      out[size_t(k) * out_stride + i] = k / group * leaves + leaf_of(X, i, F, t, first_tree + k, depth, cat, ccol);
+  }
+}
+
+__global__ void loss_gradient_kernel(int objective, int K, size_t n, const float *__restrict__ y,
+                                     const unsigned char *__restrict__ label, const float *__restrict__ yhat, float initial,
+                                     float inv_n, float *__restrict__ grad) {
+  for (size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += size_t(gridDim.x) * blockDim.x) {
+    if (objective == 3) {  // the initial prediction is the same for every class and cancels
+      double sum = 0.0;
+      float most = yhat[i];
+      for (int k = 1; k < K; ++k) most = fmaxf(most, yhat[size_t(k) * n + i]);
+      for (int k = 0; k < K; ++k) sum += exp(double(yhat[size_t(k) * n + i]) - double(most));
+      for (int k = 0; k < K; ++k) {
+        const double p = exp(double(yhat[size_t(k) * n + i]) - double(most)) / sum;
+        grad[size_t(k) * n + i] = float(p - (k == label[i] ? 1.0 : 0.0)) * inv_n;
       }
-      out[size_t(t.label[k]) * plane_stride + i] += t.weights[size_t(k) * leaves + node - offset];
+    } else {
+      const float x = yhat[i] + initial;
+      grad[i] = ((objective == 1 ? sigmoid(x) : x) - y[i]) * inv_n;
     }
   }
 }
@@ -425,6 +460,23 @@ void launch_predict(const float *X, size_t n, int F, PackedTree t, int first_tre
   const int threads = 256;
   predict_kernel<<<grid_for(n, threads), threads, 0, s>>>(X, n, F, t, first_tree, n_trees, depth, out,
                                                           plane_stride ? plane_stride : n, cat, ccol);
+  ARB_CUDA(cudaGetLastError());
+  count_launch();
+}
+
+void launch_leaf_tokens(const float *X, size_t n, int F, PackedTree t, int first_tree, int n_trees, int group, int depth,
+                        int *out, size_t out_stride, cudaStream_t s, const unsigned *cat, int ccol) {
+  if (n_trees <= 0 || n == 0) return;
+  leaf_tokens_kernel<<<grid_for(n, 256), 256, 0, s>>>(X, n, F, t, first_tree, n_trees, group, depth, out, out_stride, cat,
+                                                      ccol);
+  ARB_CUDA(cudaGetLastError());
+  count_launch();
+}
+
+void launch_loss_gradient(int objective, int K, size_t n, const float *y, const unsigned char *label, const float *yhat,
+                          float initial, float *grad, cudaStream_t s) {
+  if (n == 0) return;
+  loss_gradient_kernel<<<grid_for(n, 256), 256, 0, s>>>(objective, K, n, y, label, yhat, initial, float(1.0 / double(n)), grad);
   ARB_CUDA(cudaGetLastError());
   count_launch();
 }

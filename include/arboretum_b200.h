@@ -172,6 +172,18 @@ const char *ASharedAtomicPeak(int steps, double *pair_updates_per_s);
  * tokens[b * bag_stride + t * token_stride].  A token outside [0, rows) is an empty slot: it adds
  * nothing and gets no gradient.  bags * per_bag and rows must be below 2^31 - 1. */
 
+/* Trees of the model (labels_count a boosting round). */
+const char *ATreeCount(VoidPointer garden, int *count);
+/* The leaf that every row of `data` reaches in each of the first n_rounds trees (-1: all; a count of
+ * trees, like APredict's): out[tree][row] = tree * 2^(depth - 1) + leaf, host or device memory. */
+const char *ALeafTokens(VoidPointer garden, VoidPointer data, int n_rounds, int *out);
+/* `steps` AdamW steps on the leaf values of all trees together, on the gradient of the mean loss over
+ * `data` (its targets; the garden's objective): lookup, gradient by sorted tokens and AdamW step as
+ * below, one tensor a tree.  The trees' tests stay.  Training can go on afterwards; predictions that
+ * AAppendLastTree has accumulated are not revised. */
+const char *ARefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2, double eps,
+                          double weight_decay, int state_bits);
+
 /* out[b][:] = scale * sum over t of table[token(b, t)][:], summed in fp32, rounded once */
 const char *AEmbedding(const void *table, int type, int64_t rows, int64_t dim, int64_t row_stride,
                        const void *tokens, int token_bytes, int64_t bags, int64_t per_bag,

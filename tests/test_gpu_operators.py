@@ -617,3 +617,145 @@ def test_a_device_that_is_not_there():
     e = arb.lib().AEmbedding(t.data_ptr(), 0, 4, 4, 4, i.data_ptr(), 4, 2, 1, 1, 0, 1.0, o.data_ptr(), 0, 4, 4095, None)
     assert e is not None and b"CUDA error" in e
     assert torch.equal(arb.embedding(i, t), o)  # and the context is as it was
+
+
+# ---- a forest's leaf values ------------------------------------------------------------------
+def _grown(objective, rounds=5, rows=300, depth=4, classes=3):
+    rng = np.random.default_rng(objective + 7)
+    X = rng.normal(size=(rows, 6)).astype(np.float32)
+    X[::17, 2] = np.nan
+    score = X[:, 0] - 0.5 * np.nan_to_num(X[:, 2]) + rng.normal(size=rows) * 0.3
+    cfg = {"objective": objective, "method": 1, "internals": {"hist_size": 63, "seed": 0},
+           "verbose": {"gpu": False, "booster": False, "data": False},
+           "tree": {"eta": 0.2, "max_depth": depth, "lambda": 1.0, "min_child_weight": 1.0, "initial_y": 0.4}}
+    target = {"y": score.astype(np.float32)}
+    if objective == 1:
+        target = {"y": (score > 0).astype(np.float32)}
+    if objective == 3:
+        cfg["tree"]["labels_count"] = classes
+        target = {"labels": np.digitize(score, [-0.5, 0.5]).astype(np.uint8)}
+    data = arb.DMatrix(X, **target)
+    return arb.train(cfg, data, rounds), data, X, target
+
+
+def _weights(model):
+    import json
+    return np.array([t["weights"] for t in json.loads(model.dump())["model"]])
+
+
+def _link(objective, yhat):
+    if objective == 1:
+        return 1 / (1 + np.exp(-yhat))
+    if objective == 3:
+        e = np.exp(yhat - yhat.max(1, keepdims=True))
+        return e / e.sum(1, keepdims=True)
+    return yhat
+
+
+@pytest.mark.parametrize("objective", [0, 1, 3])
+def test_refined_leaves_follow_the_formula(objective):
+    """Tokens, lookup, gradient by token and AdamW step together, against the same steps in 64 bits."""
+    model, data, X, target = _grown(objective)
+    K = 3 if objective == 3 else 1
+    n = len(X)
+    tok = model.leaf_tokens(data)
+    w = _weights(model).astype(np.float64)
+    T, leaves = w.shape
+    assert tok.shape == (n, T) and tok.dtype == np.int32
+    leaf = tok - np.arange(T) * leaves
+    assert (leaf >= 0).all() and (leaf < leaves).all()
+    out = torch.empty(T, n, dtype=torch.int32, device="cuda")
+    assert np.array_equal(model.leaf_tokens(data, out=out).cpu().numpy(), tok)
+    assert np.array_equal(model.leaf_tokens(data, n_rounds=2), tok[:, :2])
+    start = 0.4 if objective != 1 else np.log(0.4 / 0.6)
+
+    def yhat(w):
+        each = w[np.arange(T), leaf]
+        return np.stack([each[:, k::K].sum(1) for k in range(K)], 1)
+    # a prediction: a float32 sum of T leaf values and the start
+    off = (T + 2) * U * (np.abs(w[np.arange(T), leaf]).sum(1).max() + abs(start))
+    got = model.predict(data).reshape(n, K)
+    assert np.abs(got - _link(objective, yhat(w) + start)).max() <= off + 4 * U
+    lr, b1, b2, eps, wd, steps = 0.05, 0.9, 0.99, 1e-2, 0.02, 4
+    m, v = np.zeros_like(w), np.zeros_like(w)
+    largest = 0.0
+    for s in range(1, steps + 1):
+        p = _link(objective, yhat(w) + start)
+        r = p - (np.eye(K)[target["labels"]] if objective == 3 else target["y"].astype(np.float64)[:, None])
+        largest = max(largest, np.abs(r).max())
+        g = np.zeros_like(w)
+        for t in range(T):
+            g[t] = np.bincount(leaf[:, t], weights=r[:, t % K] / n, minlength=leaves)
+        m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+        w = w * (1 - lr * wd) - lr / (1 - b1 ** s) * m / (np.sqrt(v / (1 - b2 ** s)) + eps)
+    model.refine_leaves(data, steps, lr=lr, betas=(b1, b2), eps=eps, weight_decay=wd)
+    # a gradient is a float32 sum of at most n residuals, each off by a few roundings; a step passes its
+    # error on with a slope of at most lr / eps (twice: once through m, once through the root), and the
+    # moved values change the next residuals by no more than that again
+    slack = (n + 8) * U * largest * lr / eps * 2 * steps * 2
+    assert np.abs(_weights(model) - w).max() <= slack + 16 * U * np.abs(w).max()
+    got = model.predict(data).reshape(n, K)
+    assert np.abs(got - _link(objective, yhat(_weights(model)) + start)).max() <= off * 2 + 8 * U
+    again = arb.load(model.dump())
+    again.labels_count = K
+    assert np.array_equal(again.predict(data).reshape(n, K), got)
+    # training goes on from the moved values
+    model.grow_tree()
+    grown = _weights(model)
+    assert np.array_equal(grown[:T].astype(np.float32), _weights(again).astype(np.float32)) and len(grown) == T + K
+    internal = model.train_yhat().T
+    assert np.abs(_link(objective, internal.astype(np.float64)) - model.predict(data).reshape(n, K)).max() <= 2 * off + 8 * U
+
+
+def test_refinement_in_8_bits_and_without_steps():
+    model, data, X, target = _grown(0)
+    before = _weights(model)
+    model.refine_leaves(data, 0)
+    assert np.array_equal(_weights(model), before)
+    # each step moves a value by lr times a ratio of at most sqrt(1 / (1 - 0.999)) or so; here by less than 2 lr
+    model.refine_leaves(data, 10, lr=1e-3, state_bits=8)
+    after = _weights(model)
+    assert np.isfinite(after).all() and not np.array_equal(after, before) and np.abs(after - before).max() < 10 * 2e-3
+    loaded = arb.load(model.dump())
+    other = arb.DMatrix(X, **target)
+    loaded.refine_leaves(other, 3)  # a loaded model, another matrix
+    assert not np.array_equal(_weights(loaded), after)
+
+
+def test_refinement_refuses():
+    model, data, X, _ = _grown(0, rounds=1)
+    with pytest.raises(arb.ArboretumError, match="no targets"):
+        model.refine_leaves(arb.DMatrix(X), 1)
+    with pytest.raises(arb.ArboretumError, match="betas"):
+        model.refine_leaves(data, 1, betas=(1.0, 0.9))
+    with pytest.raises(arb.ArboretumError, match="feature"):
+        model.refine_leaves(arb.DMatrix(X[:, :1], y=X[:, 0]), 1)
+    with pytest.raises(ValueError, match="out must be"):
+        model.leaf_tokens(data, out=torch.empty(2, 300, dtype=torch.int32, device="cuda"))
+
+
+def test_refinement_of_many_rows():
+    """The order kept by runs of bags, and the table in shared memory: the same operators at a size
+    where the library chooses them, against the lookups of the public functions."""
+    rng = np.random.default_rng(3)
+    rows = 120000
+    X = rng.normal(size=(rows, 5)).astype(np.float32)
+    y = (X[:, 0] * 2 + rng.normal(size=rows) * 0.1).astype(np.float32)
+    cfg = {"objective": 0, "method": 1, "internals": {"hist_size": 63, "seed": 0},
+           "verbose": {"gpu": False, "booster": False, "data": False}, "tree": {"eta": 0.1, "max_depth": 3, "initial_y": 0.0}}
+    data = arb.DMatrix(X, y=y)
+    model = arb.train(cfg, data, 8)
+    T, leaves = _weights(model).shape
+    tok = model.leaf_tokens(data, out=torch.empty(T, rows, dtype=torch.int32, device="cuda"))
+    table = torch.tensor(_weights(model), dtype=F32, device="cuda").view(-1, 1)
+    target = torch.tensor(y, device="cuda")[:, None]
+    grad = torch.zeros_like(table)
+    o = arb.AdamW(list(table.view(T, leaves)), lr=0.01, eps=1e-8, weight_decay=0.0,
+                  grads=list(grad.view(T, leaves)))
+    order = arb.token_order(tok, T * leaves, pooled=True)
+    for _ in range(3):
+        r = (arb.embedding(tok, table, pooled=True) + 0.0 - target) * np.float32(1.0 / rows)
+        arb.embedding_grad(r, order, T * leaves, out=grad)
+        o.step()
+    model.refine_leaves(data, 3, lr=0.01)
+    assert np.array_equal(_weights(model).astype(np.float32), table.view(T, leaves).cpu().numpy())

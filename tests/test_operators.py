@@ -127,3 +127,21 @@ def test_python_refusals():
             (ValueError, "CUDA", lambda: arb.AdamW([t]))):
         with pytest.raises(error, match=words):
             call()
+
+
+def test_leaf_entry_points_refuse():
+    import json
+    h = ctypes.c_void_p()
+    cfg = {"objective": 0, "method": 1, "tree": {"max_depth": 2}}
+    assert LIB.AInitGarden(json.dumps(cfg).encode(), ctypes.byref(h)) is None
+    n = ctypes.c_int(-1)
+    assert LIB.ATreeCount(h, ctypes.byref(n)) is None and n.value == 0
+    assert "NULL" in _message(LIB.ATreeCount(None, ctypes.byref(n))) and "NULL" in _message(LIB.ALeafTokens(h, None, -1, P))
+    assert "NULL" in _message(LIB.ARefineLeaves(h, None, 1, 0.1, 0.9, 0.99, 1e-8, 0.0, 32))
+    data = arb.DMatrix(np.zeros((3, 2), np.float32), y=np.zeros(3, np.float32))
+    for words, a in (("negative", (-1, 0.1, 0.9, 0.99, 1e-8, 0.0, 32)), ("state_bits", (1, 0.1, 0.9, 0.99, 1e-8, 0.0, 16)),
+                     ("finite", (1, float("nan"), 0.9, 0.99, 1e-8, 0.0, 32)), ("no tree", (1, 0.1, 0.9, 0.99, 1e-8, 0.0, 32))):
+        assert words in _message(LIB.ARefineLeaves(h, data.handle, *a))
+    assert "n_rounds" in _message(LIB.ALeafTokens(h, data.handle, -2, P))
+    assert LIB.ALeafTokens(h, data.handle, -1, P) is None  # no trees: nothing to write
+    assert LIB.AFreeGarden(h) is None
