@@ -29,30 +29,52 @@ struct GradPointers {
   const void *at[kMaxGrads];
 };
 
-// 32 bits for an element: the mixing of the boosting gradients' dither.  `key` holds what the eight
-// elements of a thread share: the upper half of the index, the step and the seed.
+// 32 bits for an element, by the mixing of the boosting gradients' dither:
+//   x = index ^ step, seed, upper half of index;  x ^= x >> 16;  x *= A;  x ^= x >> 15;  x *= B;  x ^= x >> 16
+// The first fold is the same for the eight elements of a thread, whose indices differ in three bits; the
+// last one leaves the upper half as it is.
 __device__ __forceinline__ unsigned hash_key(unsigned long long index, unsigned step, unsigned seed) {
-  return unsigned(index) ^ (unsigned(index >> 32) * 0x9E3779B1u) ^ (step * 0x85EBCA6Bu) ^ (seed * 0xC2B2AE35u);
+  const unsigned x = unsigned(index) ^ (unsigned(index >> 32) * 0x9E3779B1u) ^ (step * 0x85EBCA6Bu) ^ (seed * 0xC2B2AE35u);
+  return x ^ (x >> 16);
 }
-__device__ __forceinline__ unsigned hash_bits(unsigned x) {
-  x ^= x >> 16;
+__device__ __forceinline__ unsigned hash_before_last(unsigned x) {  // x: key ^ element
   x *= 0x7FEB352Du;
   x ^= x >> 15;
-  x *= 0x846CA68Bu;
-  x ^= x >> 16;
-  return x;
+  return x * 0x846CA68Bu;
 }
 
 // two e4m3 codes as floats
 __device__ __forceinline__ float2 decode2(unsigned codes) {
   return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3)));
 }
-// Magnitude of the code for x = value / scale * 2^-120 >= 0: there e4m3's exponents are float's
-// smallest, so a code is the top of the bits, and the dither is added to the 20 bits that go.
-// `random` holds 16 bits, shifted up by four.
-__device__ __forceinline__ unsigned encode(float x, unsigned random) {
-  return min((__float_as_uint(x) + ((random & 0xFFFF0u) | 8u)) >> 20, 126u);
+// x = |value| / scale * 2^-120: there e4m3's exponents are float's smallest, so a code is the seven bits
+// from 20 on, and the dither is added to the 20 bits that go.  `random` holds 16 bits, shifted up by four.
+constexpr unsigned kCodeOne = 1u << 20, kCodeMost = (126u << 20) | 0xFFFFFu;
+__device__ __forceinline__ unsigned dithered(float x, unsigned random) { return min(__float_as_uint(x) + random + 8u, kCodeMost); }
+// the upper bytes of four words
+__device__ __forceinline__ unsigned upper_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
+
+// two float operations in one instruction, each rounded like the single one
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 x, y, z, w; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 w, x, y, z; "
+      "mov.b64 {%0, %1}, w;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+// a + b as a * one + b: of a packed product and a packed sum the assembler makes one operation with one
+// rounding, whatever it is told; `one` is 1 that it does not know of
+__device__ __forceinline__ float2 add2(float2 a, float2 b, float one) { return fma2(a, make_float2(one, one), b); }
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
 // exponent field of the scale of a block whose largest magnitude has these bits: the largest code
 // stands for 448 = 1.75 * 2^8.  255: the block holds a value that is not finite
 __device__ __forceinline__ unsigned scale_field(unsigned top_bits) {
@@ -67,7 +89,7 @@ __device__ __forceinline__ float inv_scale_of(unsigned field) {
 }
 
 struct Scalars {
-  float beta1, one_beta1, beta2, one_beta2, inv_root_bc2, step_size, keep, eps, grad_scale;
+  float beta1, one_beta1, beta2, one_beta2, inv_root_bc2, step_size, keep, eps, grad_scale, one;
   unsigned step;
 };
 
@@ -81,21 +103,23 @@ __device__ __forceinline__ Scalars scalars_of(const AdamWLaunch &a) {
   c.keep = float(1.0 - lr * a.decay);
   c.eps = a.eps;
   c.grad_scale = a.grad_scale ? *a.grad_scale : 1.0f;
+  c.one = a.state->one;
   c.step = unsigned(a.state->step + 1);
   return c;
 }
 
 // Root of v >= 0, rounded to the nearest like sqrtf: one Newton step on the hardware's reciprocal root
 // with the residual in a fused multiply-add (Markstein's correction), a third of sqrtf's instructions.
-// Exhaustively equal to sqrtf for zero and all of [2^-100, 2^126]; the others take sqrtf.
-__device__ __forceinline__ float root_of(float v) {
-  float q;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaxf(v, 0x1p-100f)));  // v == 0: finite, the product is zero
-  const float s = __fmul_rn(v, q);
-  return __fmaf_rn(__fmaf_rn(-s, s, v), __fmul_rn(0.5f, q), s);
+// Exhaustively equal to sqrtf on all of [2^-100, 2^126]; the others take sqrtf.
+__device__ __forceinline__ float2 root_of(float2 v) {
+  float2 q;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(v.x));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(v.y));
+  const float2 s = mul2(v, q);
+  return fma2(fma2(mul2(s, both(-1.0f)), s, v), mul2(q, both(0.5f)), s);
 }
-__device__ __forceinline__ bool root_is_plain(unsigned largest, unsigned smallest_less_one) {
-  return largest <= 0x7E800000u && smallest_less_one >= 0x0D800000u - 1u;  // 2^126, 2^-100; zero less one is large
+__device__ __forceinline__ bool root_is_plain(unsigned largest, unsigned smallest) {
+  return largest <= 0x7E800000u && smallest >= 0x0D800000u;  // 2^126, 2^-100
 }
 // larger magnitude; a NaN stays
 __device__ __forceinline__ float larger(float a, float b) {
@@ -110,9 +134,9 @@ __device__ __forceinline__ float quotient(float a, float b) {
   return a * r;
 }
 
-constexpr int kThreads = 256;
+template <int BITS>
+constexpr int kThreads = BITS == 8 ? 128 : 256;
 constexpr int kEach = 8;                      // neighbouring elements of a thread
-constexpr int kTileElems = kThreads * kEach;  // elements of a CTA at a time
 constexpr int kLanes = kMomentBlock / kEach;  // lanes that hold an 8-bit block: half a warp
 
 // eight elements as they lie in memory; `whole`: all are there and the address is 16-byte aligned
@@ -141,6 +165,7 @@ __device__ __forceinline__ void store_each(T *p, const float (&x)[kEach], int le
 // A thread's share of a tile.  All loads of a tile are issued before the first value is used.
 template <int BITS, typename P, typename G, bool MASTER>
 struct Tile {
+  static constexpr int kPairs = kEach / 2;
   using W = typename std::conditional<MASTER, float, P>::type;
   Vec<W, kEach> w;
   Vec<G, kEach> g;
@@ -171,95 +196,111 @@ struct Tile {
 
   // (elements past a tensor's end have no weight and no gradient, and moments of zero: they stay so)
   __device__ __forceinline__ void step(const AdamWLaunch &a, const Scalars &c, P *param, long long at, int left, bool vec) const {
-    float p[kEach], gr[kEach], m[kEach], v[kEach];
+    float gr[kEach], pr[kEach];
+    float2 m[kPairs], v[kPairs];
     g.get(gr);
-    w.get(p);
+    w.get(pr);
     if constexpr (BITS == 32) {
-      m32.get(m);
-      v32.get(v);
+      float x[kEach];
+      m32.get(x);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) m[j] = make_float2(x[2 * j], x[2 * j + 1]);
+      v32.get(x);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) v[j] = make_float2(x[2 * j], x[2 * j + 1]);
     } else {
 #pragma unroll
-      for (int j = 0; j < kEach; j += 2) {
-        const float2 mj = decode2((j < 4 ? cm.x : cm.y) >> (j % 4 * 8) & 0xFFFFu);
-        const float2 rj = decode2((j < 4 ? cr.x : cr.y) >> (j % 4 * 8) & 0xFFFFu);
-        m[j] = mj.x * s1, m[j + 1] = mj.y * s1;
-        const float r0 = rj.x * s2, r1 = rj.y * s2;
-        v[j] = r0 * r0, v[j + 1] = r1 * r1;
+      for (int j = 0; j < kPairs; ++j) {
+        m[j] = mul2(decode2((j < 2 ? cm.x : cm.y) >> (j % 2 * 16) & 0xFFFFu), both(s1));
+        const float2 r = mul2(decode2((j < 2 ? cr.x : cr.y) >> (j % 2 * 16) & 0xFFFFu), both(s2));
+        v[j] = mul2(r, r);
       }
     }
     unsigned largest = 0, smallest = 0xffffffffu;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-      const float gj = gr[j] * c.grad_scale;
-      m[j] = m[j] * c.beta1 + gj * c.one_beta1;
-      v[j] = v[j] * c.beta2 + (gj * gj) * c.one_beta2;
-      largest = max(largest, __float_as_uint(v[j]));
-      smallest = min(smallest, __float_as_uint(v[j]) - 1u);
+    for (int j = 0; j < kPairs; ++j) {
+      const float2 gj = mul2(make_float2(gr[2 * j], gr[2 * j + 1]), both(c.grad_scale));
+      m[j] = add2(mul2(m[j], both(c.beta1)), mul2(gj, both(c.one_beta1)), c.one);
+      v[j] = add2(mul2(v[j], both(c.beta2)), mul2(mul2(gj, gj), both(c.one_beta2)), c.one);
+      largest = max(max(largest, __float_as_uint(v[j].x)), __float_as_uint(v[j].y));
+      smallest = min(min(smallest, __float_as_uint(v[j].x)), __float_as_uint(v[j].y));
     }
-    float root[kEach];
-    if (root_is_plain(largest, smallest)) {
+    const bool plain = root_is_plain(largest, smallest);
+    float im = 0.0f, ir = 0.0f;
+    bool one = true;
+    if constexpr (BITS == 8) {
+      float top_m = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kEach; ++j) root[j] = root_of(v[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) root[j] = sqrtf(v[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < kEach; ++j)
-      p[j] = p[j] * c.keep - quotient(m[j], root[j] * c.inv_root_bc2 + c.eps) * c.step_size;
-    const bool full = left >= kEach;
-    store_each(param, p, left, full && vec);
-    if constexpr (MASTER) store_each(a.master + at, p, left, full);
-    if constexpr (BITS == 32) {
-      store_each(static_cast<float *>(a.moment1) + at, m, left, full);
-      store_each(static_cast<float *>(a.moment2) + at, v, left, full);
-    } else {
-      float top_m = 0.0f, top_r = 0.0f;
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        top_m = larger(top_m, fabsf(m[j]));
-        top_r = larger(top_r, root[j]);
-      }
+      for (int j = 0; j < kPairs; ++j) top_m = larger(larger(top_m, fabsf(m[j].x)), fabsf(m[j].y));
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) {
         top_m = larger(top_m, __shfl_xor_sync(0xffffffffu, top_m, o));
-        top_r = larger(top_r, __shfl_xor_sync(0xffffffffu, top_r, o));
+        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));  // v >= 0: its bits are in its order
       }
-      if (left <= 0) return;
+      const float top_r = sqrtf(__uint_as_float(largest));  // the largest root is the root of the largest
       const unsigned fm = scale_field(__float_as_uint(top_m) & 0x7FFFFFFFu), fr = scale_field(__float_as_uint(top_r) & 0x7FFFFFFFu);
-      const unsigned key = hash_key((unsigned long long)at, c.step, a.seed);  // at is a multiple of eight
-      unsigned em[kEach], er[kEach];
-      // the scale's inverse and e4m3's shift of 2^-120 are one factor unless it would fall below float's
-      // smallest normal number: moments beyond 448 * 64
-      if (fm <= 133u && fr <= 133u) {
-        const float im = __uint_as_float((134u - fm) << 23), ir = __uint_as_float((134u - fr) << 23);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          const unsigned h = hash_bits(key ^ unsigned(j));
-          em[j] = encode(fabsf(m[j]) * im, h << 4);
-          er[j] = encode(root[j] * ir, h >> 12);
-        }
-      } else {
-        const float im = inv_scale_of(fm), ir = inv_scale_of(fr);
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-          const unsigned h = hash_bits(key ^ unsigned(j));
-          em[j] = encode(fabsf(m[j]) * im * 0x1p-120f, h << 4);
-          er[j] = encode(root[j] * ir * 0x1p-120f, h >> 12);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kEach; ++j) {
-        em[j] |= m[j] < 0.0f ? 128u : 0u;
-        er[j] = max(er[j], min(__float_as_uint(root[j]), 1u));  // above zero stays above zero
-      }
-      const auto pack = [](const unsigned *e) { return e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24; };
-      *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(a.moment1) + at) = make_uint2(pack(em), pack(em + 4));
-      *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(a.moment2) + at) = make_uint2(pack(er), pack(er + 4));
-      if (threadIdx.x % kLanes == 0) {
+      if (threadIdx.x % kLanes == 0 && left > 0) {
         a.scale1[at / kMomentBlock] = scale_of(fm);
         a.scale2[at / kMomentBlock] = scale_of(fr);
       }
+      // The scale's inverse and e4m3's shift of 2^-120 are one factor unless it would fall below float's
+      // smallest normal number (moments beyond 448 * 64): then the second factor follows.
+      one = fm <= 133u && fr <= 133u;
+      im = one ? __uint_as_float((134u - fm) << 23) : inv_scale_of(fm);
+      ir = one ? __uint_as_float((134u - fr) << 23) : inv_scale_of(fr);
+    }
+    if (left <= 0) return;
+    // zeros and very small or large second moments take a path of their own: it is the same step
+    if (plain) finish<true>(a, c, param, at, left, vec, pr, m, v, im, ir, one);
+    else finish<false>(a, c, param, at, left, vec, pr, m, v, im, ir, one);
+  }
+
+  // from the moments on; PLAIN: all second moments are in [2^-100, 2^126]
+  template <bool PLAIN>
+  __device__ __forceinline__ void finish(const AdamWLaunch &a, const Scalars &c, P *param, long long at, int left, bool vec,
+                                         float (&pr)[kEach], const float2 (&m)[kPairs], const float2 (&v)[kPairs],
+                                         float im, float ir, bool one) const {
+    float2 p[kPairs], root[kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) root[j] = PLAIN ? root_of(v[j]) : make_float2(sqrtf(v[j].x), sqrtf(v[j].y));
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      const float2 below = add2(mul2(root[j], both(c.inv_root_bc2)), both(c.eps), c.one);
+      const float2 part = mul2(make_float2(quotient(m[j].x, below.x), quotient(m[j].y, below.y)), both(-c.step_size));
+      p[j] = add2(mul2(make_float2(pr[2 * j], pr[2 * j + 1]), both(c.keep)), part, c.one);
+    }
+    const auto flat = [](const float2 (&x)[kPairs], float (&y)[kEach]) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) y[2 * j] = x[j].x, y[2 * j + 1] = x[j].y;
+    };
+    const bool full = left >= kEach;
+    flat(p, pr);
+    store_each(param, pr, left, full && vec);
+    if constexpr (MASTER) store_each(a.master + at, pr, left, full);
+    if constexpr (BITS == 32) {
+      float x[kEach];
+      flat(m, x);
+      store_each(static_cast<float *>(a.moment1) + at, x, left, full);
+      flat(v, x);
+      store_each(static_cast<float *>(a.moment2) + at, x, left, full);
+    } else {
+      unsigned em[kEach], er[kEach];
+      const unsigned key = hash_key((unsigned long long)at, c.step, a.seed);  // at is a multiple of eight
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        const float2 mj = m[j / 2], rj = root[j / 2];
+        const float mx = j % 2 ? mj.y : mj.x, rx = j % 2 ? rj.y : rj.x;
+        float ym = fabsf(mx) * im, yr = rx * ir;
+        if (!one) ym *= 0x1p-120f, yr *= 0x1p-120f;
+        const unsigned h = hash_before_last(key ^ unsigned(j)), upper = h >> 12;
+        // the code in the upper byte, below the sign; a root above zero stays above zero
+        em[j] = dithered(ym, ((h << 4) ^ upper) & 0xFFFF0u) << 4 | (__float_as_uint(mx) & 0x80000000u);
+        er[j] = max(dithered(yr, upper & 0xFFFF0u), PLAIN ? kCodeOne : min(__float_as_uint(rx), kCodeOne)) << 4;
+      }
+      *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(a.moment1) + at) =
+          make_uint2(upper_bytes(em[0], em[1], em[2], em[3]), upper_bytes(em[4], em[5], em[6], em[7]));
+      *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(a.moment2) + at) =
+          make_uint2(upper_bytes(er[0], er[1], er[2], er[3]), upper_bytes(er[4], er[5], er[6], er[7]));
     }
   }
 };
@@ -273,25 +314,21 @@ __device__ __forceinline__ void step_chunk(const AdamWLaunch &a, const Scalars &
   const long long slot = t.slot + first;
   const int n = int(min(t.n - first, (long long)kAdamWChunk));
   // a thread behind the end (n - i <= 0) loads and stores nothing, but takes part in the shuffles
-  int i = threadIdx.x * kEach;
-  Tile<BITS, P, G, MASTER> tile;
-  if constexpr (BITS == 8) tile.load(a, param + i, grad + i, slot + i, n - i, vec, grad_vec);
+  constexpr int kTileElems = kThreads<BITS> * kEach;  // elements of a CTA at a time
 #pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += kTileElems, i += kTileElems) {
-    if constexpr (BITS == 8) {  // few bytes and much arithmetic: the next tile is on its way meanwhile
-      const Tile<BITS, P, G, MASTER> now = tile;
-      const int next = i + kTileElems;
-      tile.load(a, param + next, grad + next, slot + next, n - next, vec, grad_vec);
-      now.step(a, c, param + i, slot + i, n - i, vec);
-    } else {
-      tile.load(a, param + i, grad + i, slot + i, n - i, vec, grad_vec);
-      tile.step(a, c, param + i, slot + i, n - i, vec);
-    }
+  for (int i0 = 0; i0 < n; i0 += kTileElems) {
+    const int i = i0 + threadIdx.x * kEach;
+    Tile<BITS, P, G, MASTER> tile;
+    tile.load(a, param + i, grad + i, slot + i, n - i, vec, grad_vec);
+    tile.step(a, c, param + i, slot + i, n - i, vec);
   }
 }
 
+// Many small CTAs: with moments in 8 bits the step is bound by issued instructions (71 an element) and
+// wants as many warps as 40 registers allow: 128 M elements take 308 us with 12 CTAs of 128 threads an
+// SM, 354 with 5 of 256.  Moments in 32 bits are bound by memory: 64 M elements with a copy take 276 us.
 template <int BITS, bool MASTER>
-__global__ void __launch_bounds__(kThreads, BITS == 8 ? 3 : 4) adamw_kernel(AdamWLaunch a, const __grid_constant__ GradPointers grads,
+__global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 12 : 4) adamw_kernel(AdamWLaunch a, const __grid_constant__ GradPointers grads,
                                                             int first_tensor, int first_chunk, int n_chunks, bool last) {
   __shared__ Scalars shared_scalars;
   if (threadIdx.x == 0) shared_scalars = scalars_of(a);
@@ -327,7 +364,7 @@ namespace {
 template <int BITS, bool MASTER>
 void launch_with(const AdamWLaunch &a, const GradPointers &g, int first_tensor, int first_chunk, int chunks, bool last,
                  cudaStream_t s) {
-  adamw_kernel<BITS, MASTER><<<std::max(1, chunks), kThreads, 0, s>>>(a, g, first_tensor, first_chunk, chunks, last);
+  adamw_kernel<BITS, MASTER><<<std::max(1, chunks), kThreads<BITS>, 0, s>>>(a, g, first_tensor, first_chunk, chunks, last);
   ARB_CUDA(cudaGetLastError());
   count_launch();
 }

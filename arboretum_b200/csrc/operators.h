@@ -101,6 +101,7 @@ struct AdamWState {  // device: the step count and what follows from it, advance
   float inv_root_bc2;       // 1 / sqrt(1 - beta2_t)
   unsigned done;            // CTAs of the running step that have finished
   long long step;           // steps taken
+  float one;                // 1
   __host__ __device__ void derive() {
     inv_bc1 = 1.0 / (1.0 - beta1_t);
     inv_root_bc2 = float(1.0 / sqrt(1.0 - beta2_t));

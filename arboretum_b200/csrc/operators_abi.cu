@@ -108,6 +108,7 @@ void put_step(AdamW *o, int64_t step, cudaStream_t s) {
   st.beta2_t = std::pow(o->launch.beta2, double(step) + 1);
   st.step = step;
   st.done = 0;
+  st.one = 1.0f;
   st.derive();
   ARB_CUDA(cudaMemcpyAsync(o->launch.state, &st, sizeof st, cudaMemcpyHostToDevice, s));
   ARB_CUDA(cudaStreamSynchronize(s));

@@ -333,7 +333,7 @@ def _encode(x, index, step, seed, shift, positive):
     fe = np.maximum(np.frexp(value)[1] - 1, -6)
     f = np.round(value / 2.0 ** (fe - 3)).astype(np.int64)  # 8 .. 15, or below 8 at the smallest exponent
     code = np.where(f >= 8, (fe + 7) * 8 + (f - 8), f)
-    return (code | np.where(x < 0, 128, 0)).astype(np.uint8), scale.astype(np.float32)
+    return (code | np.where(np.signbit(x), 128, 0)).astype(np.uint8), scale.astype(np.float32)
 
 
 class Plain:
