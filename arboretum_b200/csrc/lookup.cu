@@ -162,46 +162,48 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunc
 // table's values come from shared memory, where 32 random words cost a few cycles and a gather
 // through the first-level cache one for every line it touches.
 constexpr int kTableThreads = 1024;
-template <typename I, int DIM, int K>
-__device__ __forceinline__ void add_table(const float *values, unsigned rows, const I *p, long long step, long long other,
-                                          bool paired, float (&sum)[2][DIM]) {
+// tokens of two bags, K slots
+template <typename I, int K>
+struct TokenPairs {
   struct alignas(2 * sizeof(I)) Both { I v[2]; };
   Both tok[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
+  __device__ __forceinline__ void load(const I *p, long long step, long long other, bool paired) {
     if (paired) {  // one access for both bags
-      tok[k] = *reinterpret_cast<const Both *>(p);
+#pragma unroll
+      for (int k = 0; k < K; ++k) tok[k] = *reinterpret_cast<const Both *>(p + k * step);
     } else {
-      tok[k].v[0] = p[0];
-      tok[k].v[1] = p[other];
+#pragma unroll
+      for (int k = 0; k < K; ++k) tok[k].v[0] = p[k * step], tok[k].v[1] = p[k * step + other];
     }
-    p += step;
   }
+  template <int DIM>
+  __device__ __forceinline__ void add(const float *values, unsigned rows, float (&sum)[2][DIM]) const {
+    using U = typename std::make_unsigned<I>::type;
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+    for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      using U = typename std::make_unsigned<I>::type;
-      const unsigned r = U(tok[k].v[e]) < U(rows) ? unsigned(tok[k].v[e]) : rows;
+      for (int e = 0; e < 2; ++e) {
+        const unsigned r = U(tok[k].v[e]) < U(rows) ? unsigned(tok[k].v[e]) : rows;
 #pragma unroll
-      for (int d = 0; d < DIM; ++d) sum[e][d] += values[r * DIM + d];
-    }
-}
+        for (int d = 0; d < DIM; ++d) sum[e][d] += values[r * DIM + d];
+      }
+  }
+};
 
 template <typename T, typename O, typename I, int DIM>
 __global__ void __launch_bounds__(kTableThreads) lookup_table_kernel(LookupLaunch a, bool paired) {
   extern __shared__ float values[];  // [rows][DIM], and a row of zeros for empty slots
   const unsigned rows = unsigned(a.rows);
-  for (unsigned i = threadIdx.x; i < (rows + 1) * DIM; i += kTableThreads) {
+  for (unsigned i = threadIdx.x; i < (rows + 1) * DIM; i += blockDim.x) {
     const unsigned r = i / DIM, d = i - r * DIM;
     values[i] = r < rows ? to_f32(static_cast<const T *>(a.table)[(long long)r * a.row_stride + d]) : 0.0f;
   }
   __syncthreads();
-  constexpr int K = 8;  // tokens of a bag in flight
-  const int per_bag = int(a.tokens.per_bag);
+  constexpr int K = 32 / int(sizeof(I));  // slots whose tokens are under way while as many others are summed
+  const int per_bag = int(a.tokens.per_bag), full = per_bag / K * K;
   const long long step = a.tokens.token_stride;
-  for (long long b = (blockIdx.x * (long long)kTableThreads + threadIdx.x) * 2; b < a.tokens.bags;
-       b += (long long)gridDim.x * kTableThreads * 2) {
+  for (long long b = (blockIdx.x * (long long)blockDim.x + threadIdx.x) * 2; b < a.tokens.bags;
+       b += (long long)gridDim.x * blockDim.x * 2) {
     const bool two = b + 1 < a.tokens.bags;
     const long long other = two ? a.tokens.bag_stride : 0;  // a last bag alone is summed twice
     const bool both = paired && two;
@@ -209,9 +211,25 @@ __global__ void __launch_bounds__(kTableThreads) lookup_table_kernel(LookupLaunc
     float sum[2][DIM];
 #pragma unroll
     for (int d = 0; d < DIM; ++d) sum[0][d] = sum[1][d] = 0.0f;
-    int k = 0;
-    for (; k + K <= per_bag; k += K, p += K * step) add_table<I, DIM, K>(values, rows, p, step, other, both, sum);
-    for (; k < per_bag; ++k, p += step) add_table<I, DIM, 1>(values, rows, p, step, other, both, sum);
+    if (full) {
+      TokenPairs<I, K> now;
+      now.load(p, step, other, both);
+#pragma unroll 2
+      for (int k = K; k < full; k += K) {
+        p += K * step;
+        TokenPairs<I, K> next;
+        next.load(p, step, other, both);
+        now.add(values, rows, sum);
+        now = next;
+      }
+      now.add(values, rows, sum);
+      p += K * step;
+    }
+    for (int k = full; k < per_bag; ++k, p += step) {
+      TokenPairs<I, 1> last;
+      last.load(p, step, other, both);
+      last.add(values, rows, sum);
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
       if (e == 0 || two) {
@@ -357,7 +375,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortPass p) {
       const unsigned digit = (key[j] >> p.shift) & (kDigits - 1);
       const unsigned to = base[digit] + warp_cnt[w][digit] + rank[j];
       p.key_out[to] = key[j];
-      if (p.local_out) p.local_out[to] = (unsigned short)(bag[j] & (kBlockBags - 1));
+      if (p.local_out) p.local_out[to] = (unsigned short)((bag[j] & (kBlockBags - 1)) * 4);
       else p.bag_out[to] = bag[j];
     }
   }
@@ -623,52 +641,83 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGr
 // values from shared memory.  (Gathered through the second-level cache, 4 bytes of a 32-byte sector
 // each, the same sums of 128 M leaf tokens took 478 us, that cache's bandwidth.)
 constexpr int kNarrowThreads = 512, kNarrowLanes = 8;  // lanes a row
-constexpr unsigned kLongRow = 512;                     // tokens from which a warp takes a row together
+constexpr int kNarrowEach = 8;                         // neighbouring positions of a lane: one access of 16 bytes
+constexpr unsigned kLongRow = 512;                     // bags from which a warp takes a row together
 
-template <int DIM>
-__device__ __forceinline__ void add_narrow(const float *grads, const unsigned short *__restrict__ local, unsigned p0,
-                                           unsigned p1, int lane, int lanes, float (&sum)[DIM]) {
-  constexpr int K = 8;
-  for (unsigned p = p0 + lane; p < p1; p += lanes * K) {
-    unsigned at[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) at[k] = p + k * lanes < p1 ? local[p + k * lanes] : unsigned(kBlockBags);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int d = 0; d < DIM; ++d) sum[d] += grads[at[k] * DIM + d];
+// A lane's eight positions from `at` on (a multiple of eight) that lie in p0 .. p1.
+struct NarrowIds {
+  uint4 ids;
+  unsigned valid;  // bit j: position at + j is the row's
+  __device__ __forceinline__ void load(const unsigned short *__restrict__ local, unsigned at, unsigned p0, unsigned p1) {
+    const unsigned lo = at < p0 ? p0 - at : 0u;  // below eight: at is no more than seven before p0
+    const unsigned hi = at < p1 ? min(p1 - at, 8u) : 0u;
+    valid = hi > lo ? (1u << hi) - (1u << lo) : 0u;
+    ids = make_uint4(0u, 0u, 0u, 0u);
+    if (valid) ids = *reinterpret_cast<const uint4 *>(local + at);
   }
-}
+  template <int DIM>
+  __device__ __forceinline__ void add(const float *grads, float (&sum)[DIM]) const {
+    const unsigned word[4] = {ids.x, ids.y, ids.z, ids.w};
+#pragma unroll
+    for (int j = 0; j < kNarrowEach; ++j) {
+      const unsigned offset = (j % 2 ? word[j / 2] >> 16 : word[j / 2] & 0xFFFFu) * DIM;  // bytes: ids are kept times four
+      if (valid >> j & 1u) {
+#pragma unroll
+        for (int d = 0; d < DIM; ++d) sum[d] += *reinterpret_cast<const float *>(reinterpret_cast<const char *>(grads) + offset + 4 * d);
+      }
+    }
+  }
+};
 
+// Bound by latency unless the next rows' accesses are under way: while a row group is summed, the bags of
+// the next one and the first positions of the one after it are being fetched.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradLaunch a, TokenOrder o, float *__restrict__ partial) {
-  extern __shared__ float grads[];  // [kBlockBags][DIM], and zeros for positions past a row's end
+  extern __shared__ float grads[];  // [kBlockBags][DIM]
+  overlap_release();
+  overlap_wait();
   const long long bag0 = (long long)blockIdx.y * kBlockBags;
   const int n = int(min((long long)kBlockBags, o.bags - bag0));
   for (int i = threadIdx.x; i < n * DIM; i += kNarrowThreads) {
     const int r = i / DIM, d = i - r * DIM;
     grads[i] = to_f32(static_cast<const T *>(a.grad)[(bag0 + r) * a.grad_stride + d]);
   }
-  if (threadIdx.x < DIM) grads[kBlockBags * DIM + threadIdx.x] = 0.0f;
-  __syncthreads();
   const unsigned *begin = o.begin + size_t(blockIdx.y) * (o.rows + 1);
   float *out = partial + size_t(blockIdx.y) * o.rows * DIM;
   const int lane = threadIdx.x & 31, part = lane & (kNarrowLanes - 1);
   constexpr int kRows = 32 / kNarrowLanes;  // rows of a warp at a time
+  constexpr int kStep = kNarrowThreads / 32 * kRows;
   const long long v_end = min((long long)o.rows, (blockIdx.x + 1ll) * a.rows_per_cta);
-  for (long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * kRows; v0 < v_end;
-       v0 += kNarrowThreads / 32 * kRows) {
-    const long long v = v0 + lane / kNarrowLanes;
-    unsigned p0 = 0, p1 = 0;
-    if (v < v_end) p0 = begin[v], p1 = begin[v + 1];
-    const bool is_long = p1 - p0 >= kLongRow;
+  long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * kRows;
+  const auto range = [&](long long w0) {  // positions of this lane's row of the group that begins with row w0
+    const long long v = w0 + lane / kNarrowLanes;
+    return v < v_end ? make_uint2(begin[v], begin[v + 1]) : make_uint2(0u, 0u);
+  };
+  const auto first_at = [&](uint2 r) { return (r.x & ~7u) + kNarrowEach * part; };
+  uint2 now = range(v0), next = range(v0 + kStep);
+  NarrowIds ids;
+  ids.load(o.local, first_at(now), now.x, now.y);
+  __syncthreads();
+  for (; v0 < v_end; v0 += kStep) {  // the same for the whole warp
+    const uint2 after = range(v0 + 2 * kStep);
+    NarrowIds ids_next;
+    ids_next.load(o.local, first_at(next), next.x, next.y);
+    const bool is_long = now.y - now.x >= kLongRow;
     float sum[DIM];
 #pragma unroll
     for (int d = 0; d < DIM; ++d) sum[d] = 0.0f;
-    add_narrow<DIM>(grads, o.local, p0, is_long ? p0 : p1, part, kNarrowLanes, sum);
+    if (!is_long) {
+      ids.add<DIM>(grads, sum);
+      for (unsigned at = first_at(now) + kNarrowLanes * kNarrowEach; at < now.y; at += kNarrowLanes * kNarrowEach) {
+        NarrowIds more;
+        more.load(o.local, at, now.x, now.y);
+        more.add<DIM>(grads, sum);
+      }
+    }
 #pragma unroll
     for (int d = 0; d < DIM; ++d)
       for (int s = 1; s < kNarrowLanes; s <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], s);
+    const long long v = v0 + lane / kNarrowLanes;
     if (part == 0 && v < v_end && !is_long)
 #pragma unroll
       for (int d = 0; d < DIM; ++d) out[v * DIM + d] = sum[d];
@@ -676,11 +725,15 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradL
     while (todo) {
       const int src = __ffs(todo) - 1;
       todo &= todo - 1;
-      const unsigned q0 = __shfl_sync(0xffffffffu, p0, src), q1 = __shfl_sync(0xffffffffu, p1, src);
+      const unsigned q0 = __shfl_sync(0xffffffffu, now.x, src), q1 = __shfl_sync(0xffffffffu, now.y, src);
       float all[DIM];
 #pragma unroll
       for (int d = 0; d < DIM; ++d) all[d] = 0.0f;
-      add_narrow<DIM>(grads, o.local, q0, q1, lane, 32, all);
+      for (unsigned at = (q0 & ~7u) + kNarrowEach * lane; at < q1; at += 32 * kNarrowEach) {
+        NarrowIds more;
+        more.load(o.local, at, q0, q1);
+        more.add<DIM>(grads, all);
+      }
 #pragma unroll
       for (int d = 0; d < DIM; ++d)
         for (int s = 1; s < 32; s <<= 1) all[d] += __shfl_xor_sync(0xffffffffu, all[d], s);
@@ -688,6 +741,9 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradL
 #pragma unroll
         for (int d = 0; d < DIM; ++d) out[(v0 + src / kNarrowLanes) * DIM + d] = all[d];
     }
+    now = next;
+    next = after;
+    ids = ids_next;
   }
 }
 
@@ -696,6 +752,8 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradL
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLaunch a, TokenOrder o, int tx_bits, int vecs,
                                                                     int chunks, int splits, float *__restrict__ partial) {
+  overlap_release();
+  overlap_wait();
   const int tx = 1 << tx_bits, lane = threadIdx.x & (tx - 1);
   const long long v = blockIdx.x * (long long)(kGradThreads >> tx_bits) + (threadIdx.x >> tx_bits);
   if (v >= o.rows) return;
@@ -717,7 +775,7 @@ __global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLa
 #pragma unroll
         for (int i = 0; i < K; ++i) {
           x[i].clear();
-          if (p + i < p1) x[i].load(grad + (bag0 + o.local[p + i]) * a.grad_stride);
+          if (p + i < p1) x[i].load(grad + (bag0 + o.local[p + i] / 4) * a.grad_stride);
         }
 #pragma unroll
         for (int i = 0; i < K; ++i) x[i].add_to(sum);
@@ -729,15 +787,28 @@ __global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLa
   }
 }
 
-// the shares' sums, joined in their order
+// the shares' sums: eight groups of lanes take every eighth share, and their sums are added in order
 template <typename O>
 __global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLaunch a, long long rows, int splits,
                                                                     const float *__restrict__ partial) {
+  __shared__ float part[kGradThreads];
+  constexpr int kSlices = kGradThreads / 32;
+  overlap_release();
+  overlap_wait();
+  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   const long long n = rows * a.dim;
-  for (long long i = blockIdx.x * (long long)kGradThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kGradThreads) {
+  for (long long i0 = blockIdx.x * 32ll; i0 < n; i0 += gridDim.x * 32ll) {
+    const long long i = i0 + lane;
     float sum = 0.0f;
+    if (i < n)
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) sum += partial[size_t(k) * n + i];
+      for (int k = slice; k < splits; k += kSlices) sum += partial[size_t(k) * n + i];
+    __syncthreads();
+    part[threadIdx.x] = sum;
+    __syncthreads();
+    if (slice != 0 || i >= n) continue;
+#pragma unroll
+    for (int g = 1; g < kSlices; ++g) sum += part[g * 32 + lane];
     sum *= a.scale;
     O *at = static_cast<O *>(a.out) + i / a.dim * a.out_stride + i % a.dim;
     if (!a.accumulate) from_f32(sum, *at);
@@ -982,7 +1053,11 @@ void lookup_table_with(const LookupLaunch &a, cudaStream_t s) {
   const size_t smem = size_t(a.rows + 1) * DIM * sizeof(float);
   const bool paired = a.tokens.bag_stride == 1 && a.tokens.token_stride % 2 == 0 &&
                       reinterpret_cast<uintptr_t>(a.tokens.at) % (2 * sizeof(I)) == 0;
-  lookup_table_kernel<T, O, I, DIM><<<device_sm_count(), kTableThreads, smem, s>>>(a, paired);
+  // as many rounds as 1024 threads an SM need, and then no more threads than fill them evenly
+  const int64_t pairs = (a.tokens.bags + 1) / 2, sms = device_sm_count();
+  const int64_t rounds = (pairs + sms * kTableThreads - 1) / (sms * kTableThreads);
+  const int threads = int(std::max<int64_t>(256, ((pairs + sms * rounds - 1) / (sms * rounds) + 31) / 32 * 32));
+  lookup_table_kernel<T, O, I, DIM><<<int(sms), threads, smem, s>>>(a, paired);
 }
 
 template <typename T, typename O>
@@ -1166,7 +1241,7 @@ template <typename T, int DIM>
 void narrow_grad_with(LookupGradLaunch a, const TokenOrder &o, float *partial, cudaStream_t s) {
   static bool ready[kMaxDevices] = {};
   const int dev = current_device();
-  constexpr int smem = (kBlockBags + 1) * DIM * int(sizeof(float));
+  constexpr int smem = kBlockBags * DIM * int(sizeof(float));
   if (!ready[dev]) {
     ARB_CUDA(cudaFuncSetAttribute(narrow_grad_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ready[dev] = true;
@@ -1177,7 +1252,7 @@ void narrow_grad_with(LookupGradLaunch a, const TokenOrder &o, float *partial, c
   constexpr int kStep = kNarrowThreads / kNarrowLanes;  // rows a CTA takes at a time
   a.rows_per_cta = int(std::max<int64_t>(kStep, ((o.rows + shares - 1) / shares + kStep - 1) / kStep * kStep));
   const dim3 grid(unsigned((o.rows + a.rows_per_cta - 1) / a.rows_per_cta), unsigned(o.blocks));
-  narrow_grad_kernel<T, DIM><<<grid, kNarrowThreads, smem, s>>>(a, o, partial);
+  launch_overlapped(narrow_grad_kernel<T, DIM>, grid, dim3(kNarrowThreads), smem, s, a, o, partial);
 }
 
 template <typename T, int VEC>
@@ -1187,7 +1262,7 @@ void blocked_grad_with(const LookupGradLaunch &a, const TokenOrder &o, int split
   const int chunks = (vecs + (1 << tx_bits) - 1) >> tx_bits;
   const int64_t groups = kGradThreads >> tx_bits;
   const dim3 grid(unsigned((o.rows + groups - 1) / groups), unsigned(std::min(chunks, 65535)), unsigned(splits));
-  blocked_grad_kernel<T, VEC><<<grid, kGradThreads, 0, s>>>(a, o, tx_bits, vecs, chunks, splits, partial);
+  launch_overlapped(blocked_grad_kernel<T, VEC>, grid, dim3(kGradThreads), 0, s, a, o, tx_bits, vecs, chunks, splits, partial);
 }
 
 template <typename T, typename O>
@@ -1200,7 +1275,8 @@ void blocked_grad(const LookupGradLaunch &a, const TokenOrder &o, int vec, float
   else if (vec * sizeof(T) == 16) blocked_grad_with<T, 16 / sizeof(T)>(a, o, splits, partial, s);
   else if (vec * sizeof(T) >= 4) blocked_grad_with<T, 4 / sizeof(T)>(a, o, splits, partial, s);
   else blocked_grad_with<T, 1>(a, o, splits, partial, s);
-  blocked_join_kernel<O><<<grid_of(o.rows * a.dim, kGradThreads, 8), kGradThreads, 0, s>>>(a, o.rows, splits, partial);
+  launch_overlapped(blocked_join_kernel<O>, dim3(grid_of(o.rows * a.dim, 32, 32)), dim3(kGradThreads), 0, s, a,
+                    (long long)o.rows, splits, static_cast<const float *>(partial));
   count_launch();
 }
 
