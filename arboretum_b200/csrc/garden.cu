@@ -1818,7 +1818,7 @@ void Garden::RefineLeaves(DataMatrix *data, const Refinement &r) {
   const TokenOrder shape(nullptr, int64_t(n), per_class, rows);
   DevBuf d_orders, d_scratch;
   d_orders.alloc(shape.bytes * K);
-  d_scratch.alloc(std::max<size_t>(256, std::max(token_order_scratch(shape.count), lookup_grad_scratch(shape, 1))));
+  d_scratch.alloc(std::max<size_t>(256, std::max(token_order_scratch(shape), lookup_grad_scratch(shape, 1))));
   for (size_t k = 0; k < K; ++k) {
     views.push_back(TokenView{d_tokens.as<int>() + k * n, 4, int64_t(n), per_class, 1, int64_t(K * n)});
     orders.push_back(TokenOrder(d_orders.as<char>() + k * shape.bytes, int64_t(n), per_class, rows));

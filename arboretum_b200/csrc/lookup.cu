@@ -259,7 +259,6 @@ struct SortPass {
   int tiles, shift;
   bool first, by_slot;     // by_slot: pairs are numbered slot after slot (neighbouring bags lie side by side)
   bool blocked;            // keys are (run of bags, token)
-  unsigned short *local_out;  // last pass of a blocked order: bags within their run
 };
 
 __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsigned &key, unsigned &bag) {
@@ -274,7 +273,7 @@ __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsign
   const long long row = row_at(p.tokens, p.rows, b, k);
   key = row >= 0 ? unsigned(row) : unsigned(p.rows);
   bag = unsigned(b);
-  if (p.blocked) key += (bag >> kBlockBits) * unsigned(p.rows + 1);
+  if (p.blocked) key += bag / kBlockBags * unsigned(p.rows + 1);
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
@@ -375,8 +374,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortPass p) {
       const unsigned digit = (key[j] >> p.shift) & (kDigits - 1);
       const unsigned to = base[digit] + warp_cnt[w][digit] + rank[j];
       p.key_out[to] = key[j];
-      if (p.local_out) p.local_out[to] = (unsigned short)((bag[j] & (kBlockBags - 1)) * 4);
-      else p.bag_out[to] = bag[j];
+      p.bag_out[to] = bag[j];
     }
   }
 }
@@ -401,6 +399,55 @@ __global__ void order_begin_kernel(const unsigned *__restrict__ key, long long n
       const long long l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
       for (long long v = l + lane; v <= h; v += 32) begin[v] = unsigned(w * 32 + src);
     }
+  }
+}
+
+// ---- vectors of a blocked order ----------------------------------------------------------------
+// A segment (run, row) takes as many vectors of eight bags as it needs, the empty slots behind a run's
+// last row none.  Sums over tiles of segments, their exclusive sums, then every segment's first vector.
+constexpr int kVecTile = 2048;
+__device__ __forceinline__ unsigned vectors_of(const unsigned *__restrict__ begin, long long k, const TokenOrder &o) {
+  return k < o.segments() && k % (o.rows + 1) != o.rows ? (begin[k + 1] - begin[k] + 7) / 8 : 0u;
+}
+__global__ void __launch_bounds__(256) vec_count_kernel(const unsigned *__restrict__ begin, TokenOrder o, unsigned *__restrict__ tile) {
+  unsigned sum = 0;
+  for (int j = 0; j < kVecTile / 256; ++j) sum += vectors_of(begin, blockIdx.x * (long long)kVecTile + j * 256 + threadIdx.x, o);
+  unsigned all;
+  block_exclusive(sum, &all);
+  if (threadIdx.x == 0) tile[blockIdx.x] = all;
+}
+__global__ void __launch_bounds__(256) vec_tiles_kernel(unsigned *tile, int tiles) {
+  unsigned run = 0;
+  for (int t = 0; t < tiles; t += 256) {
+    const int i = t + int(threadIdx.x);
+    const unsigned v = i < tiles ? tile[i] : 0u;
+    unsigned all;
+    const unsigned before = block_exclusive(v, &all);
+    if (i < tiles) tile[i] = run + before;
+    run += all;
+  }
+}
+__global__ void __launch_bounds__(256) vec_begin_kernel(const unsigned *__restrict__ begin, TokenOrder o, const unsigned *__restrict__ tile) {
+  unsigned run = tile[blockIdx.x];
+  for (int j = 0; j < kVecTile / 256; ++j) {
+    const long long k = blockIdx.x * (long long)kVecTile + j * 256 + threadIdx.x;
+    const unsigned n = vectors_of(begin, k, o);
+    unsigned all;
+    const unsigned first = run + block_exclusive(n, &all);
+    run += all;
+    if (k > o.segments()) continue;
+    o.vec_begin[k] = first;
+    if (n)  // the end of the last vector
+      for (unsigned p = begin[k + 1] - begin[k]; p < n * 8; ++p) o.local[size_t(first) * 8 + p] = kNoBag;
+  }
+}
+__global__ void vec_move_kernel(const unsigned *__restrict__ key, const unsigned *__restrict__ bag, const unsigned *__restrict__ begin,
+                                TokenOrder o) {
+  const unsigned rows1 = unsigned(o.rows + 1);
+  for (long long p = blockIdx.x * (long long)blockDim.x + threadIdx.x; p < o.count; p += (long long)gridDim.x * blockDim.x) {
+    const unsigned k = key[p], run = k / rows1;
+    if (k - run * rows1 == unsigned(o.rows)) continue;
+    o.local[size_t(o.vec_begin[k]) * 8 + (unsigned(p) - begin[k])] = (unsigned short)((bag[p] - run * kBlockBags) * 4);
   }
 }
 
@@ -638,42 +685,17 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGr
 // ---- the gradient over a blocked order -------------------------------------------------------
 // Narrow rows: a CTA brings the gradients of one run of bags into shared memory and sums the rows of
 // its share of the table over them: 2 bytes a token are read from device memory, the gradient's
-// values from shared memory.  (Gathered through the second-level cache, 4 bytes of a 32-byte sector
-// each, the same sums of 128 M leaf tokens took 478 us, that cache's bandwidth.)
-constexpr int kNarrowThreads = 512, kNarrowLanes = 8;  // lanes a row
-constexpr int kNarrowEach = 8;                         // neighbouring positions of a lane: one access of 16 bytes
-constexpr unsigned kLongRow = 512;                     // bags from which a warp takes a row together
-
-// A lane's eight positions from `at` on (a multiple of eight) that lie in p0 .. p1.
-struct NarrowIds {
-  uint4 ids;
-  unsigned valid;  // bit j: position at + j is the row's
-  __device__ __forceinline__ void load(const unsigned short *__restrict__ local, unsigned at, unsigned p0, unsigned p1) {
-    const unsigned lo = at < p0 ? p0 - at : 0u;  // below eight: at is no more than seven before p0
-    const unsigned hi = at < p1 ? min(p1 - at, 8u) : 0u;
-    valid = hi > lo ? (1u << hi) - (1u << lo) : 0u;
-    ids = make_uint4(0u, 0u, 0u, 0u);
-    if (valid) ids = *reinterpret_cast<const uint4 *>(local + at);
-  }
-  template <int DIM>
-  __device__ __forceinline__ void add(const float *grads, float (&sum)[DIM]) const {
-    const unsigned word[4] = {ids.x, ids.y, ids.z, ids.w};
-#pragma unroll
-    for (int j = 0; j < kNarrowEach; ++j) {
-      const unsigned offset = (j % 2 ? word[j / 2] >> 16 : word[j / 2] & 0xFFFFu) * DIM;  // bytes: ids are kept times four
-      if (valid >> j & 1u) {
-#pragma unroll
-        for (int d = 0; d < DIM; ++d) sum[d] += *reinterpret_cast<const float *>(reinterpret_cast<const char *>(grads) + offset + 4 * d);
-      }
-    }
-  }
-};
-
-// Bound by latency unless the next rows' accesses are under way: while a row group is summed, the bags of
-// the next one and the first positions of the one after it are being fetched.
+// values from shared memory, where 32 random words take three to four cycles.  (Gathered through the
+// second-level cache, 4 bytes of a 32-byte sector each, the same sums of 128 M leaf tokens took 478 us,
+// that cache's bandwidth; a few lanes a row instead of a stream, 162 us.)
+//
+// A warp walks the vectors of 32 rows as one stream, 32 vectors at a time: a lane sums its vector's eight
+// values, a segmented sum over the lanes adds up the vectors of a row, and what is left of a row at the
+// end of the 32 is carried on.  Every address is known in advance, so the next vectors are on their way.
+constexpr int kNarrowThreads = 512;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradLaunch a, TokenOrder o, float *__restrict__ partial) {
-  extern __shared__ float grads[];  // [kBlockBags][DIM]
+  extern __shared__ float grads[];  // [kBlockBags][DIM], and zeros for kNoBag
   overlap_release();
   overlap_wait();
   const long long bag0 = (long long)blockIdx.y * kBlockBags;
@@ -682,68 +704,58 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradL
     const int r = i / DIM, d = i - r * DIM;
     grads[i] = to_f32(static_cast<const T *>(a.grad)[(bag0 + r) * a.grad_stride + d]);
   }
-  const unsigned *begin = o.begin + size_t(blockIdx.y) * (o.rows + 1);
-  float *out = partial + size_t(blockIdx.y) * o.rows * DIM;
-  const int lane = threadIdx.x & 31, part = lane & (kNarrowLanes - 1);
-  constexpr int kRows = 32 / kNarrowLanes;  // rows of a warp at a time
-  constexpr int kStep = kNarrowThreads / 32 * kRows;
-  const long long v_end = min((long long)o.rows, (blockIdx.x + 1ll) * a.rows_per_cta);
-  long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * kRows;
-  const auto range = [&](long long w0) {  // positions of this lane's row of the group that begins with row w0
-    const long long v = w0 + lane / kNarrowLanes;
-    return v < v_end ? make_uint2(begin[v], begin[v + 1]) : make_uint2(0u, 0u);
-  };
-  const auto first_at = [&](uint2 r) { return (r.x & ~7u) + kNarrowEach * part; };
-  uint2 now = range(v0), next = range(v0 + kStep);
-  NarrowIds ids;
-  ids.load(o.local, first_at(now), now.x, now.y);
+  if (threadIdx.x < DIM) grads[kBlockBags * DIM + threadIdx.x] = 0.0f;
   __syncthreads();
-  for (; v0 < v_end; v0 += kStep) {  // the same for the whole warp
-    const uint2 after = range(v0 + 2 * kStep);
-    NarrowIds ids_next;
-    ids_next.load(o.local, first_at(next), next.x, next.y);
-    const bool is_long = now.y - now.x >= kLongRow;
-    float sum[DIM];
+  const unsigned *begin = o.vec_begin + size_t(blockIdx.y) * (o.rows + 1);
+  float *out = partial + size_t(blockIdx.y) * o.rows * DIM;
+  const int lane = threadIdx.x & 31;
+  const unsigned below = (2u << lane) - 1u;  // this lane and those before it
+  const long long v_end = min((long long)o.rows, (blockIdx.x + 1ll) * a.rows_per_cta);
+  for (long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * 32; v0 < v_end; v0 += kNarrowThreads) {
+    // lane l looks after row v0 + l: its vectors are first .. last
+    const long long v = min(v0 + lane, (long long)v_end - 1);
+    const unsigned first = begin[v], last = v0 + lane < v_end ? begin[v + 1] : first;
+    const unsigned w_end = __shfl_sync(0xffffffffu, begin[v + 1], 31);
+    unsigned w0 = __shfl_sync(0xffffffffu, first, 0);
+    const uint4 *stream = reinterpret_cast<const uint4 *>(o.local) + lane;
+    const uint4 none = make_uint4(kNoBag * 0x10001u, kNoBag * 0x10001u, kNoBag * 0x10001u, kNoBag * 0x10001u);
+    float total[DIM], carry[DIM];
 #pragma unroll
-    for (int d = 0; d < DIM; ++d) sum[d] = 0.0f;
-    if (!is_long) {
-      ids.add<DIM>(grads, sum);
-      for (unsigned at = first_at(now) + kNarrowLanes * kNarrowEach; at < now.y; at += kNarrowLanes * kNarrowEach) {
-        NarrowIds more;
-        more.load(o.local, at, now.x, now.y);
-        more.add<DIM>(grads, sum);
+    for (int d = 0; d < DIM; ++d) total[d] = carry[d] = 0.0f;
+    uint4 ids = w0 + lane < w_end ? stream[w0] : none;
+    for (; w0 < w_end; w0 += 32) {
+      const uint4 next = w0 + 32 + lane < w_end ? stream[w0 + 32] : none;
+      const unsigned word[4] = {ids.x, ids.y, ids.z, ids.w};
+      float sum[DIM];
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) sum[d] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned offset = (j % 2 ? word[j / 2] >> 16 : word[j / 2] & 0xFFFFu) * DIM;
+#pragma unroll
+        for (int d = 0; d < DIM; ++d) sum[d] += *reinterpret_cast<const float *>(reinterpret_cast<const char *>(grads) + offset + 4 * d);
       }
-    }
+      // lanes whose vector is the first of its row
+      const unsigned starts = __reduce_or_sync(0xffffffffu, first != last && first - w0 < 32u ? 1u << (first - w0) : 0u);
+      const unsigned before = starts & below;
+      const int from = before ? 31 - __clz(before) : 0;  // first lane of this lane's row
 #pragma unroll
-    for (int d = 0; d < DIM; ++d)
-      for (int s = 1; s < kNarrowLanes; s <<= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], s);
-    const long long v = v0 + lane / kNarrowLanes;
-    if (part == 0 && v < v_end && !is_long)
+      for (int d = 0; d < DIM; ++d) {
 #pragma unroll
-      for (int d = 0; d < DIM; ++d) out[v * DIM + d] = sum[d];
-    unsigned todo = __ballot_sync(0xffffffffu, is_long && part == 0);
-    while (todo) {
-      const int src = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const unsigned q0 = __shfl_sync(0xffffffffu, now.x, src), q1 = __shfl_sync(0xffffffffu, now.y, src);
-      float all[DIM];
-#pragma unroll
-      for (int d = 0; d < DIM; ++d) all[d] = 0.0f;
-      for (unsigned at = (q0 & ~7u) + kNarrowEach * lane; at < q1; at += 32 * kNarrowEach) {
-        NarrowIds more;
-        more.load(o.local, at, q0, q1);
-        more.add<DIM>(grads, all);
+        for (int s = 1; s < 32; s <<= 1) {
+          const float x = __shfl_up_sync(0xffffffffu, sum[d], s);
+          if (lane - s >= from) sum[d] += x;
+        }
+        if (!before) sum[d] += carry[d];  // the row began in an earlier 32
+        carry[d] = __shfl_sync(0xffffffffu, sum[d], 31);
+        const float x = __shfl_sync(0xffffffffu, sum[d], int(last - 1 - w0) & 31);
+        if (first != last && last - 1 - w0 < 32u) total[d] = x;
       }
-#pragma unroll
-      for (int d = 0; d < DIM; ++d)
-        for (int s = 1; s < 32; s <<= 1) all[d] += __shfl_xor_sync(0xffffffffu, all[d], s);
-      if (lane == 0)
-#pragma unroll
-        for (int d = 0; d < DIM; ++d) out[(v0 + src / kNarrowLanes) * DIM + d] = all[d];
+      ids = next;
     }
-    now = next;
-    next = after;
-    ids = ids_next;
+    if (v0 + lane < v_end)
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) out[(v0 + lane) * DIM + d] = total[d];
   }
 }
 
@@ -766,19 +778,21 @@ __global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLa
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
     for (int k = k0; k < k1; ++k) {
-      const unsigned *begin = o.begin + size_t(k) * (o.rows + 1) + v;
+      const unsigned *begin = o.vec_begin + size_t(k) * (o.rows + 1) + v;
       const long long bag0 = (long long)k * kBlockBags;
-      const unsigned p1 = begin[1];
-      constexpr int K = 8;
-      for (unsigned p = begin[0]; p < p1; p += K) {
-        Vec<T, VEC> x[K];
+      const unsigned end = begin[1];
+      for (unsigned w = begin[0]; w < end; ++w) {
+        const uint4 ids = reinterpret_cast<const uint4 *>(o.local)[w];
+        const unsigned word[4] = {ids.x, ids.y, ids.z, ids.w};
+        Vec<T, VEC> x[8];
 #pragma unroll
-        for (int i = 0; i < K; ++i) {
+        for (int i = 0; i < 8; ++i) {
+          const unsigned id = i % 2 ? word[i / 2] >> 16 : word[i / 2] & 0xFFFFu;
           x[i].clear();
-          if (p + i < p1) x[i].load(grad + (bag0 + o.local[p + i] / 4) * a.grad_stride);
+          if (id != kNoBag) x[i].load(grad + (bag0 + id / 4) * a.grad_stride);
         }
 #pragma unroll
-        for (int i = 0; i < K; ++i) x[i].add_to(sum);
+        for (int i = 0; i < 8; ++i) x[i].add_to(sum);
       }
     }
     float *out = partial + ((size_t(blockIdx.z) * o.rows + v) * vecs + c) * VEC;
@@ -1127,10 +1141,10 @@ TokenOrder::TokenOrder(void *mem, int64_t bags_, int64_t per_bag, int64_t rows_)
     return static_cast<void *>(q);
   };
   counts = static_cast<unsigned *>(take(256));
-  bag = nullptr, local = nullptr, begin = nullptr, frequent = item = nullptr, named = nullptr;
+  bag = nullptr, local = nullptr, vec_begin = nullptr, frequent = item = nullptr, named = nullptr;
   if (blocks > 1) {
-    begin = static_cast<unsigned *>(take(size_t(blocks) * size_t(rows + 1) * 4));
-    local = static_cast<unsigned short *>(take(size_t(count) * 2));
+    vec_begin = static_cast<unsigned *>(take(size_t(segments() + 1) * 4));
+    local = static_cast<unsigned short *>(take(size_t(most_vectors()) * 16));
   } else {
     named = static_cast<unsigned char *>(take(size_t(rows)));
     bag = static_cast<unsigned *>(take(size_t(count) * 4));
@@ -1140,8 +1154,14 @@ TokenOrder::TokenOrder(void *mem, int64_t bags_, int64_t per_bag, int64_t rows_)
   bytes = at;
 }
 
-size_t token_order_scratch(int64_t count) {
-  return count <= kMostClusterTokens ? 0 : SortScratch(nullptr, count).bytes;
+namespace {
+int vec_tiles(const TokenOrder &o) { return int((o.segments() + 1 + kVecTile - 1) / kVecTile); }
+}  // namespace
+
+size_t token_order_scratch(const TokenOrder &o) {
+  if (o.count <= kMostClusterTokens) return 0;
+  const size_t vectors = o.blocks > 1 ? pad256(size_t(o.segments() + 1) * 4) + pad256(size_t(vec_tiles(o)) * 4) : 0;
+  return SortScratch(nullptr, o.count).bytes + vectors;
 }
 
 namespace {
@@ -1187,7 +1207,7 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
     return;
   }
   const int64_t keys = o.blocks * (o.rows + 1) - 1;  // the largest key
-  const unsigned *sorted = nullptr;
+  const unsigned *sorted = nullptr, *sorted_bag = nullptr;
   if (n > 0) {
     const SortScratch sc(scratch, n);
     const int passes = (key_bits(keys) + kDigitBits - 1) / kDigitBits;
@@ -1202,8 +1222,7 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
       p.key_in = sc.key[(i + 1) & 1];
       p.bag_in = sc.bag[(i + 1) & 1];
       p.key_out = sc.key[i & 1];
-      p.bag_out = last ? o.bag : sc.bag[i & 1];
-      p.local_out = last ? o.local : nullptr;
+      p.bag_out = last && o.blocks == 1 ? o.bag : sc.bag[i & 1];
       sort_count_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
       sort_scan_kernel<<<kDigits, 256, 0, s>>>(p);
       sort_move_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
@@ -1211,10 +1230,18 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
       count_launch(3);
     }
     sorted = sc.key[(passes - 1) & 1];
+    sorted_bag = sc.bag[(passes - 1) & 1];
   }
   if (o.blocks > 1) {
-    order_begin_kernel<<<grid_of(n + 1, 256, 8), 256, 0, s>>>(sorted, n, keys, o.begin);
-    count_launch();
+    const SortScratch sc(scratch, n);
+    unsigned *begin = reinterpret_cast<unsigned *>(static_cast<char *>(scratch) + sc.bytes);
+    unsigned *tile = begin + pad256(size_t(o.segments() + 1) * 4) / 4;
+    order_begin_kernel<<<grid_of(n + 1, 256, 8), 256, 0, s>>>(sorted, n, o.segments(), begin);
+    vec_count_kernel<<<vec_tiles(o), 256, 0, s>>>(begin, o, tile);
+    vec_tiles_kernel<<<1, 256, 0, s>>>(tile, vec_tiles(o));
+    vec_begin_kernel<<<vec_tiles(o), 256, 0, s>>>(begin, o, tile);
+    vec_move_kernel<<<grid_of(n, 256, 8), 256, 0, s>>>(sorted, sorted_bag, begin, o);
+    count_launch(5);
   } else {
     ARB_CUDA(cudaMemsetAsync(o.counts, 0, 2 * sizeof *o.counts, s));
     if (o.rows > 0) ARB_CUDA(cudaMemsetAsync(o.named, 0, size_t(o.rows), s));
@@ -1241,7 +1268,7 @@ template <typename T, int DIM>
 void narrow_grad_with(LookupGradLaunch a, const TokenOrder &o, float *partial, cudaStream_t s) {
   static bool ready[kMaxDevices] = {};
   const int dev = current_device();
-  constexpr int smem = kBlockBags * DIM * int(sizeof(float));
+  constexpr int smem = (kBlockBags + 1) * DIM * int(sizeof(float));
   if (!ready[dev]) {
     ARB_CUDA(cudaFuncSetAttribute(narrow_grad_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ready[dev] = true;
@@ -1249,7 +1276,7 @@ void narrow_grad_with(LookupGradLaunch a, const TokenOrder &o, float *partial, c
   // shares of the table a run: a few CTAs for every place on the device, so that the last ones fill it
   const int places = device_sm_count() * (DIM == 1 ? 3 : 1);
   const int64_t shares = std::max<int64_t>(1, (4 * int64_t(places) + o.blocks - 1) / o.blocks);
-  constexpr int kStep = kNarrowThreads / kNarrowLanes;  // rows a CTA takes at a time
+  constexpr int kStep = kNarrowThreads;  // rows a CTA takes at a time
   a.rows_per_cta = int(std::max<int64_t>(kStep, ((o.rows + shares - 1) / shares + kStep - 1) / kStep * kStep));
   const dim3 grid(unsigned((o.rows + a.rows_per_cta - 1) / a.rows_per_cta), unsigned(o.blocks));
   launch_overlapped(narrow_grad_kernel<T, DIM>, grid, dim3(kNarrowThreads), smem, s, a, o, partial);

@@ -42,15 +42,19 @@ void launch_lookup(const LookupLaunch &a, cudaStream_t s);
 //
 // blocks == 1: the bags sorted by token, and the sorted positions cut into items of work.
 // blocks > 1: many bags of several tokens over few rows (the leaves of a forest).  The order is kept
-// apart for every run of kBlockBags bags: within run k the bags of row v are
-// local[begin[k * (rows + 1) + v] .. begin[k * (rows + 1) + v + 1]), numbered from the run's first one
-// in 16 bits.  The gradients of a run fit into shared memory.
-constexpr int kBlockBits = 14, kBlockBags = 1 << kBlockBits;
+// apart for every run of kBlockBags bags, whose gradients fit into shared memory.  Bags are numbered
+// from the run's first one, times four (the byte of a float), in 16 bits; within a run the bags of row v
+// are vectors of eight, vec_begin[k * (rows + 1) + v] .. vec_begin[k * (rows + 1) + v + 1], the last one
+// filled up with kNoBag: no vector holds bags of two rows, and all are 16-byte aligned.
+constexpr int kBlockBags = 16383;
+constexpr unsigned short kNoBag = kBlockBags * 4;
 struct TokenOrder {
   int64_t bags, count, rows;
   int blocks;
-  unsigned short *local;  // blocks > 1: count
-  unsigned *begin;        // blocks > 1: blocks * (rows + 1)
+  unsigned short *local;  // blocks > 1: eight a vector
+  unsigned *vec_begin;    // blocks > 1: segments() + 1
+  __host__ __device__ int64_t segments() const { return blocks * (rows + 1); }
+  int64_t most_vectors() const { return count / 8 + blocks * rows + 1; }
   unsigned *bag;          // blocks == 1, and the rest: count
   // The bags of a row are cut at multiples of `piece` (a power of two) where two of these lie inside
   // them, so an item has fewer than 2 * piece bags.
@@ -63,7 +67,7 @@ struct TokenOrder {
   size_t bytes;
   TokenOrder(void *mem, int64_t bags, int64_t per_bag, int64_t rows);
 };
-size_t token_order_scratch(int64_t count);
+size_t token_order_scratch(const TokenOrder &o);
 void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, cudaStream_t s);
 
 struct LookupGradLaunch {

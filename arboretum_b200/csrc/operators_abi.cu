@@ -143,8 +143,9 @@ const char *ATokenOrderBytes(int64_t bags, int64_t per_bag, int64_t rows, int64_
   ARB_TRY
   ARB_CHECK(order_bytes && scratch_bytes, "NULL argument");
   check_counts(bags, per_bag, rows);
-  *order_bytes = int64_t(TokenOrder(nullptr, bags, per_bag, rows).bytes);
-  *scratch_bytes = int64_t(token_order_scratch(bags * per_bag));
+  const TokenOrder o(nullptr, bags, per_bag, rows);
+  *order_bytes = int64_t(o.bytes);
+  *scratch_bytes = int64_t(token_order_scratch(o));
   ARB_CATCH
 }
 
@@ -152,11 +153,12 @@ const char *ATokenOrder(const void *tokens, int token_bytes, int64_t bags, int64
                         int64_t token_stride, int64_t rows, void *order, void *scratch, int device, void *stream) {
   ARB_TRY
   const TokenView t = check_tokens(tokens, token_bytes, bags, per_bag, bag_stride, token_stride, rows);
-  ARB_CHECK(order && (scratch || token_order_scratch(t.count()) == 0), "NULL argument");
+  const TokenOrder o(order, bags, per_bag, rows);
+  ARB_CHECK(order && (scratch || token_order_scratch(o) == 0), "NULL argument");
   check_aligned(order, 256, "order");
   check_aligned(scratch, 256, "scratch");
   DeviceScope scope(device);
-  launch_token_order(t, TokenOrder(order, bags, per_bag, rows), scratch, static_cast<cudaStream_t>(stream));
+  launch_token_order(t, o, scratch, static_cast<cudaStream_t>(stream));
   ARB_CATCH
 }
 
