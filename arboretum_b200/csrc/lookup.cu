@@ -244,9 +244,11 @@ __global__ void __launch_bounds__(kTableThreads) lookup_table_kernel(LookupLaunc
 // Least-significant-digit radix sort of (token, bag): every pass counts the digits of each tile,
 // turns the counts into positions (digit by digit, tile by tile) and moves the pairs, keeping the
 // order of equal digits.  An empty slot sorts as token `rows`, behind everything.
-constexpr int kDigitBits = 8, kDigits = 1 << kDigitBits;
-constexpr int kSortThreads = 256, kSortItems = 16, kTile = kSortThreads * kSortItems;
-constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits;
+constexpr int kSortThreads = kDigits, kSortWarps = kSortThreads / 32;  // a thread takes a digit
+// pairs of a thread: few of them give every SM a tile of a small batch, many long runs of a large one
+constexpr int kFewItems = 4, kManyItems = 16;
+constexpr int64_t kManyTokens = int64_t(1) << 20;
 
 struct SortPass {
   TokenView tokens;        // first pass: where keys come from
@@ -276,12 +278,27 @@ __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsign
   if (p.blocked) key += bag / kBlockBags * unsigned(p.rows + 1);
 }
 
+// lanes of the warp with the same digit: a ballot a bit (the match instruction takes its time with many
+// different values)
+__device__ __forceinline__ unsigned lanes_with(unsigned digit, int bits) {
+  unsigned same = 0xffffffffu;
+  for (int i = 0; i < bits; ++i) {
+    const unsigned set = __ballot_sync(0xffffffffu, digit >> i & 1u);
+    same &= digit >> i & 1u ? set : ~set;
+  }
+  return same;
+}
+
+template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
   __shared__ unsigned cnt[kDigits];
-  for (int i = threadIdx.x; i < kDigits; i += kSortThreads) cnt[i] = 0;
+  overlap_release();
+  overlap_wait();
+  cnt[threadIdx.x] = 0;
   __syncthreads();
-  const long long t0 = blockIdx.x * (long long)kTile;
-  for (int j = 0; j < kSortItems; ++j) {
+  const long long t0 = blockIdx.x * (long long)(kSortThreads * ITEMS);
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
     const long long i = t0 + j * kSortThreads + threadIdx.x;
     if (i < p.n) {
       unsigned key, bag;
@@ -290,13 +307,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < kDigits; i += kSortThreads) p.counts[size_t(i) * p.tiles + blockIdx.x] = cnt[i];
+  p.counts[size_t(threadIdx.x) * p.tiles + blockIdx.x] = cnt[threadIdx.x];
 }
 
-// exclusive sum over a CTA's 256 threads
+// exclusive sum over the threads of a CTA
 __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned *total) {
-  __shared__ unsigned warp_sum[8];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  __shared__ unsigned warp_sum[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
   unsigned x = v;
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
@@ -305,7 +322,7 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned *total)
   if (lane == 31) warp_sum[w] = x;
   __syncthreads();
   unsigned before = 0, all = 0;
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < warps; ++i) {
     if (i < w) before += warp_sum[i];
     all += warp_sum[i];
   }
@@ -316,6 +333,8 @@ __device__ __forceinline__ unsigned block_exclusive(unsigned v, unsigned *total)
 
 // one CTA a digit: its counts become exclusive sums over the tiles
 __global__ void __launch_bounds__(256) sort_scan_kernel(SortPass p) {
+  overlap_release();
+  overlap_wait();
   unsigned *row = p.counts + size_t(blockIdx.x) * p.tiles;
   unsigned run = 0;
   for (int t = 0; t < p.tiles; t += 256) {
@@ -329,53 +348,73 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(SortPass p) {
   if (threadIdx.x == 0) p.totals[blockIdx.x] = run;
 }
 
+// Pairs are put in order inside the tile first, so that what goes to one digit's place in memory leaves
+// as a run.
+template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) sort_move_kernel(SortPass p) {
-  __shared__ unsigned warp_cnt[kSortWarps][kDigits];
-  __shared__ unsigned base[kDigits];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kSortWarps * kDigits; i += kSortThreads) (&warp_cnt[0][0])[i] = 0;
+  extern __shared__ uint2 staged[];  // [kSortThreads * ITEMS]
+  __shared__ unsigned short warp_cnt[kSortWarps][kDigits];
+  __shared__ unsigned base[kDigits];          // where the tile's pairs of a digit go
+  __shared__ unsigned short first[kDigits];   // and where they begin in the tile
+  overlap_release();
+  overlap_wait();
+  constexpr int kTile = kSortThreads * ITEMS;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  for (int i = 0; i < kSortWarps; ++i) warp_cnt[i][tid] = 0;
   {
     unsigned all;
-    const unsigned before = block_exclusive(p.totals[threadIdx.x], &all);
-    base[threadIdx.x] = before + p.counts[size_t(threadIdx.x) * p.tiles + blockIdx.x];
+    const unsigned before = block_exclusive(p.totals[tid], &all);
+    base[tid] = before + p.counts[size_t(tid) * p.tiles + blockIdx.x];
   }
   __syncthreads();
-  // a warp owns kSortItems * 32 neighbouring pairs; equal digits keep their order
-  const long long w0 = blockIdx.x * (long long)kTile + w * (kSortItems * 32);
-  unsigned key[kSortItems], bag[kSortItems], rank[kSortItems];
+  // a warp owns ITEMS * 32 neighbouring pairs; equal digits keep their order
+  const long long t0 = blockIdx.x * (long long)kTile, w0 = t0 + w * (ITEMS * 32);
+  unsigned key[ITEMS], bag[ITEMS];
+  unsigned short rank[ITEMS];
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
+  for (int j = 0; j < ITEMS; ++j) {
     const long long i = w0 + j * 32 + lane;
-    const bool in = i < p.n;
-    key[j] = bag[j] = rank[j] = 0;
-    if (in) sort_pair(p, i, key[j], bag[j]);
-    const unsigned digit = in ? (key[j] >> p.shift) & (kDigits - 1) : kDigits;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
+    key[j] = 0xffffffffu, bag[j] = 0;
+    if (i < p.n) sort_pair(p, i, key[j], bag[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const bool in = w0 + j * 32 + lane < p.n;
+    const unsigned digit = (key[j] >> p.shift) & (kDigits - 1);
+    const unsigned same = lanes_with(digit, kDigitBits) & __ballot_sync(0xffffffffu, in);
     const unsigned below = __popc(same & ((1u << lane) - 1u));
-    if (in) rank[j] = warp_cnt[w][digit] + below;
+    rank[j] = (unsigned short)(warp_cnt[w][digit] + below);
     __syncwarp();
-    if (in && below == 0) warp_cnt[w][digit] += __popc(same);
+    if (in && below == 0) warp_cnt[w][digit] += (unsigned short)__popc(same);
     __syncwarp();
   }
   __syncthreads();
   {
-    unsigned run = 0;
+    unsigned run = 0, all;
+#pragma unroll
     for (int i = 0; i < kSortWarps; ++i) {
-      const unsigned c = warp_cnt[i][threadIdx.x];
-      warp_cnt[i][threadIdx.x] = run;
+      const unsigned c = warp_cnt[i][tid];
+      warp_cnt[i][tid] = (unsigned short)run;
       run += c;
     }
+    first[tid] = (unsigned short)block_exclusive(run, &all);
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < kSortItems; ++j) {
-    const long long i = w0 + j * 32 + lane;
-    if (i < p.n) {
+  for (int j = 0; j < ITEMS; ++j) {
+    if (w0 + j * 32 + lane < p.n) {
       const unsigned digit = (key[j] >> p.shift) & (kDigits - 1);
-      const unsigned to = base[digit] + warp_cnt[w][digit] + rank[j];
-      p.key_out[to] = key[j];
-      p.bag_out[to] = bag[j];
+      staged[first[digit] + warp_cnt[w][digit] + rank[j]] = make_uint2(key[j], bag[j]);
     }
+  }
+  __syncthreads();
+  const int n = int(min((long long)kTile, p.n - t0));
+  for (int i = tid; i < n; i += kSortThreads) {
+    const uint2 v = staged[i];
+    const unsigned digit = (v.x >> p.shift) & (kDigits - 1);
+    const unsigned to = base[digit] + (i - first[digit]);
+    p.key_out[to] = v.x;
+    p.bag_out[to] = v.y;
   }
 }
 
@@ -516,36 +555,56 @@ __device__ __forceinline__ size_t slot_of(unsigned q, unsigned piece) {
 struct GradLanes {
   int tx_bits, ly_bits;  // of a sum: lanes across the columns, lanes along the bags
   int zero_bits;         // lanes across the columns of an untouched row
+  int chunks;            // runs of tx * U vectors in a row
 };
 
 constexpr int kGradThreads = 256;
 
-// sum over positions p0 + slice, p0 + slice + ly, .. below p1 of the gradient rows they name
+// The vectors of one gradient row that a lane takes.
 template <typename T, int VEC, int U>
-__device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsigned *__restrict__ bag, unsigned p0, unsigned p1,
-                                         int slice, int ly, int tx, int c0, int vecs, float (&sum)[U][VEC]) {
-  constexpr int K = U > 1 ? 4 : 8;  // bags whose loads are in flight together
-  const T *grad = static_cast<const T *>(a.grad);
+struct RowPart {
+  Vec<T, VEC> v[U];
+  __device__ __forceinline__ void load(const LookupGradLaunch &a, bool in, unsigned bag, int c0, int tx, int vecs) {
+    const T *row = static_cast<const T *>(a.grad) + (long long)bag * a.grad_stride;
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      v[u].clear();
+      if (in && c0 + u * tx < vecs) v[u].load(row + (long long)(c0 + u * tx) * VEC);
+    }
+  }
+};
+
+// Sum over the sorted positions p .. end of the gradient rows they name, for a group of tx * ly lanes:
+// the group's lanes fetch as many bags at once and hand them around; slice s takes every ly-th position.
+// `id` is the bag of this lane's position of the first tx * ly, `head` the row of its slice's first
+// position, both already fetched.  For whole warps.
+template <typename T, int VEC, int U>
+__device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsigned *__restrict__ bag, unsigned p, unsigned end,
+                                         unsigned id, const RowPart<T, VEC, U> &head, int slice, int ly, int tx, int c0, int vecs,
+                                         float (&sum)[U][VEC]) {
+  constexpr int K = U > 1 ? 2 : 8;  // bags whose loads are in flight together
+  const int width = tx * ly, group0 = threadIdx.x & 31 & ~(width - 1), place = threadIdx.x & (width - 1);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[u][j] = 0.0f;
-  for (unsigned p = p0 + slice; p < p1; p += ly * K) {
-    long long row[K];
+  for (int u = 0; u < U; ++u) head.v[u].get(sum[u]);
+  for (int k_first = ly;; k_first = 0) {
+    const int n = int(min(end - p, unsigned(width)));
+    for (int k0 = k_first; __any_sync(0xffffffffu, k0 < n); k0 += ly * K) {
+      RowPart<T, VEC, U> row[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) row[k] = p + k * ly < p1 ? (long long)bag[p + k * ly] * a.grad_stride : -1;
-    Vec<T, VEC> v[K][U];
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (row[k] >= 0 && c0 + u * tx < vecs) v[k][u].load(grad + row[k] + (long long)(c0 + u * tx) * VEC);
-        else v[k][u].clear();
+      for (int k = 0; k < K; ++k) {
+        const int at = k0 + k * ly + slice;
+        const unsigned b = __shfl_sync(0xffffffffu, id, group0 + (at & (width - 1)));
+        row[k].load(a, at < n, b, c0, tx, vecs);
       }
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[k][u].add_to(sum[u]);
+        for (int u = 0; u < U; ++u) row[k].v[u].add_to(sum[u]);
+    }
+    const bool more = end - p > unsigned(width);
+    if (!__any_sync(0xffffffffu, more)) break;
+    p = more ? p + width : end;
+    id = p + place < end ? bag[p + place] : 0u;
   }
   for (int o = tx; o < tx * ly; o <<= 1)  // the slices of a group are neighbouring lanes of a warp
 #pragma unroll
@@ -582,24 +641,45 @@ __device__ __forceinline__ void write_row(const LookupGradLaunch &a, long long r
 constexpr int kZeroRows = 8;
 template <typename T, typename O, int VEC, int U>
 __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLaunch a, TokenOrder o, GradLanes sh, int vecs,
-                                                                   int chunks, unsigned item_blocks, float *partial) {
+                                                                   unsigned item_blocks, float *partial) {
   overlap_release();
   overlap_wait();
   if (blockIdx.x < item_blocks) {
     const int tx = 1 << sh.tx_bits, lane = threadIdx.x & (tx - 1);
     const int ly = 1 << sh.ly_bits, slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
     const int bits = sh.tx_bits + sh.ly_bits;
-    const unsigned groups = kGradThreads >> bits;
-    const long long items = (long long)o.counts[0] * chunks;
-    for (long long i0 = (long long)blockIdx.x * groups; i0 < items; i0 += (long long)item_blocks * groups) {
-      const long long i = i0 + (threadIdx.x >> bits);
-      // neighbouring groups take the chunks of one row
-      const long long n = chunks == 1 ? i : items >> 32 ? i / chunks : unsigned(i) / unsigned(chunks);
-      const uint4 it = i < items ? o.item[n] : make_uint4(0, 0, 0, 0);
-      const int c0 = int(i - n * chunks) * (tx * U) + lane;
+    const int chunks = sh.chunks;
+    // Neighbouring groups take the chunks of one item.  Most items are one bag, so the accesses of an item
+    // are a chain (item, bag, row) of a few hundred bytes each: they are spread over the items before it.
+    // While an item is summed, the first rows of the next one, the bags of the one after that and the place
+    // of a third are being fetched.
+    const long long units = (long long)o.counts[0] * chunks, step = (long long)item_blocks * (kGradThreads >> bits);
+    const auto item_of = [&](long long i) {
+      return i >= units ? make_uint4(0, 0, 0, 0) : o.item[chunks == 1 ? i : units >> 32 ? i / chunks : unsigned(i) / unsigned(chunks)];
+    };
+    const auto column_of = [&](long long i) {
+      return (chunks == 1 ? 0 : int(units >> 32 ? i % chunks : unsigned(i) % unsigned(chunks))) * (tx * U) + lane;
+    };
+    const int place = threadIdx.x & (tx * ly - 1), group0 = threadIdx.x & 31 & ~(tx * ly - 1);
+    const auto bag_of = [&](const uint4 &it) { return it.x + place < it.y ? o.bag[it.x + place] : 0u; };
+    const auto head_of = [&](const uint4 &it, unsigned id, int c0) {
+      RowPart<T, VEC, U> head;
+      head.load(a, it.x + slice < it.y, __shfl_sync(0xffffffffu, id, group0 + slice), c0, tx, vecs);
+      return head;
+    };
+    long long i = blockIdx.x * (long long)(kGradThreads >> bits) + (threadIdx.x >> bits);
+    uint4 it = item_of(i), it1 = item_of(i + step), it2 = item_of(i + 2 * step);
+    unsigned id = bag_of(it), id1 = bag_of(it1);
+    int c0 = column_of(i);
+    RowPart<T, VEC, U> head = head_of(it, id, c0);
+    for (; __any_sync(0xffffffffu, i < units); i += step) {
+      const uint4 it3 = item_of(i + 3 * step);
+      const unsigned id2 = bag_of(it2);
+      const int c1 = column_of(i + step);
+      const RowPart<T, VEC, U> head1 = head_of(it1, id1, c1);
       float sum[U][VEC];
-      sum_bags<T, VEC, U>(a, o.bag, it.x, it.y, slice, ly, tx, c0, vecs, sum);
-      if (i < items && slice == 0) {
+      sum_bags<T, VEC, U>(a, o.bag, it.x, it.y, id, head, slice, ly, tx, c0, vecs, sum);
+      if (i < units && slice == 0) {
         if (it.w) {
           write_row<O, VEC, U>(a, it.z, c0, tx, vecs, sum);
         } else {
@@ -612,6 +692,7 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
             }
         }
       }
+      it = it1, it1 = it2, it2 = it3, id = id1, id1 = id2, c0 = c1, head = head1;
     }
     return;
   }
@@ -689,12 +770,13 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGr
 // second-level cache, 4 bytes of a 32-byte sector each, the same sums of 128 M leaf tokens took 478 us,
 // that cache's bandwidth; a few lanes a row instead of a stream, 162 us.)
 //
-// A warp walks the vectors of 32 rows as one stream, 32 vectors at a time: a lane sums its vector's eight
+// A warp walks the vectors of up to 32 rows as one stream, 32 vectors at a time: a lane sums its vector's eight
 // values, a segmented sum over the lanes adds up the vectors of a row, and what is left of a row at the
 // end of the 32 is carried on.  Every address is known in advance, so the next vectors are on their way.
-constexpr int kNarrowThreads = 512;
+// Three CTAs an SM hold 60 warps: 110 us for 128 M tokens, against 137 with 48 of them.
+constexpr int kNarrowThreads = 640;
 template <typename T, int DIM>
-__global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradLaunch a, TokenOrder o, float *__restrict__ partial) {
+__global__ void __launch_bounds__(kNarrowThreads, DIM == 1 ? 3 : 1) narrow_grad_kernel(LookupGradLaunch a, TokenOrder o, float *__restrict__ partial) {
   extern __shared__ float grads[];  // [kBlockBags][DIM], and zeros for kNoBag
   overlap_release();
   overlap_wait();
@@ -711,10 +793,12 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradL
   const int lane = threadIdx.x & 31;
   const unsigned below = (2u << lane) - 1u;  // this lane and those before it
   const long long v_end = min((long long)o.rows, (blockIdx.x + 1ll) * a.rows_per_cta);
-  for (long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * 32; v0 < v_end; v0 += kNarrowThreads) {
+  const int span = a.rows_per_warp;  // at most 32
+  for (long long v0 = blockIdx.x * (long long)a.rows_per_cta + threadIdx.x / 32 * span; v0 < v_end; v0 += kNarrowThreads / 32 * span) {
     // lane l looks after row v0 + l: its vectors are first .. last
-    const long long v = min(v0 + lane, (long long)v_end - 1);
-    const unsigned first = begin[v], last = v0 + lane < v_end ? begin[v + 1] : first;
+    const bool mine = lane < span && v0 + lane < v_end;
+    const long long v = min(v0 + min(lane, span - 1), (long long)v_end - 1);
+    const unsigned first = begin[v], last = mine ? begin[v + 1] : first;
     const unsigned w_end = __shfl_sync(0xffffffffu, begin[v + 1], 31);
     unsigned w0 = __shfl_sync(0xffffffffu, first, 0);
     const uint4 *stream = reinterpret_cast<const uint4 *>(o.local) + lane;
@@ -753,7 +837,7 @@ __global__ void __launch_bounds__(kNarrowThreads) narrow_grad_kernel(LookupGradL
       }
       ids = next;
     }
-    if (v0 + lane < v_end)
+    if (mine)
 #pragma unroll
       for (int d = 0; d < DIM; ++d) out[(v0 + lane) * DIM + d] = total[d];
   }
@@ -831,7 +915,7 @@ __global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLa
 }
 
 // ---- the sort of a batch in one launch -------------------------------------------------------
-// Up to 131072 tokens are sorted by one cluster of at most eight CTAs: the pairs stay in shared
+// Up to 32768 tokens are sorted by one cluster of at most eight CTAs: the pairs stay in shared
 // memory, a pass exchanges digit counts and moves the pairs through distributed shared memory, and
 // the rows' first positions and the items come out of the same launch.  Bound by latency: barriers and
 // dependent accesses.  (The general sort takes three launches a pass and leaves the device to a few
@@ -840,7 +924,7 @@ namespace cg = cooperative_groups;
 constexpr int kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
 constexpr int kMostClusterBits = 9, kMostClusterDigits = 1 << kMostClusterBits;
 static_assert(kMostClusterDigits == kClusterThreads, "a thread takes a digit");
-constexpr int kMostClusterItems = 32;
+constexpr int kMostClusterItems = 8;
 
 struct ClusterSortMemory {
   unsigned short warp_cnt[kClusterWarps][kMostClusterDigits];
@@ -848,17 +932,6 @@ struct ClusterSortMemory {
   unsigned base[kMostClusterDigits];
   unsigned warp_sum[kClusterWarps];
 };
-
-// lanes of the warp with the same digit: a ballot a bit (the match instruction takes its time with many
-// different values)
-__device__ __forceinline__ unsigned lanes_with(unsigned digit, int bits) {
-  unsigned same = 0xffffffffu;
-  for (int i = 0; i < bits; ++i) {
-    const unsigned set = __ballot_sync(0xffffffffu, digit >> i & 1u);
-    same &= digit >> i & 1u ? set : ~set;
-  }
-  return same;
-}
 
 template <int ITEMS>
 __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass p, TokenOrder o, int digit_bits, int passes) {
@@ -904,7 +977,7 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
       for (int i = 0; i < kClusterWarps; ++i) c[i] = m.warp_cnt[i][tid];
 #pragma unroll
       for (int i = 0; i < kClusterWarps; ++i) {
-        m.warp_cnt[i][tid] = (unsigned short)run;  // below kSpan, at most 16384
+        m.warp_cnt[i][tid] = (unsigned short)run;  // below kSpan
         run += c[i];
       }
       m.cta_cnt[tid] = run;
@@ -971,13 +1044,32 @@ int key_bits(int64_t rows) {  // keys are 0 .. rows
   return b;
 }
 
+int64_t tiles_of(int64_t n) {
+  const int64_t tile = kSortThreads * (n < kManyTokens ? kFewItems : kManyItems);
+  return (n + tile - 1) / tile;
+}
+template <int ITEMS>
+void sort_pass(const SortPass &p, cudaStream_t s) {
+  constexpr int smem = kSortThreads * ITEMS * int(sizeof(uint2));
+  static bool ready[kMaxDevices] = {};
+  const int dev = current_device();
+  if (!ready[dev]) {
+    ARB_CUDA(cudaFuncSetAttribute(sort_move_kernel<ITEMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ready[dev] = true;
+  }
+  launch_overlapped(sort_count_kernel<ITEMS>, dim3(p.tiles), dim3(kSortThreads), 0, s, p);
+  launch_overlapped(sort_scan_kernel, dim3(kDigits), dim3(256), 0, s, p);
+  launch_overlapped(sort_move_kernel<ITEMS>, dim3(p.tiles), dim3(kSortThreads), smem, s, p);
+  count_launch(3);
+}
+
 // scratch of the sort: two buffers of pairs, the digit counts
 struct SortScratch {
   unsigned *key[2], *bag[2], *counts, *totals;
   size_t bytes;
   SortScratch(void *mem, int64_t n) {
     const size_t pair = (size_t(n) * 4 + 255) / 256 * 256;
-    const size_t tiles = size_t((n + kTile - 1) / kTile);
+    const size_t tiles = size_t(tiles_of(n));
     char *p = static_cast<char *>(mem);
     size_t at = 0;
     auto take = [&](size_t b) {
@@ -1211,7 +1303,7 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
   if (n > 0) {
     const SortScratch sc(scratch, n);
     const int passes = (key_bits(keys) + kDigitBits - 1) / kDigitBits;
-    p.tiles = int((n + kTile - 1) / kTile);
+    p.tiles = int(tiles_of(n));
     p.counts = sc.counts;
     p.totals = sc.totals;
     p.blocked = o.blocks > 1;
@@ -1223,11 +1315,8 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
       p.bag_in = sc.bag[(i + 1) & 1];
       p.key_out = sc.key[i & 1];
       p.bag_out = last && o.blocks == 1 ? o.bag : sc.bag[i & 1];
-      sort_count_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
-      sort_scan_kernel<<<kDigits, 256, 0, s>>>(p);
-      sort_move_kernel<<<p.tiles, kSortThreads, 0, s>>>(p);
-      ARB_CUDA(cudaGetLastError());
-      count_launch(3);
+      if (n < kManyTokens) sort_pass<kFewItems>(p, s);
+      else sort_pass<kManyItems>(p, s);
     }
     sorted = sc.key[(passes - 1) & 1];
     sorted_bag = sc.bag[(passes - 1) & 1];
@@ -1273,11 +1362,16 @@ void narrow_grad_with(LookupGradLaunch a, const TokenOrder &o, float *partial, c
     ARB_CUDA(cudaFuncSetAttribute(narrow_grad_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ready[dev] = true;
   }
-  // shares of the table a run: a few CTAs for every place on the device, so that the last ones fill it
-  const int places = device_sm_count() * (DIM == 1 ? 3 : 1);
-  const int64_t shares = std::max<int64_t>(1, (4 * int64_t(places) + o.blocks - 1) / o.blocks);
-  constexpr int kStep = kNarrowThreads;  // rows a CTA takes at a time
-  a.rows_per_cta = int(std::max<int64_t>(kStep, ((o.rows + shares - 1) / shares + kStep - 1) / kStep * kStep));
+  // shares of the table a run: a few CTAs for every place on the device, so that the last ones fill it;
+  // with few rows the warps take fewer of them at a time
+  const int64_t places = device_sm_count() * (DIM == 1 ? 3 : 1);
+  const int64_t shares = std::max<int64_t>(1, (4 * places + o.blocks - 1) / o.blocks);
+  constexpr int kWarps = kNarrowThreads / 32;
+  a.rows_per_warp = 32;
+  while (a.rows_per_warp > 2 && o.blocks * ((o.rows + kWarps * a.rows_per_warp - 1) / (kWarps * a.rows_per_warp)) < 2 * places)
+    a.rows_per_warp /= 2;
+  const int64_t step = kWarps * a.rows_per_warp;  // rows a CTA takes at a time
+  a.rows_per_cta = int(std::max<int64_t>(step, ((o.rows + shares - 1) / shares + step - 1) / step * step));
   const dim3 grid(unsigned((o.rows + a.rows_per_cta - 1) / a.rows_per_cta), unsigned(o.blocks));
   launch_overlapped(narrow_grad_kernel<T, DIM>, grid, dim3(kNarrowThreads), smem, s, a, o, partial);
 }
@@ -1326,14 +1420,14 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   sh.ly_bits = 0;
   while (sh.tx_bits + sh.ly_bits < 5 && (int64_t(1) << sh.ly_bits) < length) ++sh.ly_bits;
   sh.zero_bits = std::min(8, log2_floor(std::max(1, vecs * 2 - 1)));
-  const int chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
+  sh.chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
   const int64_t groups = kGradThreads >> (sh.tx_bits + sh.ly_bits);
-  const int64_t item_blocks = std::min<int64_t>((o.most_items() * chunks + groups - 1) / groups, int64_t(device_sm_count()) * 64);
+  const int64_t item_blocks = std::min<int64_t>((o.most_items() * sh.chunks + groups - 1) / groups, int64_t(device_sm_count()) * 4);
   const int64_t zero_groups = kGradThreads >> sh.zero_bits;
   const int64_t zero_blocks = a.accumulate ? 0 : (o.rows + zero_groups * kZeroRows - 1) / (zero_groups * kZeroRows);
   if (item_blocks + zero_blocks == 0) return;
   launch_overlapped(lookup_grad_kernel<T, O, VEC, U>, dim3(unsigned(item_blocks + zero_blocks)), dim3(kGradThreads), 0, s,
-                    a, o, sh, vecs, chunks, unsigned(item_blocks), partial);
+                    a, o, sh, vecs, unsigned(item_blocks), partial);
   if (o.count > o.piece) {
     const int join_chunks = (vecs + 31) / 32;
     const dim3 join(unsigned(std::min<int64_t>(o.count / o.piece, device_sm_count() * 2)), unsigned(std::min(join_chunks, 65535)));
@@ -1347,7 +1441,7 @@ template <typename T, typename O, int VEC>
 void lookup_grad_vec(const LookupGradLaunch &a, const TokenOrder &o, float *partial, cudaStream_t s) {
   ARB_CHECK(a.dim / VEC <= (int64_t(1) << 30), "rows of more than 2^30 vectors");
   // a wide row gives every lane several vectors: more bytes in flight for one look at the row's bags
-  if (VEC > 1 && a.dim / VEC >= 128) lookup_grad_with<T, O, VEC, VEC == 1 ? 1 : 4>(a, o, partial, s);
+  if (VEC > 1 && a.dim / VEC >= 128) lookup_grad_with<T, O, VEC, VEC == 1 ? 1 : 2>(a, o, partial, s);
   else lookup_grad_with<T, O, VEC, 1>(a, o, partial, s);
 }
 

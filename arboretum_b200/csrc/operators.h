@@ -79,7 +79,7 @@ struct LookupGradLaunch {
   int out_type;
   int64_t out_stride;
   bool accumulate;
-  int rows_per_cta = 0;  // set by the launcher
+  int rows_per_cta = 0, rows_per_warp = 0;  // set by the launcher
 };
 size_t lookup_grad_scratch(const TokenOrder &o, int64_t dim);
 void launch_lookup_grad(const LookupGradLaunch &a, const TokenOrder &o, void *scratch, cudaStream_t s);
