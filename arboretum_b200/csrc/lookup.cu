@@ -92,7 +92,7 @@ __device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, i
 // adds the first.  With few bags the tokens of a bag are split over ly groups of lanes, which join
 // their sums through shared memory in a fixed order.
 template <typename T, typename O, int VEC, bool TOGETHER>
-__global__ void __launch_bounds__(kLookupThreads) lookup_kernel(LookupLaunch a, LaneShape sh, int vecs, int chunks) {
+__global__ void __launch_bounds__(kLookupThreads, 6) lookup_kernel(LookupLaunch a, LaneShape sh, int vecs, int chunks) {
   __shared__ float part[kLookupThreads * VEC];
   const int tx = 1 << sh.tx_bits, ly = 1 << sh.ly_bits;
   const int lane = threadIdx.x & (tx - 1), slice = (threadIdx.x >> sh.tx_bits) & (ly - 1);
@@ -494,54 +494,106 @@ __global__ void vec_move_kernel(const unsigned *__restrict__ key, const unsigned
 // The bags of a row, in pieces: a frequent token's sum is shared by many warps.  The order of the list
 // depends on the order of arrival here; no value does: where a row is cut follows from the sorted
 // positions alone, and its pieces are joined in their own order.
-// Called by whole warps; `at(i)` is the token at sorted position i, `row` that of position q.
-template <typename At>
-__device__ __forceinline__ void add_item(const TokenOrder &o, bool valid, unsigned q, unsigned row, const At &at) {
+// Called by whole warps; `at(i)` is the token at sorted position i, row[] that of the positions
+// q0 + 32 j + lane. One atomic addition a warp, whatever the number of positions.
+template <int ITEMS, typename At>
+__device__ __forceinline__ void add_items(const TokenOrder &o, long long q0, const unsigned (&row)[ITEMS], const At &at) {
   const unsigned n = unsigned(o.count), piece = o.piece;
-  const bool first = valid && (q == 0 || at(q - 1) != row);
-  // q a multiple: is it inside the row, and with it another multiple before or behind?
-  const auto cut_at = [&](unsigned p) {
-    return (p >= piece && at(p - piece) == row) || (p + piece < n && at(p + piece) == row);
+  const int lane = threadIdx.x & 31;
+  // p a multiple inside the row: is another one before or behind it in the row?
+  const auto cut_at = [&](unsigned p, unsigned r) {
+    return (p >= piece && at(p - piece) == r) || (p + piece < n && at(p + piece) == r);
   };
-  const bool item = first || (valid && (q & (piece - 1)) == 0 && cut_at(q));
-  const unsigned items = __ballot_sync(0xffffffffu, item);
-  if (items == 0) return;
-  const int lane = threadIdx.x & 31, leader = __ffs(items) - 1;
-  unsigned slot = 0;
-  if (lane == leader) slot = atomicAdd(&o.counts[0], unsigned(__popc(items)));
-  slot = __shfl_sync(0xffffffffu, slot, leader) + __popc(items & ((1u << lane) - 1u));
-  if (!item) return;
-  // first position behind q, below `most`, of another row
-  const auto end_of = [&](unsigned most) {
-    unsigned lo = q, hi = most;  // at(lo) is the row's, hi is not or is the end
-    while (hi - lo > 1) {
-      const unsigned mid = lo + (hi - lo) / 2;
-      if (at(mid) == row) lo = mid;
-      else hi = mid;
-    }
-    return hi;
-  };
-  const unsigned next = (q / piece + 1) * piece;  // the next multiple; within the row it cuts if it is one of two
-  unsigned end;
-  bool whole = first;
-  if (next < n && at(next) == row && cut_at(next)) {
-    end = next;
-    if (first) o.frequent[atomicAdd(&o.counts[1], 1u)] = make_uint4(q, end_of(n), row, 0u);
-    whole = false;
-  } else {
-    end = end_of(n - q > 2 * piece ? q + 2 * piece : n);
+  bool first[ITEMS], item[ITEMS];
+  unsigned items = 0;
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const long long ql = q0 + 32 * j + lane;
+    const unsigned q = unsigned(ql);
+    const bool valid = ql < (long long)n && (long long)row[j] < o.rows;
+    first[j] = valid && (q == 0 || at(q - 1) != row[j]);
+    item[j] = first[j] || (valid && (q & (piece - 1)) == 0 && cut_at(q, row[j]));
+    items += __popc(__ballot_sync(0xffffffffu, item[j]));
   }
-  o.item[slot] = make_uint4(q, end, row, whole ? 1u : 0u);
-  if (first) o.named[row] = 1;
+  if (items == 0) return;
+  unsigned slot = 0;
+  if (lane == 0) slot = atomicAdd(&o.counts[0], items);
+  slot = __shfl_sync(0xffffffffu, slot, 0);
+#pragma unroll
+  for (int j = 0; j < ITEMS; ++j) {
+    const unsigned same = __ballot_sync(0xffffffffu, item[j]);
+    const unsigned mine = slot + __popc(same & ((1u << lane) - 1u));
+    slot += __popc(same);
+    if (!item[j]) continue;
+    const unsigned q = unsigned(q0 + 32 * j + lane), r = row[j];
+    // first position behind q, below `most`, of another row
+    const auto end_of = [&](unsigned most) {
+      unsigned lo = q, hi = most;  // at(lo) is the row's, hi is not or is the end
+      while (hi - lo > 1) {
+        const unsigned mid = lo + (hi - lo) / 2;
+        if (at(mid) == r) lo = mid;
+        else hi = mid;
+      }
+      return hi;
+    };
+    const unsigned next = (q / piece + 1) * piece;  // the next multiple; within the row it cuts if it is one of two
+    unsigned end;
+    bool whole = first[j];
+    if (next < n && at(next) == r && cut_at(next, r)) {
+      end = next;
+      if (first[j]) o.frequent[atomicAdd(&o.counts[1], 1u)] = make_uint4(q, end_of(n), r, 0u);
+      whole = false;
+    } else if (q + 1 >= n || at(q + 1) != r) {  // most rows have one bag
+      end = q + 1;
+    } else {
+      end = end_of(n - q > 2 * piece ? q + 2 * piece : n);
+    }
+    o.item[mine] = make_uint4(q, end, r, whole ? 1u : 0u);
+    if (first[j]) o.named[r] = 1;
+  }
 }
 
 __global__ void order_items_kernel(TokenOrder o, const unsigned *__restrict__ key) {
   const long long step = (long long)gridDim.x * blockDim.x;
   for (long long q0 = blockIdx.x * (long long)blockDim.x + (threadIdx.x & ~31u); q0 < o.count; q0 += step) {
     const long long q = q0 + (threadIdx.x & 31);
-    const unsigned row = q < o.count ? key[q] : 0xffffffffu;
-    add_item(o, q < o.count && row < o.rows, unsigned(q), row, [&](unsigned i) { return key[i]; });
+    const unsigned row[1] = {q < o.count ? key[q] : 0xffffffffu};
+    add_items<1>(o, q0, row, [&](unsigned i) { return key[i]; });
   }
+}
+
+// A few tokens: one CTA, and a token's place is the number of tokens before it, counted.  (The digits'
+// passes of the cluster take 10 us whatever the number of tokens.)
+constexpr int kFewTokens = 512;
+constexpr int64_t kFewRows = 1 << 18;  // marks that the sort clears itself
+__global__ void __launch_bounds__(kFewTokens) order_few_kernel(SortPass p, TokenOrder o, bool clear) {
+  __shared__ __align__(16) unsigned key[kFewTokens];
+  __shared__ unsigned sorted[kFewTokens];
+  const int tid = threadIdx.x, n = int(p.n);
+  if (tid < 2) o.counts[tid] = 0;
+  if (clear)
+    for (long long i = tid; i < (p.rows + 15) / 16; i += blockDim.x)
+      reinterpret_cast<uint4 *>(o.named)[i] = make_uint4(0u, 0u, 0u, 0u);  // padded to 256 bytes
+  unsigned mine = 0xffffffffu, bag = 0;
+  if (tid < n) sort_pair(p, tid, mine, bag);
+  key[tid] = mine;
+  sorted[tid] = 0xffffffffu;
+  __syncthreads();
+  unsigned place = 0;
+  for (int i = 0; i < n; i += 4) {
+    const uint4 k = *reinterpret_cast<const uint4 *>(key + i);  // behind the last token: above all tokens
+    place += k.x < mine || (k.x == mine && i < tid);
+    place += k.y < mine || (k.y == mine && i + 1 < tid);
+    place += k.z < mine || (k.z == mine && i + 2 < tid);
+    place += k.w < mine || (k.w == mine && i + 3 < tid);
+  }
+  if (tid < n) {
+    sorted[place] = mine;
+    o.bag[place] = bag;
+  }
+  __syncthreads();
+  const unsigned row[1] = {sorted[tid]};
+  add_items<1>(o, tid & ~31, row, [&](unsigned i) { return sorted[i]; });
 }
 
 // Where the sum of the piece that begins at position q goes.  Of the pieces that begin within one run of
@@ -582,7 +634,7 @@ template <typename T, int VEC, int U>
 __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsigned *__restrict__ bag, unsigned p, unsigned end,
                                          unsigned id, const RowPart<T, VEC, U> &head, int slice, int ly, int tx, int c0, int vecs,
                                          float (&sum)[U][VEC]) {
-  constexpr int K = U > 1 ? 2 : 8;  // bags whose loads are in flight together
+  constexpr int K = U > 1 ? 3 : 8;  // bags whose loads are in flight together
   const int width = tx * ly, group0 = threadIdx.x & 31 & ~(width - 1), place = threadIdx.x & (width - 1);
 #pragma unroll
   for (int u = 0; u < U; ++u) head.v[u].get(sum[u]);
@@ -616,22 +668,20 @@ __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsign
 template <typename O, int VEC, int U>
 __device__ __forceinline__ void write_row(const LookupGradLaunch &a, long long row, int c0, int tx, int vecs,
                                           float (&sum)[U][VEC]) {
-  O *out = static_cast<O *>(a.out) + row * a.out_stride;
+  O *out = static_cast<O *>(a.out) + row * a.out_stride + (long long)c0 * VEC;
+  Vec<O, VEC> old[U];  // all on their way before the first is needed
+  if (a.accumulate) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * tx < vecs) old[u].load(out + (long long)(u * tx) * VEC);
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (c0 + u * tx < vecs) {
-      O *at = out + (long long)(c0 + u * tx) * VEC;
-      if (a.accumulate) {
-        float old[VEC];
-        load_vec<O, VEC>(at, old);
+    if (c0 + u * tx >= vecs) continue;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[u][j] = sum[u][j] * a.scale + old[j];
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum[u][j] *= a.scale;
-      }
-      store_vec<O, VEC>(at, sum[u]);
-    }
+    for (int j = 0; j < VEC; ++j) sum[u][j] *= a.scale;
+    if (a.accumulate) old[u].add_to(sum[u]);
+    store_vec<O, VEC>(out + (long long)(u * tx) * VEC, sum[u]);
   }
 }
 
@@ -934,7 +984,7 @@ struct ClusterSortMemory {
 };
 
 template <int ITEMS>
-__global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass p, TokenOrder o, int digit_bits, int passes) {
+__global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass p, TokenOrder o, int digit_bits, int passes, bool clear) {
   extern __shared__ __align__(16) unsigned char raw[];
   uint2 *pair = reinterpret_cast<uint2 *>(raw);
   ClusterSortMemory &m = *reinterpret_cast<ClusterSortMemory *>(raw + sizeof(uint2) * kClusterThreads * ITEMS);
@@ -953,8 +1003,9 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
     if (i < p.n) sort_pair(p, i, key[j], bag[j]);
   }
   if (rank == 0 && tid < 2) o.counts[tid] = 0;
-  for (long long i = (long long)rank * kClusterThreads + tid; i < (p.rows + 15) / 16; i += ctas * kClusterThreads)
-    reinterpret_cast<uint4 *>(o.named)[i] = make_uint4(0u, 0u, 0u, 0u);  // padded to 256 bytes
+  if (clear)
+    for (long long i = (long long)rank * kClusterThreads + tid; i < (p.rows + 15) / 16; i += ctas * kClusterThreads)
+      reinterpret_cast<uint4 *>(o.named)[i] = make_uint4(0u, 0u, 0u, 0u);  // padded to 256 bytes
   for (int pass = 0; pass < passes; ++pass) {
     const int shift = pass * digit_bits;
     for (int i = tid; i < kClusterWarps * kMostClusterDigits / 2; i += kClusterThreads)
@@ -1021,13 +1072,12 @@ __global__ void __launch_bounds__(kClusterThreads) order_cluster_kernel(SortPass
       bag[j] = v.y;
     }
   }
-  for (int j = 0; j < ITEMS; ++j) {
-    const int at = at0 + j * 32;
-    const long long q = (long long)rank * kSpan + at;
-    if (q - lane >= p.n) break;  // the same for the whole warp
-    const uint2 mine = pair[at];
-    if (q < p.n) o.bag[q] = mine.y;
-    add_item(o, q < p.n && mine.x < p.rows, unsigned(q), mine.x, [&](unsigned i) {
+  const long long q0 = (long long)rank * kSpan + w * (ITEMS * 32);
+  if (q0 < p.n) {
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j)
+      if (q0 + j * 32 + lane < p.n) o.bag[q0 + j * 32 + lane] = bag[j];
+    add_items<ITEMS>(o, q0, key, [&](unsigned i) {
       return int(i / kSpan) == rank ? pair[i % kSpan].x : cluster.map_shared_rank(pair, int(i / kSpan))[i % kSpan].x;
     });
   }
@@ -1258,7 +1308,7 @@ size_t token_order_scratch(const TokenOrder &o) {
 
 namespace {
 template <int ITEMS>
-void launch_cluster_order(const SortPass &p, const TokenOrder &o, cudaStream_t s) {
+void launch_cluster_order(const SortPass &p, const TokenOrder &o, bool clear, cudaStream_t s) {
   constexpr size_t smem = sizeof(uint2) * kClusterThreads * ITEMS + sizeof(ClusterSortMemory);
   static bool ready[kMaxDevices] = {};  // setting it twice does no harm
   const int dev = current_device();
@@ -1280,7 +1330,7 @@ void launch_cluster_order(const SortPass &p, const TokenOrder &o, cudaStream_t s
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  ARB_CUDA(cudaLaunchKernelEx(&cfg, order_cluster_kernel<ITEMS>, p, o, (bits + passes - 1) / passes, passes));
+  ARB_CUDA(cudaLaunchKernelEx(&cfg, order_cluster_kernel<ITEMS>, p, o, (bits + passes - 1) / passes, passes, clear));
   count_launch();
 }
 }  // namespace
@@ -1294,8 +1344,17 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
   p.first = true;
   p.by_slot = std::abs(t.bag_stride) < std::abs(t.token_stride);
   if (n > 0 && n <= kMostClusterTokens) {
-    if (n <= int64_t(8) * kClusterThreads * 4) launch_cluster_order<4>(p, o, s);
-    else launch_cluster_order<kMostClusterItems>(p, o, s);
+    const bool clear = o.rows <= kFewRows;  // else the marks are cleared by the whole device
+    if (!clear) ARB_CUDA(cudaMemsetAsync(o.named, 0, size_t(o.rows), s));
+    if (n <= kFewTokens) {
+      order_few_kernel<<<1, kFewTokens, 0, s>>>(p, o, clear);
+      ARB_CUDA(cudaGetLastError());
+      count_launch();
+    } else if (n <= int64_t(8) * kClusterThreads * 4) {
+      launch_cluster_order<4>(p, o, clear, s);
+    } else {
+      launch_cluster_order<kMostClusterItems>(p, o, clear, s);
+    }
     return;
   }
   const int64_t keys = o.blocks * (o.rows + 1) - 1;  // the largest key
@@ -1440,8 +1499,11 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
 template <typename T, typename O, int VEC>
 void lookup_grad_vec(const LookupGradLaunch &a, const TokenOrder &o, float *partial, cudaStream_t s) {
   ARB_CHECK(a.dim / VEC <= (int64_t(1) << 30), "rows of more than 2^30 vectors");
-  // a wide row gives every lane several vectors: more bytes in flight for one look at the row's bags
-  if (VEC > 1 && a.dim / VEC >= 128) lookup_grad_with<T, O, VEC, VEC == 1 ? 1 : 2>(a, o, partial, s);
+  // a wide row gives every lane up to 32 bytes of it: more in flight for one look at the row's bags
+  // (16384 x 4096 bf16 and 9001 x 770 fp16 tokens, sums alone: 198 and 24 us with these and three bags in
+  // flight, 207 and 30 with two vectors and two bags, 308 and 29 with four and eight: registers)
+  constexpr int kWide = std::min(4, 32 / (VEC * int(sizeof(T))));
+  if (a.dim / VEC >= 32 * kWide) lookup_grad_with<T, O, VEC, kWide>(a, o, partial, s);
   else lookup_grad_with<T, O, VEC, 1>(a, o, partial, s);
 }
 

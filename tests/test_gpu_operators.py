@@ -166,6 +166,23 @@ def test_gradient_of_frequent_tokens(bags, rows, dim, kind):
         assert torch.equal(got, arb.embedding_grad(grad.cuda(), tok.cuda()[:, 0], rows))  # no order of arrival in it
 
 
+@pytest.mark.parametrize("count", [1, 31, 512, 513, 2049, 16384, 16385, 32768, 32769, 1 << 20, (1 << 20) + 77])
+@pytest.mark.parametrize("rows", [1, 700, 1 << 18, (1 << 18) + 1])
+def test_every_sort_and_cut(count, rows):
+    """Numbers of tokens around the limits of the sorts, rows around that of the marks they clear, rows
+    cut into pieces at every place; integers, so that sums in any order are exact."""
+    gen = _rng(count, rows)
+    u = torch.rand(count, generator=gen, dtype=torch.float64)
+    for tok in (((rows + 1.0) ** u - 1).long().clamp(0, rows - 1) * 7919 % rows,  # few frequent ones
+                (torch.arange(count) // 45) % rows):                              # runs of 45
+        tok[torch.rand(count, generator=gen) < 0.05] = -1
+        grad = torch.randint(-8, 9, (count, 2), generator=gen).float()
+        want, _, _ = _plain_grad(grad, tok[:, None], rows, 1.0)
+        assert want.abs().max() < 2 ** 24
+        got = arb.embedding_grad(grad.cuda(), tok.cuda(), rows)
+        assert torch.equal(got.cpu().double(), want)
+
+
 @pytest.mark.parametrize("bags,per_bag,leaves,dim", [(1, 3, 8, 1), (1000, 50, 16, 1), (30011, 20, 256, 1), (513, 7, 64, 3), (100003, 3, 2, 2)])
 def test_forest_layout(bags, per_bag, leaves, dim):
     """Tokens tree after tree, every tree with rows of its own: lookup and gradient through the strides."""
