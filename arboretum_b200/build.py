@@ -50,8 +50,12 @@ def _bindings():
     """The Python module of the operators on torch tensors: g++ against torch's headers, linked to
     the library beside it."""
     import sysconfig
-    import torch
-    from torch.utils import cpp_extension
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError as e:
+        print("the operators on torch tensors are left out: %s" % e)
+        return
     src = os.path.join(CSRC, "bindings.cpp")
     if not _stale(BINDINGS, [src, os.path.join(HERE, "..", "include", "arboretum_b200.h")]):
         return

@@ -685,6 +685,18 @@ __device__ __forceinline__ void write_row(const LookupGradLaunch &a, long long r
   }
 }
 
+// Zeros for one row by tx lanes: 16-byte stores wherever the row begins, single ones before and behind.
+template <typename O>
+__device__ __forceinline__ void zero_row(O *row, long long dim, int lane, int tx) {
+  const long long head = min((long long)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(O)), dim);
+  const long long vecs = (dim - head) / (16 / int(sizeof(O))), tail = head + vecs * (16 / int(sizeof(O)));
+  O zero;
+  from_f32(0.0f, zero);
+  for (long long c = lane; c < head; c += tx) row[c] = zero;
+  for (long long c = lane; c < vecs; c += tx) reinterpret_cast<uint4 *>(row + head)[c] = make_uint4(0u, 0u, 0u, 0u);
+  for (long long c = tail + lane; c < dim; c += tx) row[c] = zero;
+}
+
 // CTAs below item_blocks sum the items' bags: a whole row is written at once, a piece of a frequent one
 // goes to `partial`.  The other CTAs write the zeros of the rows that no bag names, kZeroRows rows a
 // group of lanes: the marks of all of them are read at once, and the stores wait for nothing else.
@@ -703,13 +715,19 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
     // are a chain (item, bag, row) of a few hundred bytes each: they are spread over the items before it.
     // While an item is summed, the first rows of the next one, the bags of the one after that and the place
     // of a third are being fetched.
-    const long long units = (long long)o.counts[0] * chunks, step = (long long)item_blocks * (kGradThreads >> bits);
-    const auto item_of = [&](long long i) {
-      return i >= units ? make_uint4(0, 0, 0, 0) : o.item[chunks == 1 ? i : units >> 32 ? i / chunks : unsigned(i) / unsigned(chunks)];
+    const unsigned items = o.counts[0];
+    // a group's units are `groups` apart; item and chunk of the next one follow by addition
+    const unsigned groups = item_blocks * (kGradThreads >> bits), next_item = groups / chunks, next_chunk = groups % chunks;
+    struct Unit {
+      unsigned item;
+      int chunk;
     };
-    const auto column_of = [&](long long i) {
-      return (chunks == 1 ? 0 : int(units >> 32 ? i % chunks : unsigned(i) % unsigned(chunks))) * (tx * U) + lane;
+    const auto after = [&](Unit u) {
+      u.item += next_item, u.chunk += int(next_chunk);
+      if (u.chunk >= chunks) u.chunk -= chunks, ++u.item;
+      return u;
     };
+    const auto item_of = [&](const Unit &u) { return u.item < items ? o.item[u.item] : make_uint4(0, 0, 0, 0); };
     const int place = threadIdx.x & (tx * ly - 1), group0 = threadIdx.x & 31 & ~(tx * ly - 1);
     const auto bag_of = [&](const uint4 &it) { return it.x + place < it.y ? o.bag[it.x + place] : 0u; };
     const auto head_of = [&](const uint4 &it, unsigned id, int c0) {
@@ -717,19 +735,20 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
       head.load(a, it.x + slice < it.y, __shfl_sync(0xffffffffu, id, group0 + slice), c0, tx, vecs);
       return head;
     };
-    long long i = blockIdx.x * (long long)(kGradThreads >> bits) + (threadIdx.x >> bits);
-    uint4 it = item_of(i), it1 = item_of(i + step), it2 = item_of(i + 2 * step);
+    const unsigned begin = blockIdx.x * (kGradThreads >> bits) + (threadIdx.x >> bits);
+    Unit u = {begin / chunks, int(begin % chunks)}, u1 = after(u), u2 = after(u1);
+    uint4 it = item_of(u), it1 = item_of(u1), it2 = item_of(u2);
     unsigned id = bag_of(it), id1 = bag_of(it1);
-    int c0 = column_of(i);
-    RowPart<T, VEC, U> head = head_of(it, id, c0);
-    for (; __any_sync(0xffffffffu, i < units); i += step) {
-      const uint4 it3 = item_of(i + 3 * step);
+    RowPart<T, VEC, U> head = head_of(it, id, u.chunk * (tx * U) + lane);
+    while (__any_sync(0xffffffffu, u.item < items)) {
+      const Unit u3 = after(u2);
+      const uint4 it3 = item_of(u3);
       const unsigned id2 = bag_of(it2);
-      const int c1 = column_of(i + step);
-      const RowPart<T, VEC, U> head1 = head_of(it1, id1, c1);
+      const RowPart<T, VEC, U> head1 = head_of(it1, id1, u1.chunk * (tx * U) + lane);
+      const int c0 = u.chunk * (tx * U) + lane;
       float sum[U][VEC];
       sum_bags<T, VEC, U>(a, o.bag, it.x, it.y, id, head, slice, ly, tx, c0, vecs, sum);
-      if (i < units && slice == 0) {
+      if (u.item < items && slice == 0) {
         if (it.w) {
           write_row<O, VEC, U>(a, it.z, c0, tx, vecs, sum);
         } else {
@@ -742,7 +761,7 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
             }
         }
       }
-      it = it1, it1 = it2, it2 = it3, id = id1, id1 = id2, c0 = c1, head = head1;
+      u = u1, u1 = u2, u2 = u3, it = it1, it1 = it2, it2 = it3, id = id1, id1 = id2, head = head1;
     }
     return;
   }
@@ -751,64 +770,74 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
   unsigned char named[kZeroRows];
 #pragma unroll
   for (int r = 0; r < kZeroRows; ++r) named[r] = row0 + r * groups < o.rows ? o.named[row0 + r * groups] : 1;
-  float zero[VEC];
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) zero[j] = 0.0f;
+  const int lane = threadIdx.x & (tx - 1);
 #pragma unroll
   for (int r = 0; r < kZeroRows; ++r) {
     if (named[r]) continue;
     O *out = static_cast<O *>(a.out) + (row0 + r * groups) * a.out_stride;
-    for (int c = threadIdx.x & (tx - 1); c < vecs; c += tx) store_vec<O, VEC>(out + (long long)c * VEC, zero);
+    if constexpr (VEC * sizeof(O) >= 16) {  // every row begins on 16 bytes
+      constexpr int kWords = VEC * int(sizeof(O)) / 16;
+      for (int c = lane; c < vecs * kWords; c += tx) reinterpret_cast<uint4 *>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+      zero_row(out, a.dim, lane, tx);
+    }
   }
 }
 
 // The pieces of a frequent row, joined in their order: eight groups of 32 lanes take every eighth piece
-// of 32 vectors of columns, and the groups' sums are added one after another.
-template <typename O, int VEC>
+// of a run of columns, and the groups' sums are added one after another.
+template <typename O, int VEC, int U>
 __global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGradLaunch a, TokenOrder o, int vecs, int chunks,
                                                                         const float *__restrict__ partial) {
-  __shared__ float part[kGradThreads * VEC];
+  __shared__ float part[kGradThreads * VEC * U];
   constexpr int kSlices = kGradThreads / 32, K = 4;
   const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
   overlap_release();
   overlap_wait();
   const unsigned frequent = o.counts[1];
-  for (unsigned h = blockIdx.x; h < frequent; h += gridDim.x) {
+  for (unsigned h = blockIdx.x; h < frequent; h += gridDim.x)
+   for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
     const uint4 f = o.frequent[h];
     const unsigned second = (f.x / o.piece + 1) * o.piece;  // pieces: the first, then one at every multiple
     const unsigned pieces = 1 + (f.y - second + o.piece - 1) / o.piece;
-    for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
-      const int c = chunk * 32 + lane;
-      float sum[1][VEC];
+    const int c0 = chunk * (32 * U) + lane;
+    float sum[U][VEC];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[0][j] = 0.0f;
-      for (unsigned k0 = slice; k0 < pieces; k0 += kSlices * K) {
-        float v[K][VEC];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const unsigned n = k0 + k * kSlices;
-          const bool in = n < pieces && c < vecs;
-          const unsigned q = n == 0 ? f.x : second + (n - 1) * o.piece;
-          const float *at = partial + slot_of(q, o.piece) * size_t(a.dim) + (long long)c * VEC;
+      for (int j = 0; j < VEC; ++j) sum[u][j] = 0.0f;
+    for (unsigned k0 = slice; k0 < pieces; k0 += kSlices * K) {
+      float v[K][U][VEC];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) v[k][j] = in ? at[j] : 0.0f;
-        }
+      for (int k = 0; k < K; ++k) {
+        const unsigned n = k0 + k * kSlices;
+        const unsigned q = n == 0 ? f.x : second + (n - 1) * o.piece;
+        const float *at = partial + slot_of(q, o.piece) * size_t(a.dim) + (long long)c0 * VEC;
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) sum[0][j] += v[k][j];
+          for (int j = 0; j < VEC; ++j) v[k][u][j] = n < pieces && c0 + u * 32 < vecs ? at[u * 32 * VEC + j] : 0.0f;
       }
-      __syncthreads();
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) part[j * kGradThreads + threadIdx.x] = sum[0][j];
-      __syncthreads();
-      if (slice == 0 && c < vecs) {
+      for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          for (int g = 1; g < kSlices; ++g) sum[0][j] += part[j * kGradThreads + g * 32 + lane];
-        }
-        write_row<O, VEC, 1>(a, f.z, c, 0, vecs, sum);
-      }
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) sum[u][j] += v[k][u][j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) part[(u * VEC + j) * kGradThreads + threadIdx.x] = sum[u][j];
+    __syncthreads();
+    if (slice == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          for (int g = 1; g < kSlices; ++g) sum[u][j] += part[(u * VEC + j) * kGradThreads + g * 32 + lane];
+      write_row<O, VEC, U>(a, f.z, c0, 32, vecs, sum);
     }
   }
 }
@@ -1173,7 +1202,9 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   const int64_t vecs = a.dim / VEC;
   ARB_CHECK(vecs <= (int64_t(1) << 30), "rows of more than 2^30 vectors");
   const bool pooled = a.tokens.per_bag != 1;
-  const int u = !pooled && vecs >= 256 ? 4 : 1;
+  // one token a bag: 64 bytes of a wide row a lane, in vectors as wide as its alignment allows
+  constexpr int kWide = std::min(8, 64 / (VEC * int(sizeof(T))));
+  const int u = !pooled && vecs >= 32 * kWide ? kWide : 1;
   LaneShape sh;
   // lanes across the columns: enough for the row, at most half a CTA
   sh.tx_bits = std::min(7, log2_floor(std::max<int64_t>(1, (vecs + u - 1) / u * 2 - 1)));
@@ -1191,7 +1222,7 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   const dim3 grid(unsigned((a.tokens.bags + groups - 1) / groups), unsigned(std::min(chunks, 65535)));
   if (pooled && sh.tx_bits >= 3) lookup_kernel<T, O, VEC, true><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
   else if (pooled) lookup_kernel<T, O, VEC, false><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
-  else if (u == 4) lookup_rows_kernel<T, O, VEC, 4><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
+  else if (u > 1) lookup_rows_kernel<T, O, VEC, kWide><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
   else lookup_rows_kernel<T, O, VEC, 1><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
 }
 
@@ -1478,7 +1509,8 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   const int64_t length = std::min<int64_t>(o.piece, o.count / std::max<int64_t>(1, std::min(o.count, o.rows)));
   sh.ly_bits = 0;
   while (sh.tx_bits + sh.ly_bits < 5 && (int64_t(1) << sh.ly_bits) < length) ++sh.ly_bits;
-  sh.zero_bits = std::min(8, log2_floor(std::max(1, vecs * 2 - 1)));
+  const int64_t zero_words = (a.dim * int64_t(sizeof(O)) + 15) / 16;
+  sh.zero_bits = int(std::min(8, log2_floor(std::max<int64_t>(1, zero_words * 2 - 1))));
   sh.chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
   const int64_t groups = kGradThreads >> (sh.tx_bits + sh.ly_bits);
   const int64_t item_blocks = std::min<int64_t>((o.most_items() * sh.chunks + groups - 1) / groups, int64_t(device_sm_count()) * 4);
@@ -1488,10 +1520,11 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   launch_overlapped(lookup_grad_kernel<T, O, VEC, U>, dim3(unsigned(item_blocks + zero_blocks)), dim3(kGradThreads), 0, s,
                     a, o, sh, vecs, unsigned(item_blocks), partial);
   if (o.count > o.piece) {
-    const int join_chunks = (vecs + 31) / 32;
+    constexpr int kJoin = VEC < 4 ? 4 / VEC : 1;
+    const int join_chunks = (vecs + 32 * kJoin - 1) / (32 * kJoin);
     const dim3 join(unsigned(std::min<int64_t>(o.count / o.piece, device_sm_count() * 2)), unsigned(std::min(join_chunks, 65535)));
-    launch_overlapped(lookup_grad_join_kernel<O, VEC>, join, dim3(kGradThreads), 0, s, a, o, vecs, join_chunks,
-                      static_cast<const float *>(partial));
+    launch_overlapped(lookup_grad_join_kernel<O, VEC, kJoin>, join, dim3(kGradThreads), 0, s, a, o, vecs,
+                      join_chunks, static_cast<const float *>(partial));
     count_launch();
   }
 }
@@ -1502,7 +1535,7 @@ void lookup_grad_vec(const LookupGradLaunch &a, const TokenOrder &o, float *part
   // a wide row gives every lane up to 32 bytes of it: more in flight for one look at the row's bags
   // (16384 x 4096 bf16 and 9001 x 770 fp16 tokens, sums alone: 198 and 24 us with these and three bags in
   // flight, 207 and 30 with two vectors and two bags, 308 and 29 with four and eight: registers)
-  constexpr int kWide = std::min(4, 32 / (VEC * int(sizeof(T))));
+  constexpr int kWide = std::min(VEC == 1 ? 8 : 4, 32 / (VEC * int(sizeof(T))));
   if (a.dim / VEC >= 32 * kWide) lookup_grad_with<T, O, VEC, kWide>(a, o, partial, s);
   else lookup_grad_with<T, O, VEC, 1>(a, o, partial, s);
 }

@@ -281,6 +281,22 @@ def test_rows_beyond_32_bit_offsets():
     assert (table[-1] == 12).all() and not table[:-1].any()
 
 
+def test_accumulation_of_frequent_rows_and_gradients_of_one_tensor():
+    """The same index many times, added to what is there; the output of one call as the input of the next."""
+    gen = _rng(77)
+    tok = torch.randint(0, 3, (5000,), generator=gen).cuda()
+    g = torch.randint(-4, 5, (5000, 37), generator=gen).float().cuda()
+    total = torch.zeros(4, 37, device="cuda")
+    for _ in range(3):
+        arb.embedding_grad(g, tok, 4, out=total, accumulate=True)
+    want = torch.zeros(4, 37, device="cuda").index_add(0, tok, g) * 3  # integers: exact in any order
+    assert torch.equal(total, want)
+    again = arb.embedding(tok, total)
+    assert torch.equal(again, total[tok])
+    # a table of one row, a bag that names it in every slot
+    assert torch.equal(arb.embedding(torch.zeros(2, 700, dtype=torch.int32, device="cuda"), total[:1], pooled=True), (total[:1] * 700).expand(2, 37))
+
+
 def test_refusals_on_the_device():
     t, i = torch.zeros(5, 4, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
     with pytest.raises(ValueError, match="shares memory"):
@@ -443,6 +459,31 @@ def test_adamw(sizes, bits):
         for k, x in enumerate(params):
             m, v = o.moments(k)
             assert m.shape == x.shape and v.shape == x.shape and (v >= 0).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype,grad_dtype", [(F32, F32), (BF16, BF16), (F16, F32)])
+def test_adamw_at_every_alignment(bits, dtype, grad_dtype):
+    """Parameters and gradients that begin anywhere give the bits of aligned ones; what lies around them stays."""
+    n = 1000
+    gen = _rng(n, bits)
+    start = torch.randn(n, generator=gen).to(dtype).cuda()
+    grad = torch.randn(n, generator=gen).to(grad_dtype).cuda()
+    want = start.clone()
+    first = arb.AdamW([want], lr=0.1, state_bits=bits)
+    for _ in range(2):
+        first.step([grad])
+    for shift in range(1, 9):
+        store = torch.full((n + 16,), 3.0, dtype=dtype, device="cuda")
+        p = store[shift:shift + n]
+        p.copy_(start)
+        g = torch.zeros(n + 16, dtype=grad_dtype, device="cuda")[16 - shift:][:n]
+        g.copy_(grad)
+        o = arb.AdamW([p], lr=0.1, state_bits=bits)
+        for _ in range(2):
+            o.step([g])
+        assert torch.equal(p, want) and torch.equal(o.moment1.view(torch.uint8), first.moment1.view(torch.uint8))
+        assert (store[:shift] == 3).all() and (store[shift + n:] == 3).all()
 
 
 def test_adamw_dither_keeps_the_mean():
