@@ -1285,10 +1285,12 @@ void launch_lookup(const LookupLaunch &a, cudaStream_t s) {
 
 namespace {
 size_t pad256(size_t b) { return (b + 255) / 256 * 256; }
-// Bags of a piece: few tokens want short pieces, so that a frequent row is shared widely; a large
-// batch has pieces enough, and longer ones cost fewer partial sums.
-unsigned piece_of(int64_t count) {
-  unsigned p = 32;
+// Bags of a piece: few tokens want short pieces, so that a frequent row is shared widely (2340 tokens of
+// which some come 300 times: 40 us with 16, 57 with 32), but not so short that ordinary rows are cut
+// (20275 slots over 367 rows of 1392 columns: 57 with 16, 39 with 32); a large batch has pieces enough,
+// and longer ones cost fewer partial sums.
+unsigned piece_of(int64_t count, int64_t rows) {
+  unsigned p = count / 8 < rows ? 16 : 32;
   while (p < 4096 && int64_t(p) * 8192 < count) p *= 2;
   return p;
 }
@@ -1306,7 +1308,7 @@ int blocks_of(int64_t bags, int64_t per_bag, int64_t rows) {
 }  // namespace
 
 TokenOrder::TokenOrder(void *mem, int64_t bags_, int64_t per_bag, int64_t rows_)
-    : bags(bags_), count(bags_ * per_bag), rows(rows_), blocks(blocks_of(bags_, per_bag, rows_)), piece(piece_of(count)) {
+    : bags(bags_), count(bags_ * per_bag), rows(rows_), blocks(blocks_of(bags_, per_bag, rows_)), piece(piece_of(count, rows_)) {
   size_t at = 0;
   auto take = [&](size_t b) {
     char *q = static_cast<char *>(mem) + at;
@@ -1500,6 +1502,19 @@ size_t lookup_grad_scratch(const TokenOrder &o, int64_t dim) {
 
 namespace {
 
+// CTAs of the sums' kernel that the device holds at once
+template <typename T, typename O, int VEC, int U>
+int64_t resident_sums() {
+  static int ctas[kMaxDevices] = {};
+  const int dev = current_device();
+  if (!ctas[dev]) {
+    int n = 0;
+    ARB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, lookup_grad_kernel<T, O, VEC, U>, kGradThreads, 0));
+    ctas[dev] = std::max(1, n);
+  }
+  return int64_t(ctas[dev]) * device_sm_count();
+}
+
 template <typename T, typename O, int VEC, int U>
 void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *partial, cudaStream_t s) {
   const int vecs = int(a.dim / VEC);
@@ -1513,7 +1528,7 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   sh.zero_bits = int(std::min(8, log2_floor(std::max<int64_t>(1, zero_words * 2 - 1))));
   sh.chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
   const int64_t groups = kGradThreads >> (sh.tx_bits + sh.ly_bits);
-  const int64_t item_blocks = std::min<int64_t>((o.most_items() * sh.chunks + groups - 1) / groups, int64_t(device_sm_count()) * 4);
+  const int64_t item_blocks = std::min<int64_t>((o.most_items() * sh.chunks + groups - 1) / groups, resident_sums<T, O, VEC, U>());
   const int64_t zero_groups = kGradThreads >> sh.zero_bits;
   const int64_t zero_blocks = a.accumulate ? 0 : (o.rows + zero_groups * kZeroRows - 1) / (zero_groups * kZeroRows);
   if (item_blocks + zero_blocks == 0) return;
@@ -1532,10 +1547,11 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
 template <typename T, typename O, int VEC>
 void lookup_grad_vec(const LookupGradLaunch &a, const TokenOrder &o, float *partial, cudaStream_t s) {
   ARB_CHECK(a.dim / VEC <= (int64_t(1) << 30), "rows of more than 2^30 vectors");
-  // a wide row gives every lane up to 32 bytes of it: more in flight for one look at the row's bags
-  // (16384 x 4096 bf16 and 9001 x 770 fp16 tokens, sums alone: 198 and 24 us with these and three bags in
-  // flight, 207 and 30 with two vectors and two bags, 308 and 29 with four and eight: registers)
-  constexpr int kWide = std::min(VEC == 1 ? 8 : 4, 32 / (VEC * int(sizeof(T))));
+  // A wide row gives every lane up to four vectors and 32 bytes of it: more in flight for one look at the
+  // row's bags.  With three bags in flight (sums alone, us): 16384 x 4096 bf16 198, 2340 x 5301 fp32 40;
+  // two vectors and two bags 208 and -, four and eight 308 and -, eight vectors of one element 59 for the
+  // latter: past 128 registers the SM holds too few warps.
+  constexpr int kWide = std::min(4, 32 / (VEC * int(sizeof(T))));
   if (a.dim / VEC >= 32 * kWide) lookup_grad_with<T, O, VEC, kWide>(a, o, partial, s);
   else lookup_grad_with<T, O, VEC, 1>(a, o, partial, s);
 }
