@@ -24,9 +24,11 @@ namespace arb {
 
 namespace {
 
-constexpr int kMaxGrads = 2048;  // gradient pointers of one launch (kernel parameters: 16 KB)
+// Gradient addresses of one launch, kernel parameters: 16 KB of them at most, 512 bytes for few tensors.
+constexpr int kMaxGrads = 2048, kFewGrads = 64, kSomeGrads = 512;
+template <int N>
 struct GradPointers {
-  const void *at[kMaxGrads];
+  const void *at[N];
 };
 
 // 32 bits for an element, by the mixing of the boosting gradients' dither:
@@ -327,8 +329,8 @@ __device__ __forceinline__ void step_chunk(const AdamWLaunch &a, const Scalars &
 // Many small CTAs: with moments in 8 bits the step is bound by issued instructions (71 an element) and
 // wants as many warps as 40 registers allow: 128 M elements take 308 us with 12 CTAs of 128 threads an
 // SM, 354 with 5 of 256.  Moments in 32 bits are bound by memory: 64 M elements with a copy take 276 us.
-template <int BITS, bool MASTER>
-__global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 12 : 4) adamw_kernel(AdamWLaunch a, const __grid_constant__ GradPointers grads,
+template <int BITS, bool MASTER, int N>
+__global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 12 : 4) adamw_kernel(AdamWLaunch a, const __grid_constant__ GradPointers<N> grads,
                                                             int first_tensor, int first_chunk, int n_chunks, bool last) {
   __shared__ Scalars shared_scalars;
   if (threadIdx.x == 0) shared_scalars = scalars_of(a);
@@ -361,27 +363,34 @@ __global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 12 : 4) adamw_kern
 
 namespace {
 // a chunk a CTA: the chunks of a step are uneven (tensors end inside them), so the device hands them out
-template <int BITS, bool MASTER>
-void launch_with(const AdamWLaunch &a, const GradPointers &g, int first_tensor, int first_chunk, int chunks, bool last,
+template <int BITS, bool MASTER, int N>
+void launch_with(const AdamWLaunch &a, const void *const *grads, int n, int first_tensor, int first_chunk, int chunks, bool last,
                  cudaStream_t s) {
-  adamw_kernel<BITS, MASTER><<<std::max(1, chunks), kThreads<BITS>, 0, s>>>(a, g, first_tensor, first_chunk, chunks, last);
+  GradPointers<N> g;
+  std::copy(grads, grads + n, g.at);
+  adamw_kernel<BITS, MASTER, N><<<std::max(1, chunks), kThreads<BITS>, 0, s>>>(a, g, first_tensor, first_chunk, chunks, last);
   ARB_CUDA(cudaGetLastError());
   count_launch();
+}
+template <int N, typename... Args>
+void launch_variant(const AdamWLaunch &a, Args... args) {
+  if (a.bits == 8 && a.master) launch_with<8, true, N>(a, args...);
+  else if (a.bits == 8) launch_with<8, false, N>(a, args...);
+  else if (a.master) launch_with<32, true, N>(a, args...);
+  else launch_with<32, false, N>(a, args...);
 }
 }  // namespace
 
 void launch_adamw(const AdamWLaunch &a, const void *const *grads, const std::vector<int> &first_chunk,
                   int n_tensors, cudaStream_t s) {
-  GradPointers g;
   for (int t0 = 0;; t0 += kMaxGrads) {
-    const int t1 = std::min(n_tensors, t0 + kMaxGrads);
+    const int t1 = std::min(n_tensors, t0 + kMaxGrads), n = t1 - t0;
     const bool last = t1 == n_tensors;
-    std::copy(grads + t0, grads + t1, g.at);
     const int chunks = first_chunk[t1] - first_chunk[t0];
     if (chunks > 0 || last) {  // a step without elements still counts
-      const auto launch = a.bits == 8 ? (a.master ? launch_with<8, true> : launch_with<8, false>)
-                                      : (a.master ? launch_with<32, true> : launch_with<32, false>);
-      launch(a, g, t0, first_chunk[t0], chunks, last, s);
+      if (n <= kFewGrads) launch_variant<kFewGrads>(a, grads + t0, n, t0, first_chunk[t0], chunks, last, s);
+      else if (n <= kSomeGrads) launch_variant<kSomeGrads>(a, grads + t0, n, t0, first_chunk[t0], chunks, last, s);
+      else launch_variant<kMaxGrads>(a, grads + t0, n, t0, first_chunk[t0], chunks, last, s);
     }
     if (last) break;
   }

@@ -286,9 +286,11 @@ PyObject *embedding_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
 // ---- AdamW -----------------------------------------------------------------------------------
 struct Optimizer {
   std::vector<at::Tensor> params, buffers;
-  std::vector<const void *> grads;  // given at construction
-  std::vector<at::Tensor> bound;    // they
-  bool has_bound = false, bound_fp32 = false, any_grad = false;
+  std::vector<const void *> at;     // where the parameters lie
+  std::vector<const void *> grads;  // where the gradients given at construction lie (nullptr: None)
+  std::vector<at::Tensor> bound;    // they (None left out)
+  std::vector<c10::Storage> memory; // of both: stays as long as the device's table names it
+  bool has_bound = false, bound_fp32 = false;
   VoidPointer handle = nullptr;
   int device = 0;
   void *stream = nullptr;
@@ -315,13 +317,14 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     const at::Tensor &p = o.params[size_t(i)];
     at[size_t(i)] = nullptr;
     if (item == Py_None) continue;
-    TORCH_CHECK_VALUE(THPVariable_Check(item), "a gradient must be a contiguous tensor of its parameter's shape");
+    TORCH_CHECK_VALUE(THPVariable_CheckExact(item) || THPVariable_Check(item), "a gradient must be a contiguous tensor of its parameter's shape");
     const at::Tensor &g = THPVariable_Unpack(item);
-    TORCH_CHECK_VALUE(g.sizes() == p.sizes() && g.is_contiguous(), "a gradient must be a contiguous tensor of its parameter's shape");
-    TORCH_CHECK_VALUE(g.device() == p.device(), "a gradient is on ", g.device().str(), ", its parameter on ", p.device().str());
-    single = single && g.scalar_type() == at::kFloat;
-    same = same && g.scalar_type() == p.scalar_type();
-    at[size_t(i)] = g.const_data_ptr();
+    const c10::TensorImpl *gi = g.unsafeGetTensorImpl(), *pi = p.unsafeGetTensorImpl();
+    TORCH_CHECK_VALUE(gi->sizes() == pi->sizes() && gi->is_contiguous(), "a gradient must be a contiguous tensor of its parameter's shape");
+    TORCH_CHECK_VALUE(gi->device() == pi->device(), "a gradient is on ", g.device().str(), ", its parameter on ", p.device().str());
+    single = single && gi->dtype() == caffe2::TypeMeta::Make<float>();
+    same = same && gi->dtype() == pi->dtype();
+    at[size_t(i)] = gi->data();
     if (keep) keep->push_back(g);
   }
   TORCH_CHECK_TYPE(same || single, "gradients must have their parameters' types, or all be float32");
@@ -340,7 +343,8 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(params.get()); ++i) {
     const at::Tensor &p = tensor(PySequence_Fast_GET_ITEM(params.get(), i), "a parameter");
     o->params.push_back(p);
-    o->any_grad = o->any_grad || p.requires_grad();
+    o->at.push_back(p.const_data_ptr());
+    o->memory.push_back(p.storage());
     table.push_back(AAdamWParam{p.data_ptr(), p.numel(), float_type(p, "a parameter")});
   }
   AAdamWConfig config;
@@ -361,6 +365,7 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (args[3] != Py_None) {
     o->bound_fp32 = addresses(*o, args[3], o->grads, &o->bound);
     o->has_bound = true;
+    for (const at::Tensor &g : o->bound) o->memory.push_back(g.storage());
   }
   call(AAdamWCreate(table.data(), int(table.size()), &config, at[5], o->device, &o->handle));
   PyObject *capsule = PyCapsule_New(o.get(), kOptimizer, [](PyObject *c) {
@@ -383,6 +388,13 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   ARB_BEGIN
   need(n, 4);
   Optimizer &o = optimizer(args[0]);
+  // one look at every parameter: 500 of them are further apart than the first-level cache is large
+  std::vector<c10::TensorImpl *> recorded;  // autograd has to see that these changed
+  for (size_t i = 0; i < o.params.size(); ++i) {
+    c10::TensorImpl *p = o.params[i].unsafeGetTensorImpl();
+    TORCH_CHECK_VALUE(p->data() == o.at[i], "a parameter's memory has moved since the optimizer was made");
+    if (p->requires_grad()) recorded.push_back(p);
+  }
   std::vector<const void *> given;
   const std::vector<const void *> *grads = &o.grads;
   bool fp32 = o.bound_fp32;
@@ -391,6 +403,9 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     grads = &given;
   } else {
     TORCH_CHECK_VALUE(o.has_bound, "no gradients: pass grads to step() or to the constructor");
+    size_t k = 0;
+    for (const void *g : o.grads)
+      TORCH_CHECK_VALUE(g == nullptr || o.bound[k++].unsafeGetTensorImpl()->data() == g, "a gradient's memory has moved since the optimizer was made");
   }
   double lr = 0.0;
   const float *lr_device = nullptr;
@@ -401,9 +416,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (stream.stream() != o.stream)  // the optimizer's memory must not be handed out again before that stream is done with it
     for (const at::Tensor &b : o.buffers) b.record_stream(stream);
   call(AAdamWStep(o.handle, grads->data(), int(grads->size()), fp32, lr, lr_device, grad_scale, stream.stream()));
-  if (o.any_grad)  // autograd sees that they changed
-    for (const at::Tensor &p : o.params)
-      if (p.requires_grad()) p.unsafeGetTensorImpl()->bump_version();
+  for (c10::TensorImpl *p : recorded) p->bump_version();
   Py_RETURN_NONE;
   ARB_END
 }

