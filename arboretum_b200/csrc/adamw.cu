@@ -314,7 +314,7 @@ __device__ __forceinline__ void step_chunk(const AdamWLaunch &a, const Scalars &
   P *param = static_cast<P *>(t.param) + first;
   const G *grad = static_cast<const G *>(grad_at) + first;
   const long long slot = t.slot + first;
-  const int n = int(min(t.n - first, (long long)kAdamWChunk));
+  const int n = int(min(t.n - first, (long long)a.chunk));
   // a thread behind the end (n - i <= 0) loads and stores nothing, but takes part in the shuffles
   constexpr int kTileElems = kThreads<BITS> * kEach;  // elements of a CTA at a time
 #pragma unroll 1
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 12 : 4) adamw_kern
   const void *grad = ch.tensor < 0 ? nullptr : grads.at[ch.tensor - first_tensor];
   if (grad != nullptr) {
     const AdamWTensor t = a.tensors[ch.tensor];
-    const long long first = (long long)ch.index * kAdamWChunk;
+    const long long first = (long long)ch.index * a.chunk;
     if (t.type == kF32) step_chunk<BITS, float, float, MASTER>(a, c, t, grad, first);
     else if (t.type == kBF16 && a.grad_f32) step_chunk<BITS, __nv_bfloat16, float, MASTER>(a, c, t, grad, first);
     else if (t.type == kBF16) step_chunk<BITS, __nv_bfloat16, __nv_bfloat16, MASTER>(a, c, t, grad, first);

@@ -795,49 +795,50 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_join_kernel(LookupGr
   overlap_release();
   overlap_wait();
   const unsigned frequent = o.counts[1];
-  for (unsigned h = blockIdx.x; h < frequent; h += gridDim.x)
-   for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+  for (unsigned h = blockIdx.x; h < frequent; h += gridDim.x) {
     const uint4 f = o.frequent[h];
     const unsigned second = (f.x / o.piece + 1) * o.piece;  // pieces: the first, then one at every multiple
     const unsigned pieces = 1 + (f.y - second + o.piece - 1) / o.piece;
-    const int c0 = chunk * (32 * U) + lane;
-    float sum[U][VEC];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum[u][j] = 0.0f;
-    for (unsigned k0 = slice; k0 < pieces; k0 += kSlices * K) {
-      float v[K][U][VEC];
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const unsigned n = k0 + k * kSlices;
-        const unsigned q = n == 0 ? f.x : second + (n - 1) * o.piece;
-        const float *at = partial + slot_of(q, o.piece) * size_t(a.dim) + (long long)c0 * VEC;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) v[k][u][j] = n < pieces && c0 + u * 32 < vecs ? at[u * 32 * VEC + j] : 0.0f;
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) sum[u][j] += v[k][u][j];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) part[(u * VEC + j) * kGradThreads + threadIdx.x] = sum[u][j];
-    __syncthreads();
-    if (slice == 0) {
+    for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+      const int c0 = chunk * (32 * U) + lane;
+      float sum[U][VEC];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-          for (int g = 1; g < kSlices; ++g) sum[u][j] += part[(u * VEC + j) * kGradThreads + g * 32 + lane];
-      write_row<O, VEC, U>(a, f.z, c0, 32, vecs, sum);
+        for (int j = 0; j < VEC; ++j) sum[u][j] = 0.0f;
+      for (unsigned k0 = slice; k0 < pieces; k0 += kSlices * K) {
+        float v[K][U][VEC];
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const unsigned n = k0 + k * kSlices;
+          const unsigned q = n == 0 ? f.x : second + (n - 1) * o.piece;
+          const float *at = partial + slot_of(q, o.piece) * size_t(a.dim) + (long long)c0 * VEC;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[k][u][j] = n < pieces && c0 + u * 32 < vecs ? at[u * 32 * VEC + j] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) sum[u][j] += v[k][u][j];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) part[(u * VEC + j) * kGradThreads + threadIdx.x] = sum[u][j];
+      __syncthreads();
+      if (slice == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            for (int g = 1; g < kSlices; ++g) sum[u][j] += part[(u * VEC + j) * kGradThreads + g * 32 + lane];
+        write_row<O, VEC, U>(a, f.z, c0, 32, vecs, sum);
+      }
     }
   }
 }

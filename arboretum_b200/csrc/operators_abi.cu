@@ -86,16 +86,17 @@ int64_t padded(int64_t n) { return (n + kMomentBlock - 1) / kMomentBlock * kMome
 
 // where the parts of an optimizer's workspace lie
 struct AdamWLayout {
-  int64_t length = 0, chunks = 0;
+  int64_t length = 0, chunks = 0;  // chunks: room for the shortest
   size_t tensors_at, chunks_at, bytes;
   AdamWLayout(const AAdamWParam *params, int count) {
     ARB_CHECK(count >= 0 && (count == 0 || params != nullptr), "params is NULL");
     for (int i = 0; i < count; ++i) {
       ARB_CHECK(params[i].size >= 0 && params[i].size <= kMostElements, "tensor size out of range");
       length += padded(params[i].size);
-      chunks += (params[i].size + kAdamWChunk - 1) / kAdamWChunk;
-      ARB_CHECK(length <= kMostElements && chunks <= (int64_t(1) << 30), "too many elements for one optimizer");
+      ARB_CHECK(length <= kMostElements, "too many elements for one optimizer");
     }
+    for (int i = 0; i < count; ++i) chunks += (params[i].size + kLeastAdamWChunk - 1) / kLeastAdamWChunk;
+    ARB_CHECK(chunks <= (int64_t(1) << 30), "too many elements for one optimizer");
     tensors_at = 256;  // the state comes first
     chunks_at = tensors_at + (size_t(count) * sizeof(AdamWTensor) + 255) / 256 * 256;
     bytes = chunks_at + (size_t(chunks) * sizeof(AdamWChunk) + 255) / 256 * 256;
@@ -235,6 +236,7 @@ const char *AAdamWCreate(const AAdamWParam *params, int count, const AAdamWConfi
   std::vector<AdamWTensor> tensors(static_cast<size_t>(count));
   std::vector<AdamWChunk> chunks;
   chunks.reserve(size_t(l.chunks));
+  const int chunk = adamw_chunk(l.length, c.state_bits);
   int64_t slot = 0;
   for (int i = 0; i < count; ++i) {
     check_type(params[i].type);
@@ -244,7 +246,7 @@ const char *AAdamWCreate(const AAdamWParam *params, int count, const AAdamWConfi
                              reinterpret_cast<uintptr_t>(params[i].param) % 16 == 0 ? 1 : 0};
     o->first_chunk.push_back(int(chunks.size()));
     o->type.push_back(params[i].type);
-    for (int64_t k = 0; k * kAdamWChunk < params[i].size; ++k) chunks.push_back(AdamWChunk{i, int(k)});
+    for (int64_t k = 0; k * chunk < params[i].size; ++k) chunks.push_back(AdamWChunk{i, int(k)});
     slot += padded(params[i].size);
   }
   o->first_chunk.push_back(int(chunks.size()));
@@ -257,6 +259,7 @@ const char *AAdamWCreate(const AAdamWParam *params, int count, const AAdamWConfi
   a.chunks = reinterpret_cast<AdamWChunk *>(w + l.chunks_at);
   a.moment1 = c.moment1, a.moment2 = c.moment2, a.scale1 = c.scale1, a.scale2 = c.scale2, a.master = c.master;
   a.bits = c.state_bits;
+  a.chunk = chunk;
   a.beta1 = c.beta1, a.beta2 = c.beta2, a.eps = float(c.eps), a.decay = c.weight_decay;
   a.seed = c.seed;
   DeviceScope scope(device);
