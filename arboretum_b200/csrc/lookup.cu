@@ -155,6 +155,60 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunc
   }
 }
 
+// The same for 16-bit rows that begin on any two bytes (an odd number of columns): four-byte accesses all
+// the same.  A row's elements are taken as they share aligned words where they lie; where the output's
+// words pair them differently, a word's halves come from two neighbouring lanes.  10608 rows of 4545
+// bf16: 51 us, 66 with an access an element (32 at 4546).
+template <typename T>
+__device__ __forceinline__ unsigned load_pair(const T *row, long long e, long long dim) {  // elements e, e + 1; row + e on four bytes
+  if (e >= 0 && e + 1 < dim) return *reinterpret_cast<const unsigned *>(row + e);
+  unsigned lo = 0, hi = 0;
+  if (e >= 0 && e < dim) lo = *reinterpret_cast<const unsigned short *>(row + e);
+  if (e + 1 >= 0 && e + 1 < dim) hi = *reinterpret_cast<const unsigned short *>(row + e + 1);
+  return hi << 16 | lo;
+}
+template <typename T, int U>
+__global__ void __launch_bounds__(kLookupThreads) lookup_odd_rows_kernel(LookupLaunch a, int chunks) {
+  const int lane = threadIdx.x & 31;
+  const long long b = blockIdx.x * (long long)(kLookupThreads / 32) + threadIdx.x / 32;  // a warp a row
+  if (b >= a.tokens.bags) return;
+  const long long token = row_at(a.tokens, a.rows, b, 0);
+  const T *from = static_cast<const T *>(a.table) + max(token, 0ll) * a.row_stride;
+  T *out = static_cast<T *>(a.out) + b * a.out_stride;
+  const long long dim = token < 0 ? 0 : a.dim;  // an empty slot loads nothing
+  const int s = int(reinterpret_cast<uintptr_t>(from) / 2 & 1), d = int(reinterpret_cast<uintptr_t>(out) / 2 & 1);
+  for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
+    // output word w holds elements 2 w - d and the next; its first one is in the row's word w + (s && !d),
+    // the halves swapped where s and d differ
+    const long long w0 = (long long)chunk * (32 * U) + lane;
+    unsigned word[U], next = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) word[u] = load_pair(from, 2 * (w0 + u * 32) - s - (d && !s ? 2 : 0), dim);
+    if (s != d && lane == 31) next = load_pair(from, 2 * (w0 + (U - 1) * 32 + 1) - s - (d && !s ? 2 : 0), dim);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      unsigned pair = word[u];
+      if (s != d) {  // the same for the whole warp
+        const unsigned from_next = __shfl_down_sync(0xffffffffu, word[u], 1);
+        const unsigned from_first = u + 1 < U ? __shfl_sync(0xffffffffu, word[u + 1 < U ? u + 1 : u], 0) : next;
+        pair = __byte_perm(word[u], lane == 31 ? from_first : from_next, 0x5432);  // upper half, then the next one's lower
+      }
+      T e[2];
+      memcpy(e, &pair, 4);
+      from_f32(to_f32(e[0]) * a.scale, e[0]);
+      from_f32(to_f32(e[1]) * a.scale, e[1]);
+      memcpy(&pair, e, 4);
+      const long long at = 2 * (w0 + u * 32) - d;
+      if (at >= 0 && at + 1 < a.dim) {
+        *reinterpret_cast<unsigned *>(out + at) = pair;
+      } else {
+        if (at >= 0 && at < a.dim) out[at] = e[0];
+        if (at + 1 >= 0 && at + 1 < a.dim) out[at + 1] = e[1];
+      }
+    }
+  }
+}
+
 // Bags of many tokens over a narrow table that fits into shared memory (the leaf values of a forest):
 // every CTA holds the whole table and a thread the sums of two neighbouring bags, whose tokens lie
 // side by side in memory, tree after tree.  The tokens are all that is read from device memory; the
@@ -1218,6 +1272,15 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   while (pooled && sh.tx_bits + sh.ly_bits < 8 && (int64_t(4) << sh.ly_bits) < a.tokens.per_bag &&
          ((have << sh.ly_bits) < threads_wanted || (side_by_side && sh.tx_bits + sh.ly_bits < 3)))
     ++sh.ly_bits;
+  if constexpr (VEC == 1 && sizeof(T) == 2 && std::is_same<T, O>::value) {
+    if (u > 1) {  // a wide row
+      constexpr int kWords = 8;
+      const int runs = int((a.dim / 2 + 1 + 32 * kWords - 1) / (32 * kWords));
+      const dim3 grid(unsigned((a.tokens.bags + kLookupThreads / 32 - 1) / (kLookupThreads / 32)), unsigned(std::min(runs, 65535)));
+      lookup_odd_rows_kernel<T, kWords><<<grid, kLookupThreads, 0, s>>>(a, runs);
+      return;
+    }
+  }
   const int groups = kLookupThreads >> (sh.tx_bits + sh.ly_bits);
   const int chunks = int((vecs + (int64_t(u) << sh.tx_bits) - 1) / (int64_t(u) << sh.tx_bits));
   const dim3 grid(unsigned((a.tokens.bags + groups - 1) / groups), unsigned(std::min(chunks, 65535)));

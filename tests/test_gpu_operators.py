@@ -98,8 +98,8 @@ def test_lookup_shapes_and_plain_copies():
     assert arb.embedding(tok, table, out=out) is out and torch.equal(out, table[tok])
 
 
-@pytest.mark.parametrize("offset", [0, 1, 2, 4])
-@pytest.mark.parametrize("dim,pad", [(8, 0), (8, 1), (32, 8), (33, 2), (260, 4)])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("dim,pad", [(8, 0), (8, 1), (32, 8), (33, 2), (260, 4), (301, 0), (512, 1), (777, 2), (1030, 3)])
 def test_lookup_and_gradient_of_strided_and_offset_memory(dim, pad, offset):
     """Rows and starts of every alignment; what lies between the rows stays as it was."""
     gen = _rng(dim, pad, offset)
