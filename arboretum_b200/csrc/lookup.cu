@@ -666,16 +666,44 @@ struct GradLanes {
 
 constexpr int kGradThreads = 256;
 
-// The vectors of one gradient row that a lane takes.
-template <typename T, int VEC, int U>
+// The vectors of one gradient row that a lane takes.  ODD: 16-bit rows that begin on any two bytes, in
+// pairs of columns (VEC = 2) read by aligned words; where a row's words pair the columns differently, a
+// pair's halves come from two neighbouring lanes.  A warp has one row then.
+template <typename T, int VEC, int U, bool ODD>
 struct RowPart {
   Vec<T, VEC> v[U];
+  unsigned next;  // ODD: lane 31's word behind its last one
+  bool shifted;   // ODD: the row's words begin with odd columns; the same for the whole warp
   __device__ __forceinline__ void load(const LookupGradLaunch &a, bool in, unsigned bag, int c0, int tx, int vecs) {
     const T *row = static_cast<const T *>(a.grad) + (long long)bag * a.grad_stride;
+    if constexpr (ODD) {
+      shifted = reinterpret_cast<uintptr_t>(row) / 2 & 1;
+      const long long dim = in ? a.dim : 0;
+      const int s = shifted ? 1 : 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u].raw[0] = load_pair(row, 2ll * (c0 + u * 32) - s, dim);
+      next = s && (threadIdx.x & 31) == 31 ? load_pair(row, 2ll * (c0 + (U - 1) * 32 + 1) - s, dim) : 0u;
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        v[u].clear();
+        if (in && c0 + u * tx < vecs) v[u].load(row + (long long)(c0 + u * tx) * VEC);
+      }
+    }
+  }
+  // whole warps: the halves change lanes
+  __device__ __forceinline__ void add_to(float (&sum)[U][VEC]) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      v[u].clear();
-      if (in && c0 + u * tx < vecs) v[u].load(row + (long long)(c0 + u * tx) * VEC);
+      Vec<T, VEC> x = v[u];
+      if constexpr (ODD) {
+        if (shifted) {
+          const unsigned from_next = __shfl_down_sync(0xffffffffu, v[u].raw[0], 1);
+          const unsigned from_first = u + 1 < U ? __shfl_sync(0xffffffffu, v[u + 1 < U ? u + 1 : u].raw[0], 0) : next;
+          x.raw[0] = __byte_perm(v[u].raw[0], (threadIdx.x & 31) == 31 ? from_first : from_next, 0x5432);
+        }
+      }
+      x.add_to(sum[u]);
     }
   }
 };
@@ -684,18 +712,21 @@ struct RowPart {
 // the group's lanes fetch as many bags at once and hand them around; slice s takes every ly-th position.
 // `id` is the bag of this lane's position of the first tx * ly, `head` the row of its slice's first
 // position, both already fetched.  For whole warps.
-template <typename T, int VEC, int U>
+template <typename T, int VEC, int U, bool ODD>
 __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsigned *__restrict__ bag, unsigned p, unsigned end,
-                                         unsigned id, const RowPart<T, VEC, U> &head, int slice, int ly, int tx, int c0, int vecs,
+                                         unsigned id, const RowPart<T, VEC, U, ODD> &head, int slice, int ly, int tx, int c0, int vecs,
                                          float (&sum)[U][VEC]) {
   constexpr int K = U > 1 ? 3 : 8;  // bags whose loads are in flight together
   const int width = tx * ly, group0 = threadIdx.x & 31 & ~(width - 1), place = threadIdx.x & (width - 1);
 #pragma unroll
-  for (int u = 0; u < U; ++u) head.v[u].get(sum[u]);
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[u][j] = 0.0f;
+  head.add_to(sum);
   for (int k_first = ly;; k_first = 0) {
     const int n = int(min(end - p, unsigned(width)));
     for (int k0 = k_first; __any_sync(0xffffffffu, k0 < n); k0 += ly * K) {
-      RowPart<T, VEC, U> row[K];
+      RowPart<T, VEC, U, ODD> row[K];
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int at = k0 + k * ly + slice;
@@ -703,9 +734,7 @@ __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsign
         row[k].load(a, at < n, b, c0, tx, vecs);
       }
 #pragma unroll
-      for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int u = 0; u < U; ++u) row[k].v[u].add_to(sum[u]);
+      for (int k = 0; k < K; ++k) row[k].add_to(sum);
     }
     const bool more = end - p > unsigned(width);
     if (!__any_sync(0xffffffffu, more)) break;
@@ -719,9 +748,28 @@ __device__ __forceinline__ void sum_bags(const LookupGradLaunch &a, const unsign
       for (int j = 0; j < VEC; ++j) sum[u][j] += __shfl_xor_sync(0xffffffffu, sum[u][j], o);
 }
 
-template <typename O, int VEC, int U>
+template <typename O, int VEC, int U, bool ODD = false>
 __device__ __forceinline__ void write_row(const LookupGradLaunch &a, long long row, int c0, int tx, int vecs,
                                           float (&sum)[U][VEC]) {
+  if constexpr (ODD) {  // pairs of columns, written one by one: the output's rows begin anywhere
+    O *at = static_cast<O *>(a.out) + row * a.out_stride;
+    float old[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const long long c = (long long)(c0 + u * tx) * VEC + j;
+        old[u][j] = a.accumulate && c < a.dim ? to_f32(at[c]) : 0.0f;
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const long long c = (long long)(c0 + u * tx) * VEC + j;
+        if (c < a.dim) from_f32(a.accumulate ? sum[u][j] * a.scale + old[u][j] : sum[u][j] * a.scale, at[c]);
+      }
+    return;
+  }
   O *out = static_cast<O *>(a.out) + row * a.out_stride + (long long)c0 * VEC;
   Vec<O, VEC> old[U];  // all on their way before the first is needed
   if (a.accumulate) {
@@ -755,7 +803,7 @@ __device__ __forceinline__ void zero_row(O *row, long long dim, int lane, int tx
 // goes to `partial`.  The other CTAs write the zeros of the rows that no bag names, kZeroRows rows a
 // group of lanes: the marks of all of them are read at once, and the stores wait for nothing else.
 constexpr int kZeroRows = 8;
-template <typename T, typename O, int VEC, int U>
+template <typename T, typename O, int VEC, int U, bool ODD>
 __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLaunch a, TokenOrder o, GradLanes sh, int vecs,
                                                                    unsigned item_blocks, float *partial) {
   overlap_release();
@@ -785,7 +833,7 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
     const int place = threadIdx.x & (tx * ly - 1), group0 = threadIdx.x & 31 & ~(tx * ly - 1);
     const auto bag_of = [&](const uint4 &it) { return it.x + place < it.y ? o.bag[it.x + place] : 0u; };
     const auto head_of = [&](const uint4 &it, unsigned id, int c0) {
-      RowPart<T, VEC, U> head;
+      RowPart<T, VEC, U, ODD> head;
       head.load(a, it.x + slice < it.y, __shfl_sync(0xffffffffu, id, group0 + slice), c0, tx, vecs);
       return head;
     };
@@ -793,25 +841,26 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
     Unit u = {begin / chunks, int(begin % chunks)}, u1 = after(u), u2 = after(u1);
     uint4 it = item_of(u), it1 = item_of(u1), it2 = item_of(u2);
     unsigned id = bag_of(it), id1 = bag_of(it1);
-    RowPart<T, VEC, U> head = head_of(it, id, u.chunk * (tx * U) + lane);
+    RowPart<T, VEC, U, ODD> head = head_of(it, id, u.chunk * (tx * U) + lane);
     while (__any_sync(0xffffffffu, u.item < items)) {
       const Unit u3 = after(u2);
       const uint4 it3 = item_of(u3);
       const unsigned id2 = bag_of(it2);
-      const RowPart<T, VEC, U> head1 = head_of(it1, id1, u1.chunk * (tx * U) + lane);
+      const RowPart<T, VEC, U, ODD> head1 = head_of(it1, id1, u1.chunk * (tx * U) + lane);
       const int c0 = u.chunk * (tx * U) + lane;
       float sum[U][VEC];
-      sum_bags<T, VEC, U>(a, o.bag, it.x, it.y, id, head, slice, ly, tx, c0, vecs, sum);
+      sum_bags<T, VEC, U, ODD>(a, o.bag, it.x, it.y, id, head, slice, ly, tx, c0, vecs, sum);
       if (u.item < items && slice == 0) {
         if (it.w) {
-          write_row<O, VEC, U>(a, it.z, c0, tx, vecs, sum);
+          write_row<O, VEC, U, ODD>(a, it.z, c0, tx, vecs, sum);
         } else {
           float *to = partial + slot_of(it.x, o.piece) * size_t(a.dim);
 #pragma unroll
           for (int u = 0; u < U; ++u)
             if (c0 + u * tx < vecs) {
 #pragma unroll
-              for (int j = 0; j < VEC; ++j) to[(long long)(c0 + u * tx) * VEC + j] = sum[u][j];
+              for (int j = 0; j < VEC; ++j)
+                if (!ODD || (long long)(c0 + u * tx) * VEC + j < a.dim) to[(long long)(c0 + u * tx) * VEC + j] = sum[u][j];
             }
         }
       }
@@ -829,7 +878,7 @@ __global__ void __launch_bounds__(kGradThreads) lookup_grad_kernel(LookupGradLau
   for (int r = 0; r < kZeroRows; ++r) {
     if (named[r]) continue;
     O *out = static_cast<O *>(a.out) + (row0 + r * groups) * a.out_stride;
-    if constexpr (VEC * sizeof(O) >= 16) {  // every row begins on 16 bytes
+    if constexpr (!ODD && VEC * sizeof(O) >= 16) {  // every row begins on 16 bytes
       constexpr int kWords = VEC * int(sizeof(O)) / 16;
       for (int c = lane; c < vecs * kWords; c += tx) reinterpret_cast<uint4 *>(out)[c] = make_uint4(0u, 0u, 0u, 0u);
     } else {
@@ -1567,21 +1616,21 @@ size_t lookup_grad_scratch(const TokenOrder &o, int64_t dim) {
 namespace {
 
 // CTAs of the sums' kernel that the device holds at once
-template <typename T, typename O, int VEC, int U>
+template <typename T, typename O, int VEC, int U, bool ODD>
 int64_t resident_sums() {
   static int ctas[kMaxDevices] = {};
   const int dev = current_device();
   if (!ctas[dev]) {
     int n = 0;
-    ARB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, lookup_grad_kernel<T, O, VEC, U>, kGradThreads, 0));
+    ARB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, lookup_grad_kernel<T, O, VEC, U, ODD>, kGradThreads, 0));
     ctas[dev] = std::max(1, n);
   }
   return int64_t(ctas[dev]) * device_sm_count();
 }
 
-template <typename T, typename O, int VEC, int U>
+template <typename T, typename O, int VEC, int U, bool ODD = false>
 void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *partial, cudaStream_t s) {
-  const int vecs = int(a.dim / VEC);
+  const int vecs = int((a.dim + VEC - 1) / VEC);
   GradLanes sh;
   sh.tx_bits = std::min(5, log2_floor(std::max(1, (vecs + U - 1) / U * 2 - 1)));
   // a row has count / rows bags, a piece no more than `piece`: that many lanes share them
@@ -1592,17 +1641,17 @@ void lookup_grad_with(const LookupGradLaunch &a, const TokenOrder &o, float *par
   sh.zero_bits = int(std::min(8, log2_floor(std::max<int64_t>(1, zero_words * 2 - 1))));
   sh.chunks = (vecs + (U << sh.tx_bits) - 1) / (U << sh.tx_bits);
   const int64_t groups = kGradThreads >> (sh.tx_bits + sh.ly_bits);
-  const int64_t item_blocks = std::min<int64_t>((o.most_items() * sh.chunks + groups - 1) / groups, resident_sums<T, O, VEC, U>());
+  const int64_t item_blocks = std::min<int64_t>((o.most_items() * sh.chunks + groups - 1) / groups, resident_sums<T, O, VEC, U, ODD>());
   const int64_t zero_groups = kGradThreads >> sh.zero_bits;
   const int64_t zero_blocks = a.accumulate ? 0 : (o.rows + zero_groups * kZeroRows - 1) / (zero_groups * kZeroRows);
   if (item_blocks + zero_blocks == 0) return;
-  launch_overlapped(lookup_grad_kernel<T, O, VEC, U>, dim3(unsigned(item_blocks + zero_blocks)), dim3(kGradThreads), 0, s,
+  launch_overlapped(lookup_grad_kernel<T, O, VEC, U, ODD>, dim3(unsigned(item_blocks + zero_blocks)), dim3(kGradThreads), 0, s,
                     a, o, sh, vecs, unsigned(item_blocks), partial);
   if (o.count > o.piece) {
-    constexpr int kJoin = VEC < 4 ? 4 / VEC : 1;
-    const int join_chunks = (vecs + 32 * kJoin - 1) / (32 * kJoin);
+    constexpr int kWidth = ODD ? 1 : VEC, kJoin = kWidth < 4 ? 4 / kWidth : 1;
+    const int join_vecs = int(a.dim / kWidth), join_chunks = (join_vecs + 32 * kJoin - 1) / (32 * kJoin);
     const dim3 join(unsigned(std::min<int64_t>(o.count / o.piece, device_sm_count() * 2)), unsigned(std::min(join_chunks, 65535)));
-    launch_overlapped(lookup_grad_join_kernel<O, VEC, kJoin>, join, dim3(kGradThreads), 0, s, a, o, vecs,
+    launch_overlapped(lookup_grad_join_kernel<O, kWidth, kJoin>, join, dim3(kGradThreads), 0, s, a, o, join_vecs,
                       join_chunks, static_cast<const float *>(partial));
     count_launch();
   }
@@ -1616,6 +1665,12 @@ void lookup_grad_vec(const LookupGradLaunch &a, const TokenOrder &o, float *part
   // two vectors and two bags 208 and -, four and eight 308 and -, eight vectors of one element 59 for the
   // latter: past 128 registers the SM holds too few warps.
   constexpr int kWide = std::min(4, 32 / (VEC * int(sizeof(T))));
+  if constexpr (VEC == 1 && sizeof(T) == 2) {
+    if (a.dim >= 256) {  // 16-bit rows that begin anywhere: words of two columns
+      lookup_grad_with<T, O, 2, 4, true>(a, o, partial, s);
+      return;
+    }
+  }
   if (a.dim / VEC >= 32 * kWide) lookup_grad_with<T, O, VEC, kWide>(a, o, partial, s);
   else lookup_grad_with<T, O, VEC, 1>(a, o, partial, s);
 }
