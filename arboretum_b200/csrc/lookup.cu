@@ -315,6 +315,8 @@ struct SortPass {
   int tiles, shift;
   bool first, by_slot;     // by_slot: pairs are numbered slot after slot (neighbouring bags lie side by side)
   bool blocked;            // keys are (run of bags, token)
+  unsigned *clear_counts;  // first pass of an order that is not blocked: what its items count in and mark is cleared
+  unsigned char *clear_named;
 };
 
 __device__ __forceinline__ void sort_pair(const SortPass &p, long long i, unsigned &key, unsigned &bag) {
@@ -349,6 +351,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortPass p) {
   overlap_release();
   overlap_wait();
   cnt[threadIdx.x] = 0;
+  if (p.clear_named != nullptr) {
+    if (blockIdx.x == 0 && threadIdx.x < 2) p.clear_counts[threadIdx.x] = 0;
+    const long long step = (long long)gridDim.x * kSortThreads;
+    for (long long i = blockIdx.x * (long long)kSortThreads + threadIdx.x; i < (p.rows + 15) / 16; i += step)
+      reinterpret_cast<uint4 *>(p.clear_named)[i] = make_uint4(0u, 0u, 0u, 0u);  // padded to 256 bytes
+  }
   __syncthreads();
   const long long t0 = blockIdx.x * (long long)(kSortThreads * ITEMS);
 #pragma unroll
@@ -607,7 +615,9 @@ __device__ __forceinline__ void add_items(const TokenOrder &o, long long q0, con
   }
 }
 
-__global__ void order_items_kernel(TokenOrder o, const unsigned *__restrict__ key) {
+__global__ void order_items_kernel(TokenOrder o, const unsigned *key) {
+  overlap_release();
+  overlap_wait();
   const long long step = (long long)gridDim.x * blockDim.x;
   for (long long q0 = blockIdx.x * (long long)blockDim.x + (threadIdx.x & ~31u); q0 < o.count; q0 += step) {
     const long long q = q0 + (threadIdx.x & 31);
@@ -1512,9 +1522,19 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
     p.counts = sc.counts;
     p.totals = sc.totals;
     p.blocked = o.blocks > 1;
+    // The first pass clears what the items count in and mark: two launches fewer, and the items' kernel
+    // follows the sort without a gap (38933 bags of 181 rows with their gradient: 42 us, 35 so). With
+    // more than 16 rows a token its blocks would have more to clear than to sort: a fill by the whole device.
+    const bool clear = o.blocks == 1 && o.rows <= 16 * n;
+    if (o.blocks == 1 && !clear) {
+      ARB_CUDA(cudaMemsetAsync(o.counts, 0, 2 * sizeof *o.counts, s));
+      ARB_CUDA(cudaMemsetAsync(o.named, 0, size_t(o.rows), s));
+    }
     for (int i = 0; i < passes; ++i) {
       const bool last = i == passes - 1;
       p.first = i == 0;
+      p.clear_counts = i == 0 && clear ? o.counts : nullptr;
+      p.clear_named = i == 0 && clear ? o.named : nullptr;
       p.shift = i * kDigitBits;
       p.key_in = sc.key[(i + 1) & 1];
       p.bag_in = sc.bag[(i + 1) & 1];
@@ -1537,11 +1557,12 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
     vec_move_kernel<<<grid_of(n, 256, 8), 256, 0, s>>>(sorted, sorted_bag, begin, o);
     count_launch(5);
   } else {
-    ARB_CUDA(cudaMemsetAsync(o.counts, 0, 2 * sizeof *o.counts, s));
-    if (o.rows > 0) ARB_CUDA(cudaMemsetAsync(o.named, 0, size_t(o.rows), s));
     if (n > 0) {
-      order_items_kernel<<<grid_of(n, 256, 8), 256, 0, s>>>(o, sorted);
+      launch_overlapped(order_items_kernel, dim3(grid_of(n, 256, 8)), dim3(256), 0, s, o, sorted);
       count_launch();
+    } else {  // no sort has cleared them
+      ARB_CUDA(cudaMemsetAsync(o.counts, 0, 2 * sizeof *o.counts, s));
+      if (o.rows > 0) ARB_CUDA(cudaMemsetAsync(o.named, 0, size_t(o.rows), s));
     }
   }
   ARB_CUDA(cudaGetLastError());

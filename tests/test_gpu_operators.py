@@ -225,6 +225,16 @@ def test_many_bags_over_few_rows(bags, per_bag, rows, dim):
             _near(out, want + before.double(), size + before.double().abs(), count + 1, out_dtype)
 
 
+@pytest.mark.parametrize("rows", [32769 * 16, 32769 * 16 + 1, 15])
+def test_rows_without_a_bag_of_orders_one_after_the_other(rows):
+    """Orders in memory that others left behind: rows that no bag names get zeros all the same."""
+    gen = _rng(rows)
+    for i in range(3):
+        tok = torch.randint(0, rows // 3, (32769,), generator=gen) * 3 + i  # rows other than the last order's
+        got = arb.embedding_grad(torch.ones((), device="cuda").expand(32769, 3), tok.cuda(), rows)
+        assert torch.equal(got, torch.bincount(tok, minlength=rows).float().cuda()[:, None].expand(rows, 3))
+
+
 def test_gradient_of_broadcast_inputs():
     tok = torch.randint(0, 30, (6, 50), generator=_rng(5))
     row = torch.randn(40, generator=_rng(6)).cuda()
