@@ -375,7 +375,7 @@ class Garden(object):
     def refine_leaves(self, data, steps, lr=0.01, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, state_bits=32):
         """Gradient steps on the leaf values of all trees together: ``steps`` AdamW steps on the mean
         loss of ``data`` (its ``y`` or ``labels``, this model's objective).  The trees' tests stay as
-        they are; ``predict``, ``dump`` and further ``grow_tree`` calls see the new values."""
+        they are; ``predict``, ``get_y``, ``dump`` and further ``grow_tree`` calls see the new values."""
         self._ensure_init()
         _call_and_throw_if_error(_LIB.ARefineLeaves(self.handle, data.handle, int(steps), float(lr), float(betas[0]),
                                                     float(betas[1]), float(eps), float(weight_decay), int(state_bits)))

@@ -11,6 +11,7 @@
 #include "operators.h"
 
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <cmath>
 #include <cstring>
@@ -1634,7 +1635,9 @@ void BuilderView::train_yhat(Garden *g, float *out) {
 // ---------------------------------------------------------------------------
 // Garden
 // ---------------------------------------------------------------------------
-Garden::Garden(const Configuration &c) : cfg(c) {
+static std::atomic<unsigned long long> g_models{0};
+
+Garden::Garden(const Configuration &c) : cfg(c), id(++g_models) {
   // garden.cu:571-583: only these objectives exist (multi:softmax is this
   // build's completion of the reference's stub)
   if (cfg.objective != kLinearRegression && cfg.objective != kLogisticRegression &&
@@ -1878,6 +1881,7 @@ void Garden::RefineLeaves(DataMatrix *data, const Refinement &r) {
   ARB_CUDA(cudaStreamSynchronize(stream));
   for (size_t t = 0; t < T; ++t) std::copy(values(t), values(t) + leaves, trees[t].weights.begin());
   forest_trees_on_device = 0;  // the device copy of the forest holds the old values
+  ++revision;                  // and so do the predictions that matrices have accumulated
   if (builder) builder->Repredict();
 }
 
@@ -1892,8 +1896,20 @@ void Garden::UpdateByLastTree(DataMatrix *data) {
   if (!data->d_yhat.p || data->yhat_planes != K) {
     data->d_yhat.alloc(n * K * sizeof(float));
     data->yhat_planes = K;
+    data->yhat_rounds.clear();
+    data->yhat_sources.clear();
     launch_fill(data->d_yhat.as<float>(), n * K, InternalInitialY(), stream);
   }
+  ReviseY(data);
+  if (!data->SourceOf(id)) data->yhat_sources.push_back({id, revision});
+  const int first = int(trees.size()) - K;
+  AddRounds(data, {first});
+  data->yhat_rounds.push_back(first);
+}
+
+void Garden::AddRounds(DataMatrix *data, const std::vector<int> &first_trees) {
+  const int K = int(cfg.tree.labels_count);
+  const size_t n = size_t(data->rows);
   SyncForest();
   RowFeeder feed(data);
   const PackedTree pt{d_fid.as<int>(), d_thr.as<float>(), d_w.as<float>(), d_label.as<int>(),
@@ -1908,14 +1924,27 @@ void Garden::UpdateByLastTree(DataMatrix *data) {
       ARB_CUDA(cudaMemcpyAsync(d_tmp.as<float>() + size_t(k) * count,
                                data->d_yhat.as<float>() + size_t(k) * n + first, count * sizeof(float),
                                cudaMemcpyDeviceToDevice, stream));
-    launch_predict(X, count, data->cols_dense, pt, int(trees.size()) - K, K, int(cfg.tree.depth),
-                   d_tmp.as<float>(), stream, 0, feed.categories(first), data->cols_cat);
+    for (int tree : first_trees)
+      launch_predict(X, count, data->cols_dense, pt, tree, K, int(cfg.tree.depth),
+                     d_tmp.as<float>(), stream, 0, feed.categories(first), data->cols_cat);
     for (int k = 0; k < K; ++k)
       ARB_CUDA(cudaMemcpyAsync(data->d_yhat.as<float>() + size_t(k) * n + first,
                                d_tmp.as<float>() + size_t(k) * count, count * sizeof(float),
                                cudaMemcpyDeviceToDevice, stream));
     ARB_CUDA(cudaStreamSynchronize(stream));
   }
+}
+
+// The leaf values have changed since rounds were added to the matrix's accumulated prediction: the
+// same rounds are added again, in their order.
+void Garden::ReviseY(DataMatrix *data) {
+  DataMatrix::Source *source = data->SourceOf(id);
+  if (!source || source->revision == revision) return;
+  ARB_CHECK(data->yhat_sources.size() == 1,
+            "the matrix holds predictions of another model too: they cannot follow the new leaf values");
+  launch_fill(data->d_yhat.as<float>(), size_t(data->rows) * size_t(data->yhat_planes), InternalInitialY(), stream);
+  AddRounds(data, data->yhat_rounds);
+  source->revision = revision;
 }
 
 // Garden::GetY garden.cu:637-641: link-transformed accumulated prediction
@@ -1927,6 +1956,7 @@ void Garden::GetY(DataMatrix *data, std::vector<float> &out) {
     return;
   }
   EnsureStream();
+  ReviseY(data);
   out.resize(n * K);
   DevBuf d_out;
   d_out.alloc(n * K * sizeof(float));

@@ -87,6 +87,18 @@ class DataMatrix {
   // predictions accumulated by AAppendLastTree, internal scale, [K][rows]
   DevBuf d_yhat;
   int yhat_planes = 0;
+  // what they are sums of: the models that added to them, each with the leaf values it had then
+  // (Garden::id, Garden::revision), and the first tree of every round added
+  struct Source {
+    unsigned long long model, revision;
+  };
+  std::vector<Source> yhat_sources;
+  Source *SourceOf(unsigned long long model) {
+    for (Source &s : yhat_sources)
+      if (s.model == model) return &s;
+    return nullptr;
+  }
+  std::vector<int> yhat_rounds;
 
   void InitHist(int hist_size, bool missing_bin, bool verbose, cudaStream_t s, long long chunk_rows = 0,
                 const ShardInfo *shards = nullptr);
@@ -178,6 +190,8 @@ class Garden {
   void Restore(const char *json_model);
   float InternalInitialY() const;
 
+  const unsigned long long id;  // of this model, never used again in the process
+  unsigned long long revision = 0;  // counts the changes of the leaf values of trees that were there
   std::vector<Tree> trees;
   int max_fid = -1;  // largest feature id any tree tests: a matrix given to Predict must have it
   AllreduceFn allreduce = nullptr;
@@ -192,6 +206,9 @@ class Garden {
   void SyncForest();
   void EnsureStream();
   void ReleaseBuilder();
+  // adds the rounds whose first trees are given to data's accumulated predictions
+  void AddRounds(DataMatrix *data, const std::vector<int> &first_trees);
+  void ReviseY(DataMatrix *data);
   DevBuf d_fid, d_thr, d_w, d_label, d_category;
   size_t forest_trees_on_device = 0;
   cudaStream_t stream = nullptr;

@@ -841,3 +841,41 @@ def test_refinement_of_many_rows():
         o.step()
     model.refine_leaves(data, 3, lr=0.01)
     assert np.array_equal(_weights(model).astype(np.float32), table.view(T, leaves).cpu().numpy())
+
+
+@pytest.mark.parametrize("objective", [0, 3])
+def test_accumulated_predictions_follow_refined_leaves(objective):
+    """A matrix that rounds were added to gives the refined values' predictions, in the bits of predict."""
+    grown, data, X, target = _grown(objective)
+    some = lambda n: arb.DMatrix(X[:n], **{k: v[:n] for k, v in target.items()})  # noqa: E731
+    models = []
+    for _ in range(2):
+        models.append(arb.Garden(grown.config, data))
+        models[-1].labels_count = grown.labels_count
+    model, other = models
+    kept, shared = some(200), some(150)
+    for _ in range(3):
+        model.grow_tree()
+        model.append_last_tree(kept)
+    assert np.array_equal(model.get_y(kept), model.predict(kept))
+    before = model.get_y(kept)
+    model.refine_leaves(data, 3, lr=0.05)
+    assert np.array_equal(model.get_y(kept), model.predict(kept)) and not np.array_equal(model.get_y(kept), before)
+    model.grow_tree()
+    model.append_last_tree(kept)
+    model.refine_leaves(data, 2, lr=0.05)
+    model.grow_tree()
+    model.append_last_tree(kept)  # the rounds before follow here too
+    assert np.array_equal(model.get_y(kept), model.predict(kept))
+    # two models added to one matrix: what cannot follow says so, the other model's call goes on
+    other.grow_tree()
+    model.append_last_tree(shared)
+    other.append_last_tree(shared)
+    mixed = model.get_y(shared)
+    assert np.array_equal(other.get_y(shared), mixed)
+    model.refine_leaves(data, 1)
+    with pytest.raises(arb.ArboretumError, match="another model"):
+        model.get_y(shared)
+    with pytest.raises(arb.ArboretumError, match="another model"):
+        model.append_last_tree(shared)
+    assert np.array_equal(other.get_y(shared), mixed)
