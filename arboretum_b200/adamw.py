@@ -30,7 +30,7 @@ class AdamW(object):
         p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
 
     params: contiguous float32 / bfloat16 / float16 tensors of one device, of any sizes, none
-    sharing memory with another.  Arithmetic is float32; ``master=True`` keeps a float32 copy of
+    sharing memory with another.  eps: 0 or at least 2^-126.  Arithmetic is float32; ``master=True`` keeps a float32 copy of
     the parameters that the steps update, and stores it rounded in the parameters.
 
     The moments of tensor k lie at elements ``slots[k] ..`` of the flat tensors ``moment1`` and

@@ -222,6 +222,9 @@ const char *AAdamWCreate(const AAdamWParam *params, int count, const AAdamWConfi
   ARB_CHECK(c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1, "betas must be in [0, 1)");
   ARB_CHECK(c.eps >= 0 && std::isfinite(c.eps) && c.weight_decay >= 0 && std::isfinite(c.weight_decay),
             "eps and weight_decay must be finite and not negative");
+  // the kernel's reciprocal takes a divisor below float's smallest normal number for zero: a second
+  // moment of zero would give 0 / 0
+  ARB_CHECK(c.eps == 0 || float(c.eps) >= 0x1p-126f, "eps must be 0 or at least 2^-126");
   const AdamWLayout l(params, count);
   check_aligned(workspace, 256, "workspace");
   if (l.length > 0) {

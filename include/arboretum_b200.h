@@ -223,7 +223,9 @@ typedef struct {
   int type;      /* element type */
 } AAdamWParam;
 typedef struct {
-  double beta1, beta2, eps, weight_decay;
+  double beta1, beta2;  /* in [0, 1) */
+  double eps;           /* 0, or at least 2^-126 */
+  double weight_decay;
   int state_bits;
   unsigned seed;
   void *moment1, *moment2;

@@ -879,3 +879,14 @@ def test_accumulated_predictions_follow_refined_leaves(objective):
     with pytest.raises(arb.ArboretumError, match="another model"):
         model.append_last_tree(shared)
     assert np.array_equal(other.get_y(shared), mixed)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_smallest_eps_without_gradients(bits):
+    """0 / (0 + eps) is 0 for the smallest eps there is."""
+    p = torch.ones(300, device="cuda")
+    o = arb.AdamW([p], eps=2.0 ** -126, weight_decay=0.0, state_bits=bits)
+    o.step([torch.zeros(300, device="cuda")])
+    assert (p == 1).all()
+    with pytest.raises(arb.ArboretumError, match="2.-126"):
+        arb.AdamW([p], eps=1e-40)

@@ -145,3 +145,14 @@ def test_leaf_entry_points_refuse():
     assert "n_rounds" in _message(LIB.ALeafTokens(h, data.handle, -2, P))
     assert LIB.ALeafTokens(h, data.handle, -1, P) is None  # no trees: nothing to write
     assert LIB.AFreeGarden(h) is None
+
+
+@pytest.mark.parametrize("eps,refused", [(1e-40, True), (2.0 ** -127, True), (5e-324, True), (0.0, False), (2.0 ** -126, False)])
+def test_adamw_refuses_an_eps_that_the_kernel_takes_for_zero(eps, refused):
+    """Below float32's smallest normal number the step would divide zero by zero where no gradient came."""
+    from arboretum_b200.adamw import _Config, _Param
+    h = ctypes.c_void_p()
+    config = _Config(0.9, 0.99, eps, 0.0, 32, 0, 1 << 20, 1 << 20, None, None, None)
+    # an address that is no address of the workspace's alignment ends the accepted ones before the device
+    e = _message(LIB.AAdamWCreate((_Param * 1)(_Param(1 << 20, 5, 0)), 1, ctypes.byref(config), ctypes.c_void_p(16), 0, ctypes.byref(h)))
+    assert ("2^-126" in e) == refused and ("aligned" in e) != refused
