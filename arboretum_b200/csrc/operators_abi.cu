@@ -74,6 +74,9 @@ void check_out(int type, int out_type) {
   ARB_CHECK(out_type == type || out_type == kF32, "the output has the input's type or fp32");
 }
 
+// a sum of nothing is zero, and stays so
+void check_scale(double scale) { ARB_CHECK(std::isfinite(float(scale)), "scale is not finite in fp32"); }
+
 struct AdamW {
   int device = 0;
   AdamWLaunch launch;
@@ -131,6 +134,7 @@ const char *AEmbedding(const void *table, int type, int64_t rows, int64_t dim, i
   check_out(type, out_type);
   check_matrix(out, out_type, bags, dim, out_stride, "out");
   ARB_CHECK(bags < 2 || out_stride >= dim, "rows of out overlap");
+  check_scale(scale);
   a.table = table, a.type = type, a.rows = rows, a.dim = dim, a.row_stride = row_stride;
   a.scale = float(scale);
   a.out = out, a.out_type = out_type, a.out_stride = out_stride;
@@ -188,6 +192,7 @@ const char *AEmbeddingGrad(const void *grad, int type, int64_t bags, int64_t dim
   check_out(type, out_type);
   check_matrix(out, out_type, rows, dim, out_stride, "out");
   ARB_CHECK(rows < 2 || out_stride >= dim, "rows of out overlap");
+  check_scale(scale);
   ARB_CHECK(order != nullptr, "order is NULL");
   check_aligned(order, 256, "order");
   check_aligned(scratch, 256, "scratch");

@@ -24,7 +24,7 @@ __all__ = ["embedding", "embedding_grad", "token_order", "TokenOrder"]
 
 
 def embedding(tokens, table, scale=1.0, pooled=False, out=None, out_dtype=None):
-    """Rows of ``table`` named by ``tokens``, times ``scale``.
+    """Rows of ``table`` named by ``tokens``, times ``scale`` (finite).
 
     tokens: int32 or int64.  ``pooled=False``: any shape, the result has that shape and one more
     dimension; ``pooled=True``: bags x tokens with any strides, the rows of a bag are summed.

@@ -170,7 +170,7 @@ const char *ASharedAtomicPeak(int steps, double *pair_updates_per_s);
  * Element types: 0 = fp32, 1 = bf16, 2 = fp16; an output has the input's type or fp32.
  * Tokens are int32 (token_bytes 4) or int64 (8): token t of bag b is
  * tokens[b * bag_stride + t * token_stride].  A token outside [0, rows) is an empty slot: it adds
- * nothing and gets no gradient.  bags * per_bag and rows must be below 2^31 - 1. */
+ * nothing and gets no gradient.  bags * per_bag and rows must be below 2^31 - 1.  scale is finite. */
 
 /* Trees of the model (labels_count a boosting round). */
 const char *ATreeCount(VoidPointer garden, int *count);

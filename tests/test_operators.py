@@ -156,3 +156,10 @@ def test_adamw_refuses_an_eps_that_the_kernel_takes_for_zero(eps, refused):
     # an address that is no address of the workspace's alignment ends the accepted ones before the device
     e = _message(LIB.AAdamWCreate((_Param * 1)(_Param(1 << 20, 5, 0)), 1, ctypes.byref(config), ctypes.c_void_p(16), 0, ctypes.byref(h)))
     assert ("2^-126" in e) == refused and ("aligned" in e) != refused
+
+
+@pytest.mark.parametrize("scale", [float("inf"), -float("inf"), float("nan"), 1e39])
+def test_scale_is_finite(scale):
+    """Zeros of empty bags and unnamed rows would become NaN."""
+    assert "scale" in _message(_embedding(scale=scale))
+    assert "scale" in _message(LIB.AEmbeddingGrad(P, 0, 3, 4, 4, P, 1, 10, scale, P, 0, 4, 0, P, 0, None))
