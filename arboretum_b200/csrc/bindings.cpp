@@ -287,8 +287,8 @@ PyObject *embedding_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
 struct Optimizer {
   std::vector<at::Tensor> params, buffers;
   std::vector<const void *> at;     // where the parameters lie
-  std::vector<const void *> grads;  // where the gradients given at construction lie (nullptr: None)
-  std::vector<at::Tensor> bound;    // they (None left out)
+  std::vector<const void *> grads;  // where the gradients given at construction lie (nullptr: None or empty)
+  std::vector<at::Tensor> bound;    // they, one for every parameter (undefined: None)
   std::vector<c10::Storage> memory; // of both: stays as long as the device's table names it
   bool has_bound = false, bound_fp32 = false;
   VoidPointer handle = nullptr;
@@ -316,6 +316,7 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     PyObject *item = PySequence_Fast_GET_ITEM(fast.get(), i);
     const at::Tensor &p = o.params[size_t(i)];
     at[size_t(i)] = nullptr;
+    if (keep) keep->emplace_back();
     if (item == Py_None) continue;
     TORCH_CHECK_VALUE(THPVariable_CheckExact(item) || THPVariable_Check(item), "a gradient must be a contiguous tensor of its parameter's shape");
     const at::Tensor &g = THPVariable_Unpack(item);
@@ -325,7 +326,7 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     single = single && gi->dtype() == caffe2::TypeMeta::Make<float>();
     same = same && gi->dtype() == pi->dtype();
     at[size_t(i)] = gi->data();
-    if (keep) keep->push_back(g);
+    if (keep) keep->back() = g;
   }
   TORCH_CHECK_TYPE(same || single, "gradients must have their parameters' types, or all be float32");
   return !same;
@@ -365,7 +366,8 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (args[3] != Py_None) {
     o->bound_fp32 = addresses(*o, args[3], o->grads, &o->bound);
     o->has_bound = true;
-    for (const at::Tensor &g : o->bound) o->memory.push_back(g.storage());
+    for (const at::Tensor &g : o->bound)
+      if (g.defined()) o->memory.push_back(g.storage());
   }
   call(AAdamWCreate(table.data(), int(table.size()), &config, at[5], o->device, &o->handle));
   PyObject *capsule = PyCapsule_New(o.get(), kOptimizer, [](PyObject *c) {
@@ -403,9 +405,9 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     grads = &given;
   } else {
     TORCH_CHECK_VALUE(o.has_bound, "no gradients: pass grads to step() or to the constructor");
-    size_t k = 0;
-    for (const void *g : o.grads)
-      TORCH_CHECK_VALUE(g == nullptr || o.bound[k++].unsafeGetTensorImpl()->data() == g, "a gradient's memory has moved since the optimizer was made");
+    for (size_t i = 0; i < o.grads.size(); ++i)
+      TORCH_CHECK_VALUE(!o.bound[i].defined() || o.bound[i].unsafeGetTensorImpl()->data() == o.grads[i],
+                        "a gradient's memory has moved since the optimizer was made");
   }
   double lr = 0.0;
   const float *lr_device = nullptr;

@@ -890,3 +890,25 @@ def test_adamw_smallest_eps_without_gradients(bits):
     assert (p == 1).all()
     with pytest.raises(arb.ArboretumError, match="2.-126"):
         arb.AdamW([p], eps=1e-40)
+
+
+@pytest.mark.parametrize("empty", [0, 1, 2])
+def test_adamw_bound_gradients_with_an_empty_parameter(empty):
+    """Tensors of no elements take part wherever they stand, with gradients given once or every time."""
+    sizes = [300, 41]
+    sizes.insert(empty, 0)
+    make = lambda: [torch.ones(n, device="cuda") for n in sizes]  # noqa: E731
+    a, b, grads = make(), make(), make()
+    bound, given = arb.AdamW(a, grads=grads), arb.AdamW(b)
+    left_out = arb.AdamW(make(), grads=[g if len(g) != 41 else None for g in grads])
+    for _ in range(2):
+        bound.step()
+        given.step(grads)
+        left_out.step()
+    assert all(torch.equal(x, y) for x, y in zip(a, b)) and (a[sizes.index(41)] < 1).all()
+    assert bound.steps == given.steps == left_out.steps == 2
+    assert (left_out.params[sizes.index(41)] == 1).all() and torch.equal(left_out.params[sizes.index(300)], a[sizes.index(300)])
+    grads[sizes.index(41)].data = torch.ones(41, device="cuda")
+    with pytest.raises(ValueError, match="gradient's memory has moved"):
+        bound.step()
+    left_out.step()
