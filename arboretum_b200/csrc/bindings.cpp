@@ -45,9 +45,22 @@ void call(const char *message) {
   }                                                                                      \
   END_HANDLE_TH_ERRORS
 
+// elements from a tensor's first to its last, both included
+int64_t reach(const at::Tensor &t) {
+  if (t.numel() == 0) return 0;
+  int64_t n = 1;
+  for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+  return n;
+}
+
 const at::Tensor &tensor(PyObject *o, const char *name) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a torch tensor");
-  return THPVariable_Unpack(o);
+  const at::Tensor &t = THPVariable_Unpack(o);
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.has_storage(), name, " must be a tensor with memory of its own");
+  // a storage can be freed or shrunk under its tensors (untyped_storage().resize_)
+  TORCH_CHECK_VALUE((t.storage_offset() + reach(t)) * int64_t(t.element_size()) <= int64_t(t.storage().nbytes()) || t.numel() == 0, name,
+                    " lies outside its memory");
+  return t;
 }
 
 int float_type(const at::Tensor &t, const char *name) {
@@ -78,10 +91,8 @@ struct Extent {
 };
 Extent extent(const at::Tensor &t) {
   if (t.numel() == 0) return {0, 0};
-  int64_t n = 1;
-  for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
   const uintptr_t at = reinterpret_cast<uintptr_t>(t.const_data_ptr());
-  return {at, at + uintptr_t(n) * t.element_size()};
+  return {at, at + uintptr_t(reach(t)) * t.element_size()};
 }
 void apart(const at::Tensor &out, const char *name, const at::Tensor &t) {
   const Extent a = extent(out), b = extent(t);
@@ -323,6 +334,8 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     const c10::TensorImpl *gi = g.unsafeGetTensorImpl(), *pi = p.unsafeGetTensorImpl();
     TORCH_CHECK_VALUE(gi->sizes() == pi->sizes() && gi->is_contiguous(), "a gradient must be a contiguous tensor of its parameter's shape");
     TORCH_CHECK_VALUE(gi->device() == pi->device(), "a gradient is on ", g.device().str(), ", its parameter on ", p.device().str());
+    TORCH_CHECK_VALUE(gi->numel() == 0 || (gi->storage_offset() + gi->numel()) * int64_t(gi->itemsize()) <= int64_t(gi->unsafe_storage().nbytes()),
+                      "a gradient lies outside its memory");
     single = single && gi->dtype() == caffe2::TypeMeta::Make<float>();
     same = same && gi->dtype() == pi->dtype();
     at[size_t(i)] = gi->data();

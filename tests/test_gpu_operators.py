@@ -912,3 +912,24 @@ def test_adamw_bound_gradients_with_an_empty_parameter(empty):
     with pytest.raises(ValueError, match="gradient's memory has moved"):
         bound.step()
     left_out.step()
+
+
+def test_gradients_and_outputs_whose_memory_is_gone_are_refused():
+    p = torch.ones(10, device="cuda")
+    o = arb.AdamW([p])
+    whole = torch.ones(20, device="cuda")
+    parts = whole[:10], whole[10:]
+    o.step([parts[1]])
+    whole.untyped_storage().resize_(0)
+    for g in parts:
+        with pytest.raises(ValueError, match="memory"):
+            o.step([g])
+        with pytest.raises(ValueError, match="memory"):
+            arb.AdamW([torch.ones(10, device="cuda")], grads=[g])
+    assert o.steps == 1
+    out, table = torch.zeros(24, device="cuda")[12:].view(3, 4), torch.ones(3, 4, device="cuda")
+    out.untyped_storage().resize_(0)
+    i = torch.zeros(3, dtype=torch.int64, device="cuda")
+    for call in (lambda: arb.embedding(i, table, out=out), lambda: arb.embedding_grad(table, i, 3, out=out)):
+        with pytest.raises(ValueError, match="memory"):
+            call()

@@ -163,3 +163,23 @@ def test_scale_is_finite(scale):
     """Zeros of empty bags and unnamed rows would become NaN."""
     assert "scale" in _message(_embedding(scale=scale))
     assert "scale" in _message(LIB.AEmbeddingGrad(P, 0, 3, 4, 4, P, 1, 10, scale, P, 0, 4, 0, P, 0, None))
+
+
+def test_tensors_whose_memory_is_gone_are_refused():
+    """A storage can be freed or shrunk under its tensors; a view's address is then that of nothing."""
+    t = torch.zeros(5, 4)
+    i = torch.zeros(3, dtype=torch.int64)
+    for size in (0, 4 * 15):
+        base = torch.zeros(24)
+        view, last = base[4:].view(5, 4), base[12:].view(3, 4)
+        base.untyped_storage().resize_(size)
+        for call in (lambda: arb.embedding(i, view), lambda: arb.embedding_grad(last, i, 5)):
+            with pytest.raises(ValueError, match="memory"):
+                call()
+    gone = torch.zeros(4, dtype=torch.int64)[1:]
+    gone.untyped_storage().resize_(0)
+    for call in (lambda: arb.embedding(gone, t), lambda: arb.token_order(gone, 5), lambda: arb.embedding_grad(torch.zeros(3, 4), gone, 5)):
+        with pytest.raises(ValueError, match="memory"):
+            call()
+    with pytest.raises(ValueError, match="memory"):
+        arb.embedding(i, t.to_sparse())
