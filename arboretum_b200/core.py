@@ -370,6 +370,8 @@ class Garden(object):
         torch.cuda.current_stream(out.device).synchronize()  # the library fills it on a stream of its own
         _call_and_throw_if_error(_LIB.ALeafTokens(self.handle, data.handle, int(n_rounds),
                                                   ctypes.c_void_p(out.data_ptr())))
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)  # a lookup that saved it for its backward pass has to see this
         return out.t()
 
     def refine_leaves(self, data, steps, lr=0.01, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, state_bits=32):

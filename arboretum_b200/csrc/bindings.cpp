@@ -77,6 +77,11 @@ void no_grad(const at::Tensor &t, const char *name) {
                     " requires grad, which is not recorded here: pass it detached and use embedding_grad for the backward pass");
 }
 
+// autograd has to see that this was written in place.  An inference tensor has no version.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void on_device(const at::Tensor &t, const char *name, c10::Device device) {
   TORCH_CHECK_VALUE(t.device() == device, name, " is on ", t.device().str(), ", the others are on ", device.str());
 }
@@ -200,6 +205,7 @@ PyObject *embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
   call(AEmbedding(table.const_data_ptr(), type, rows, dim, table.stride(0), b.tokens.const_data_ptr(), b.bytes, b.bags, b.per_bag,
                   b.bag_stride, b.token_stride, number(args[2]), out.rows.data_ptr(), out.type, out.rows.stride(0), device,
                   stream_of(device)));
+  if (out.given) written(out.whole);
   return THPVariable_Wrap(out.whole);
   ARB_END
 }
@@ -290,6 +296,7 @@ PyObject *embedding_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
   }
   call(AEmbeddingGrad(grad.const_data_ptr(), type, b.bags, dim, grad.stride(0), order_at, b.per_bag, rows, number(args[3]),
                       out.rows.data_ptr(), out.type, out.rows.stride(0), accumulate, scratch_at, device, stream.stream()));
+  if (out.given) written(out.whole);
   return THPVariable_Wrap(out.whole);
   ARB_END
 }
@@ -404,12 +411,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   need(n, 4);
   Optimizer &o = optimizer(args[0]);
   // one look at every parameter: 500 of them are further apart than the first-level cache is large
-  std::vector<c10::TensorImpl *> recorded;  // autograd has to see that these changed
-  for (size_t i = 0; i < o.params.size(); ++i) {
-    c10::TensorImpl *p = o.params[i].unsafeGetTensorImpl();
-    TORCH_CHECK_VALUE(p->data() == o.at[i], "a parameter's memory has moved since the optimizer was made");
-    if (p->requires_grad()) recorded.push_back(p);
-  }
+  for (size_t i = 0; i < o.params.size(); ++i)
+    TORCH_CHECK_VALUE(o.params[i].unsafeGetTensorImpl()->data() == o.at[i], "a parameter's memory has moved since the optimizer was made");
   std::vector<const void *> given;
   const std::vector<const void *> *grads = &o.grads;
   bool fp32 = o.bound_fp32;
@@ -431,7 +434,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (stream.stream() != o.stream)  // the optimizer's memory must not be handed out again before that stream is done with it
     for (const at::Tensor &b : o.buffers) b.record_stream(stream);
   call(AAdamWStep(o.handle, grads->data(), int(grads->size()), fp32, lr, lr_device, grad_scale, stream.stream()));
-  for (c10::TensorImpl *p : recorded) p->bump_version();
+  for (size_t i = 0; i < o.params.size(); ++i)  // also a parameter that was passed detached: it shares its counter
+    if ((*grads)[i] != nullptr) written(o.params[i]);
   Py_RETURN_NONE;
   ARB_END
 }

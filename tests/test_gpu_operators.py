@@ -933,3 +933,54 @@ def test_gradients_and_outputs_whose_memory_is_gone_are_refused():
     for call in (lambda: arb.embedding(i, table, out=out), lambda: arb.embedding_grad(table, i, 3, out=out)):
         with pytest.raises(ValueError, match="memory"):
             call()
+
+
+def test_autograd_sees_every_tensor_written_in_place():
+    """A backward pass that needs what a call has overwritten says so, whatever way the tensor went in."""
+    gen = _rng(5)
+    w = torch.ones(3, 4, device="cuda", requires_grad=True)
+    tok, table = torch.tensor([1, 0, 2], device="cuda"), torch.randn(3, 4, generator=gen).cuda()
+    order = arb.token_order(tok, 3)
+    for write in (lambda x: arb.embedding(tok, table, out=x), lambda x: arb.embedding(tok.view(1, 3).t(), table, pooled=True, out=x),
+                  lambda x: arb.embedding_grad(table, tok, 3, out=x), lambda x: arb.embedding_grad(table, order, 3, out=x, accumulate=True),
+                  lambda x: arb.AdamW([x]).step([table]), lambda x: arb.AdamW([x.detach()]).step([table]),
+                  lambda x: arb.AdamW([x.view(12)]).step([table.view(12)])):
+        x = torch.randn(3, 4, generator=gen).cuda()
+        y = (x * w).sum()
+        write(x)
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    # what a call has only read, or left as it was, stays usable
+    x = torch.randn(3, 4, generator=gen).cuda()
+    y = (x * w).sum()
+    arb.embedding(tok, x)
+    arb.embedding_grad(x, tok, 3)
+    arb.AdamW([x, torch.ones(4, device="cuda")]).step([None, table[0].contiguous()])
+    y.backward()
+    assert torch.equal(w.grad, x)
+
+
+def test_leaf_tokens_written_in_place_are_seen():
+    model, data, X, _ = _grown(0)
+    out = torch.zeros(5, len(X), dtype=torch.int32, device="cuda")
+    values = torch.ones(5 * 8, 2, device="cuda", requires_grad=True)
+    y = torch.nn.functional.embedding(out, values).sum()
+    model.leaf_tokens(data, out=out)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+
+
+def test_inference_tensors():
+    """They have no version to count, with and without a gradient asked for."""
+    with torch.inference_mode():
+        p, q = torch.ones(10, device="cuda"), torch.ones(10, device="cuda").requires_grad_()
+        out, tok, table = torch.zeros(3, 4, device="cuda"), torch.tensor([1, 0, 2], device="cuda"), torch.ones(3, 4, device="cuda")
+        o = arb.AdamW([p, q])
+        o.step([torch.ones(10, device="cuda")] * 2)
+    o.step([torch.ones(10, device="cuda")] * 2)
+    arb.embedding(tok, table, out=out)
+    arb.embedding_grad(table, tok, 3, out=out, accumulate=True)
+    assert torch.equal(p, q) and (p < 1).all() and o.steps == 2 and (out == 2).all()
+    with torch.inference_mode():
+        arb.embedding(tok, table, out=out)
+        assert (out == 1).all()
