@@ -72,9 +72,14 @@ int float_type(const at::Tensor &t, const char *name) {
   }
 }
 
+// Nothing here is recorded for derivatives: a tensor that carries one is refused, not stripped of it.
+void no_tangent(const at::Tensor &t, const char *name) {
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), name, " carries a tangent, which is not followed here: pass its primal");
+}
 void no_grad(const at::Tensor &t, const char *name) {
   TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), name,
                     " requires grad, which is not recorded here: pass it detached and use embedding_grad for the backward pass");
+  no_tangent(t, name);
 }
 
 // autograd has to see that this was written in place.  An inference tensor has no version.
@@ -343,6 +348,7 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     TORCH_CHECK_VALUE(gi->device() == pi->device(), "a gradient is on ", g.device().str(), ", its parameter on ", p.device().str());
     TORCH_CHECK_VALUE(gi->numel() == 0 || (gi->storage_offset() + gi->numel()) * int64_t(gi->itemsize()) <= int64_t(gi->unsafe_storage().nbytes()),
                       "a gradient lies outside its memory");
+    no_tangent(g, "a gradient");
     single = single && gi->dtype() == caffe2::TypeMeta::Make<float>();
     same = same && gi->dtype() == pi->dtype();
     at[size_t(i)] = gi->data();
@@ -363,6 +369,7 @@ PyObject *adamw(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!params) throw python_error();
   for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(params.get()); ++i) {
     const at::Tensor &p = tensor(PySequence_Fast_GET_ITEM(params.get(), i), "a parameter");
+    no_tangent(p, "a parameter");
     o->params.push_back(p);
     o->at.push_back(p.const_data_ptr());
     o->memory.push_back(p.storage());
@@ -402,6 +409,7 @@ const float *scalar(PyObject *t, const char *name, const Optimizer &o) {
   const at::Tensor &x = tensor(t, name);
   TORCH_CHECK_TYPE(x.scalar_type() == at::kFloat && x.numel() == 1, name, " must be a float32 tensor of one element");
   on_device(x, name, o.params[0].device());
+  no_tangent(x, name);
   return x.const_data_ptr<float>();
 }
 

@@ -984,3 +984,21 @@ def test_inference_tensors():
     with torch.inference_mode():
         arb.embedding(tok, table, out=out)
         assert (out == 1).all()
+
+
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+    i, t = torch.zeros(3, dtype=torch.int64, device="cuda"), torch.ones(3, 4, device="cuda")
+    o = arb.AdamW([t.clone()])
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: arb.embedding(i, dual), lambda: arb.embedding(i, t, out=dual.clone()), lambda: arb.embedding_grad(dual, i, 3),
+                     lambda: arb.AdamW([dual]), lambda: o.step([dual]), lambda: arb.AdamW([t], grads=[dual]),
+                     lambda: o.step([t], grad_scale=dual[0, :1])):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+    for call in (lambda x: arb.embedding(i, x), lambda x: arb.embedding_grad(x, i, 3)):
+        for transform in (lambda f: torch.func.jvp(f, (t,), (t,)), lambda f: torch.vmap(f)(t[None]), lambda f: torch.func.vjp(f, t)):
+            with pytest.raises((ValueError, RuntimeError)):
+                transform(call)
+    assert o.steps == 0

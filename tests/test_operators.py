@@ -183,3 +183,24 @@ def test_tensors_whose_memory_is_gone_are_refused():
             call()
     with pytest.raises(ValueError, match="memory"):
         arb.embedding(i, t.to_sparse())
+
+
+def test_tensors_with_tangents_are_refused():
+    """Forward-mode derivatives are not followed, so they are not dropped either."""
+    from torch.autograd import forward_ad
+    i = torch.zeros(3, dtype=torch.int64)
+    with forward_ad.dual_level():
+        table = forward_ad.make_dual(torch.zeros(5, 4), torch.ones(5, 4))
+        grad = forward_ad.make_dual(torch.zeros(3, 4), torch.ones(3, 4))
+        for call in (lambda: arb.embedding(i, table), lambda: arb.embedding_grad(grad, i, 5)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="tangent"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):
+            arb.embedding(i, forward_ad.unpack_dual(table).primal)
+    for call in (lambda t: arb.embedding(i, t), lambda t: arb.embedding_grad(t[:3], i, 5)):
+        with pytest.raises(Exception):  # never a result
+            torch.func.jvp(call, (torch.zeros(5, 4),), (torch.ones(5, 4),))
+        with pytest.raises(Exception):
+            torch.vmap(call)(torch.zeros(2, 5, 4))
