@@ -4,7 +4,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -167,6 +169,13 @@ Out output(PyObject *o, at::IntArrayRef shape, const at::Tensor &like, PyObject 
 
 void *stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
 
+// A trace would not see the call: the result would stand in it as a constant, or as memory nobody filled.
+void not_traced() {
+  const bool traced = at::tracer::impl::is_dispatch_enabled() ||
+                      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+  TORCH_CHECK_VALUE(!traced, "the operators on learned tables cannot be traced");
+}
+
 void need(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK_TYPE(n == want, "expected ", want, " arguments, got ", n); }
 double number(PyObject *o) {
   const double v = PyFloat_AsDouble(o);
@@ -183,6 +192,7 @@ int64_t whole_number(PyObject *o) {
 PyObject *embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
   ARB_BEGIN
   need(n, 6);
+  not_traced();
   const at::Tensor &table = tensor(args[1], "table");
   const int type = float_type(table, "table");
   TORCH_CHECK_VALUE(table.dim() == 2, "table must have two dimensions: rows x columns");
@@ -223,6 +233,7 @@ at::Tensor memory(int64_t bytes, c10::Device device) {
 PyObject *token_order(PyObject *, PyObject *const *args, Py_ssize_t n) {
   ARB_BEGIN
   need(n, 3);
+  not_traced();
   const Bags b = bags_of(args[0], PyObject_IsTrue(args[2]) == 1);
   const int64_t rows = whole_number(args[1]);
   int64_t order_bytes = 0, scratch_bytes = 0;
@@ -242,6 +253,7 @@ PyObject *token_order(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyObject *embedding_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
   ARB_BEGIN
   need(n, 9);
+  not_traced();
   at::Tensor grad = tensor(args[0], "grad");
   const int type = float_type(grad, "grad");
   no_grad(grad, "grad");
@@ -417,6 +429,7 @@ const float *scalar(PyObject *t, const char *name, const Optimizer &o) {
 PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   ARB_BEGIN
   need(n, 4);
+  not_traced();
   Optimizer &o = optimizer(args[0]);
   // one look at every parameter: 500 of them are further apart than the first-level cache is large
   for (size_t i = 0; i < o.params.size(); ++i)

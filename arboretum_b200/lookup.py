@@ -8,7 +8,7 @@ With one token a bag and wide rows this is the embedding of category codes or of
 The functions take torch CUDA tensors, work on the current stream of the tensors' device and only
 enqueue work: no synchronisation, so they can be captured into a CUDA graph.  They are not recorded
 by autograd: ``embedding_grad`` is the backward pass; tensors that require grad or carry a forward-mode
-tangent are refused.
+tangent are refused, and so are calls while torch traces them.
 """
 import torch  # noqa: F401  (_tensors.so needs its libraries)
 

@@ -204,3 +204,18 @@ def test_tensors_with_tangents_are_refused():
             torch.func.jvp(call, (torch.zeros(5, 4),), (torch.ones(5, 4),))
         with pytest.raises(Exception):
             torch.vmap(call)(torch.zeros(2, 5, 4))
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_tracing_is_refused():
+    """A trace that does not see a call would keep its result as a constant, or unfilled memory."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    i = torch.zeros(3, dtype=torch.int64)
+    t = torch.zeros(5, 4)
+    for call in (lambda x: arb.embedding(i, x), lambda x: arb.embedding_grad(x[:3], i, 5), lambda x: arb.token_order(x[:, 0].long(), 5).rows * x):
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, (t,))
+        with pytest.raises(ValueError, match="traced"):
+            make_fx(call)(t)
+        with pytest.raises(ValueError, match="CUDA"):
+            call(t)
