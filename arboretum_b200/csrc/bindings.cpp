@@ -62,6 +62,8 @@ const at::Tensor &tensor(PyObject *o, const char *name) {
   // a storage can be freed or shrunk under its tensors (untyped_storage().resize_)
   TORCH_CHECK_VALUE((t.storage_offset() + reach(t)) * int64_t(t.element_size()) <= int64_t(t.storage().nbytes()) || t.numel() == 0, name,
                     " lies outside its memory");
+  // of such a view the memory holds the values with their signs turned
+  TORCH_CHECK_VALUE(!t.is_neg(), name, " is a view to be negated: pass its resolve_neg()");
   return t;
 }
 
@@ -360,6 +362,7 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     TORCH_CHECK_VALUE(gi->device() == pi->device(), "a gradient is on ", g.device().str(), ", its parameter on ", p.device().str());
     TORCH_CHECK_VALUE(gi->numel() == 0 || (gi->storage_offset() + gi->numel()) * int64_t(gi->itemsize()) <= int64_t(gi->unsafe_storage().nbytes()),
                       "a gradient lies outside its memory");
+    TORCH_CHECK_VALUE(!g.is_neg(), "a gradient is a view to be negated: pass its resolve_neg()");
     no_tangent(g, "a gradient");
     single = single && gi->dtype() == caffe2::TypeMeta::Make<float>();
     same = same && gi->dtype() == pi->dtype();

@@ -1002,3 +1002,15 @@ def test_tangents_are_refused():
             with pytest.raises((ValueError, RuntimeError)):
                 transform(call)
     assert o.steps == 0
+
+
+def test_views_to_be_negated_are_refused():
+    i, t = torch.zeros(3, dtype=torch.int64, device="cuda"), torch.ones(3, 4, device="cuda")
+    turned = torch._neg_view(torch.ones(3, 4, device="cuda"))
+    o = arb.AdamW([t])
+    for call in (lambda: arb.embedding(i, t, out=turned), lambda: arb.embedding_grad(t, i, 3, out=turned), lambda: o.step([turned]),
+                 lambda: arb.AdamW([turned]), lambda: arb.AdamW([t], grads=[turned]), lambda: o.step([t], lr=turned[0, :1]),
+                 lambda: o.step([t], grad_scale=turned[0, :1])):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    assert torch.equal(arb.embedding(i, turned.resolve_neg()), -t) and o.steps == 0

@@ -219,3 +219,17 @@ def test_tracing_is_refused():
             make_fx(call)(t)
         with pytest.raises(ValueError, match="CUDA"):
             call(t)
+
+
+def test_views_to_be_negated_are_refused():
+    """The imaginary part of a conjugate is such a view: its memory holds the opposite."""
+    i = torch.zeros(3, dtype=torch.int64)
+    t = torch.zeros(5, 4)
+    part = torch.zeros(5, 1, dtype=torch.complex64).conj().imag
+    assert part.is_neg()
+    for call in (lambda: arb.embedding(i, part), lambda: arb.embedding(i, torch._neg_view(t)), lambda: arb.embedding_grad(torch._neg_view(t[:3]), i, 5),
+                 lambda: arb.embedding_grad(part[:3], i, 5), lambda: arb.embedding(torch._neg_view(i), t), lambda: arb.token_order(torch._neg_view(i), 5)):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    with pytest.raises(ValueError, match="CUDA"):
+        arb.embedding(i, part.resolve_neg())
