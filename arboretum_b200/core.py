@@ -37,7 +37,7 @@ def _load_lib():
                  "ABuildHistogramFromParents", "ANcclUniqueId", "AInitNccl", "AThresholdsNoAlloc", "ASharedAtomicPeak",
                  "AReleaseCachedMemory", "AEmbedding", "ATokenOrderBytes", "ATokenOrder", "AEmbeddingGradBytes",
                  "AEmbeddingGrad", "AAdamWBytes", "AAdamWCreate", "AAdamWSetStep", "AAdamWGetStep", "AAdamWStep",
-                 "AFreeAdamW", "ATreeCount", "ALeafTokens", "ARefineLeaves"):
+                 "AFreeAdamW", "ATreeCount", "AModelDevice", "ALeafTokens", "ARefineLeaves"):
         getattr(lib, name).restype = ctypes.c_char_p
     lib.ADumpModel.argtypes = [ctypes.POINTER(ctypes.c_char_p), ctypes.c_void_p]
     lib.AFreeDMatrix.argtypes = [ctypes.c_void_p]
@@ -92,6 +92,7 @@ def _load_lib():
     lib.AAdamWStep.argtypes = [ptr, ptr, i32, i32, f64, ptr, ptr, ptr]
     lib.AFreeAdamW.argtypes = [ptr]
     lib.ATreeCount.argtypes = [ptr, ptr]
+    lib.AModelDevice.argtypes = [ptr, ptr]
     lib.ALeafTokens.argtypes = [ptr, ptr, i32, ptr]
     lib.ARefineLeaves.argtypes = [ptr, ptr, i32, f64, f64, f64, f64, f64, i32]
     return lib
@@ -351,10 +352,16 @@ class Garden(object):
         _call_and_throw_if_error(_LIB.AGetGradientStep(self.handle, ctypes.byref(g), ctypes.byref(h)))
         return g.value, h.value
 
+    def _device(self):
+        device = ctypes.c_int(-1)
+        _call_and_throw_if_error(_LIB.AModelDevice(self.handle, ctypes.byref(device)))
+        return device.value
+
     def leaf_tokens(self, data, n_rounds=-1, out=None):
         """The leaf every row reaches in each of the first ``n_rounds`` trees (-1: all), as tokens of
         the table of all leaves: ``tree * leaves + leaf``, int32 [rows][trees], stored tree after tree.
-        ``out``: a contiguous int32 CUDA tensor [trees][rows] to fill; its transpose is returned."""
+        ``out``: a contiguous int32 tensor [trees][rows] on the model's device to fill; its transpose is
+        returned."""
         self._ensure_init()
         count = ctypes.c_int(0)
         _call_and_throw_if_error(_LIB.ATreeCount(self.handle, ctypes.byref(count)))
@@ -367,6 +374,9 @@ class Garden(object):
         if out.dtype != torch.int32 or tuple(out.shape) != (use, data.rows) or not out.is_contiguous() \
                 or out.device.type != 'cuda':
             raise ValueError("out must be a contiguous int32 CUDA tensor of %d trees x %d rows" % (use, data.rows))
+        device = self._device()
+        if out.device.index != device:
+            raise ValueError("out is on %s, the model works on cuda:%d" % (out.device, device))
         torch.cuda.current_stream(out.device).synchronize()  # the library fills it on a stream of its own
         _call_and_throw_if_error(_LIB.ALeafTokens(self.handle, data.handle, int(n_rounds),
                                                   ctypes.c_void_p(out.data_ptr())))

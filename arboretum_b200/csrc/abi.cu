@@ -351,6 +351,15 @@ const char *ATreeCount(VoidPointer garden, int *count) {
   ARB_CATCH
 }
 
+const char *AModelDevice(VoidPointer garden, int *device) {
+  ARB_TRY
+  ARB_CHECK(garden && device, "NULL argument");
+  Garden *g = static_cast<Garden *>(garden);
+  g->EnsureStream();
+  *device = g->device;
+  ARB_CATCH
+}
+
 const char *ALeafTokens(VoidPointer garden, VoidPointer data, int n_rounds, int *out) {
   ARB_TRY
   ARB_CHECK(garden && data && out, "NULL argument");
@@ -361,6 +370,10 @@ const char *ALeafTokens(VoidPointer garden, VoidPointer data, int n_rounds, int 
   const size_t bytes = use * size_t(d->rows) * sizeof(int);
   if (bytes == 0) return nullptr;
   if (is_device_pointer(out)) {
+    g->EnsureStream();
+    cudaPointerAttributes at;
+    ARB_CUDA(cudaPointerGetAttributes(&at, out));
+    ARB_CHECK(at.device == g->device, "out lies on another device than the model");
     g->LeafTokens(d, int(use), 1, out, size_t(d->rows));
   } else {
     g->EnsureStream();

@@ -1654,6 +1654,7 @@ Garden::Garden(const Configuration &c) : cfg(c), id(++g_models) {
 void Garden::EnsureStream() {
   if (stream) return;
   if (cfg.internal.device >= 0) ARB_CUDA(cudaSetDevice(cfg.internal.device));
+  ARB_CUDA(cudaGetDevice(&device));
   ARB_CUDA(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
 }
 
@@ -1756,6 +1757,7 @@ void Garden::LeafTokens(DataMatrix *data, int use, int group, int *out, size_t s
   const size_t n = size_t(data->rows);
   ARB_CHECK(max_fid < data->cols(), "the model tests a feature the matrix does not have");
   SyncForest();
+  ARB_CHECK(data->device < 0 || data->device == device, "the matrix lies on another device than the model");
   RowFeeder feed(data);
   const PackedTree pt{d_fid.as<int>(), d_thr.as<float>(), d_w.as<float>(), d_label.as<int>(),
                       d_category.as<unsigned>()};

@@ -212,6 +212,7 @@ class Garden {
   DevBuf d_fid, d_thr, d_w, d_label, d_category;
   size_t forest_trees_on_device = 0;
   cudaStream_t stream = nullptr;
+  int device = -1;  // of the stream
   Builder *builder = nullptr;
 };
 

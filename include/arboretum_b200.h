@@ -174,8 +174,12 @@ const char *ASharedAtomicPeak(int steps, double *pair_updates_per_s);
 
 /* Trees of the model (labels_count a boosting round). */
 const char *ATreeCount(VoidPointer garden, int *count);
+/* Ordinal of the device the model works on: `device` of its configuration, else the one that was
+ * current when it first needed one (this call, at the latest). */
+const char *AModelDevice(VoidPointer garden, int *device);
 /* The leaf that every row of `data` reaches in each of the first n_rounds trees (-1: all; a count of
- * trees, like APredict's): out[tree][row] = tree * 2^(depth - 1) + leaf, host or device memory. */
+ * trees, like APredict's): out[tree][row] = tree * 2^(depth - 1) + leaf, host memory or memory of the
+ * model's device. */
 const char *ALeafTokens(VoidPointer garden, VoidPointer data, int n_rounds, int *out);
 /* `steps` AdamW steps on the leaf values of all trees together, on the gradient of the mean loss over
  * `data` (its targets; the garden's objective): lookup, gradient by sorted tokens and AdamW step as

@@ -1014,3 +1014,16 @@ def test_views_to_be_negated_are_refused():
         with pytest.raises(ValueError, match="negated"):
             call()
     assert torch.equal(arb.embedding(i, turned.resolve_neg()), -t) and o.steps == 0
+
+
+def test_leaf_tokens_on_the_models_device():
+    import ctypes
+    model, data, X, _ = _grown(0)
+    device = ctypes.c_int(-1)
+    assert arb.lib().AModelDevice(model.handle, ctypes.byref(device)) is None and device.value == torch.cuda.current_device()
+    want = model.leaf_tokens(data)
+    out = torch.empty(5, len(X), dtype=torch.int32, device=torch.device("cuda", device.value))
+    assert np.array_equal(model.leaf_tokens(data, out=out).cpu().numpy(), want)
+    if torch.cuda.device_count() > 1:
+        with pytest.raises(ValueError, match="the model works on"):
+            model.leaf_tokens(data, out=out.to("cuda:%d" % (1 - device.value)))

@@ -233,3 +233,25 @@ def test_views_to_be_negated_are_refused():
             call()
     with pytest.raises(ValueError, match="CUDA"):
         arb.embedding(i, part.resolve_neg())
+
+
+def test_leaf_tokens_refuse_another_device(monkeypatch):
+    """The model's kernel does not write to the memory of a device it does not work on."""
+    data = arb.DMatrix(np.zeros((3, 2), np.float32), y=np.zeros(3, np.float32))
+    model = arb.Garden({"objective": 0, "method": 1, "tree": {"max_depth": 2}}, data)
+
+    class Out:  # looks like a tensor of the second device, of no trees
+        dtype, shape, device = torch.int32, (0, 3), torch.device("cuda", 1)
+        is_contiguous = is_inference = lambda self: True
+        data_ptr = lambda self: 1 << 20  # noqa: E731
+        t = lambda self: self  # noqa: E731
+
+    class Stream:
+        synchronize = lambda self: None  # noqa: E731
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: Stream())
+    monkeypatch.setattr(arb.Garden, "_device", lambda self: 0, raising=False)
+    with pytest.raises(ValueError, match="cuda:1, the model works on cuda:0"):
+        model.leaf_tokens(data, out=Out())
+    monkeypatch.setattr(arb.Garden, "_device", lambda self: 1, raising=False)
+    assert isinstance(model.leaf_tokens(data, out=Out()), Out)
+    assert "NULL" in _message(LIB.AModelDevice(None, ctypes.byref(ctypes.c_int(0)))) and "NULL" in _message(LIB.AModelDevice(model.handle, None))
