@@ -1037,9 +1037,12 @@ __global__ void __launch_bounds__(kNarrowThreads, DIM == 1 ? 3 : 1) narrow_grad_
 }
 
 // Wider rows over a blocked order: a group of tx lanes takes a row's columns over a share of the runs
-// (blockIdx.z of `splits`), from device memory.
+// (blockIdx.z of `splits`), from device memory.  A share of a row that every bag names is one group's sum
+// over a hundred thousand bags and more, so it is held in 64 bits: left to right in fp32 a sum of 100003
+// equal values was off by 8200 half steps.  Bound by that chain where rows are few: 65536 bags of 4 over
+// 2 x 8 fp32 columns keep 5 CTAs busy.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLaunch a, TokenOrder o, int tx_bits, int vecs,
+__global__ void __launch_bounds__(kGradThreads, 4) blocked_grad_kernel(LookupGradLaunch a, TokenOrder o, int tx_bits, int vecs,
                                                                     int chunks, int splits, float *__restrict__ partial) {
   overlap_release();
   overlap_wait();
@@ -1051,9 +1054,9 @@ __global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLa
     const int c = chunk * tx + lane;
     if (c >= vecs) continue;
     const T *grad = static_cast<const T *>(a.grad) + (long long)c * VEC;
-    float sum[VEC];
+    double total[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+    for (int j = 0; j < VEC; ++j) total[j] = 0.0;
     for (int k = k0; k < k1; ++k) {
       const unsigned *begin = o.vec_begin + size_t(k) * (o.rows + 1) + v;
       const long long bag0 = (long long)k * kBlockBags;
@@ -1068,21 +1071,27 @@ __global__ void __launch_bounds__(kGradThreads) blocked_grad_kernel(LookupGradLa
           x[i].clear();
           if (id != kNoBag) x[i].load(grad + (bag0 + id / 4) * a.grad_stride);
         }
+        float sum[VEC];  // of eight bags: seven additions
+        x[0].get(sum);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i].add_to(sum);
+        for (int i = 1; i < 8; ++i) x[i].add_to(sum);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) total[j] += double(sum[j]);
       }
     }
+    // one rounding a share; the shares are joined in 64 bits again
     float *out = partial + ((size_t(blockIdx.z) * o.rows + v) * vecs + c) * VEC;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) out[j] = sum[j];
+    for (int j = 0; j < VEC; ++j) out[j] = float(total[j]);
   }
 }
 
-// the shares' sums: eight groups of lanes take every eighth share, and their sums are added in order
+// the shares' sums, in 64 bits (there may be 65535 of them): eight groups of lanes take every eighth
+// share, and their sums are added in order
 template <typename O>
 __global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLaunch a, long long rows, int splits,
                                                                     const float *__restrict__ partial) {
-  __shared__ float part[kGradThreads];
+  __shared__ double part[kGradThreads];
   constexpr int kSlices = kGradThreads / 32;
   overlap_release();
   overlap_wait();
@@ -1090,17 +1099,17 @@ __global__ void __launch_bounds__(kGradThreads) blocked_join_kernel(LookupGradLa
   const long long n = rows * a.dim;
   for (long long i0 = blockIdx.x * 32ll; i0 < n; i0 += gridDim.x * 32ll) {
     const long long i = i0 + lane;
-    float sum = 0.0f;
+    double total = 0.0;
     if (i < n)
 #pragma unroll 8
-      for (int k = slice; k < splits; k += kSlices) sum += partial[size_t(k) * n + i];
+      for (int k = slice; k < splits; k += kSlices) total += double(partial[size_t(k) * n + i]);
     __syncthreads();
-    part[threadIdx.x] = sum;
+    part[threadIdx.x] = total;
     __syncthreads();
     if (slice != 0 || i >= n) continue;
 #pragma unroll
-    for (int g = 1; g < kSlices; ++g) sum += part[g * 32 + lane];
-    sum *= a.scale;
+    for (int g = 1; g < kSlices; ++g) total += part[g * 32 + lane];
+    const float sum = float(total) * a.scale;
     O *at = static_cast<O *>(a.out) + i / a.dim * a.out_stride + i % a.dim;
     if (!a.accumulate) from_f32(sum, *at);
     else if (sum != 0.0f) from_f32(to_f32(*at) + sum, *at);  // a row without bags keeps its bits
@@ -1422,7 +1431,9 @@ unsigned piece_of(int64_t count, int64_t rows) {
 namespace {
 constexpr int64_t kMostClusterTokens = int64_t(8) * kClusterThreads * kMostClusterItems;
 // An order is kept by runs of bags where a row has 32 bags a run or more, on average: then a run's
-// sums are worth more than the look at where its bags begin.
+// sums are worth more than the look at where its bags begin.  Chosen for rows of up to three columns,
+// whose gradients of a run fit shared memory; an order does not know the columns, so wider rows over few
+// rows take it too, at the price named at blocked_grad_kernel.
 int blocks_of(int64_t bags, int64_t per_bag, int64_t rows) {
   const int64_t blocks = (bags + kBlockBags - 1) / kBlockBags;
   const bool many = per_bag > 1 && bags * per_bag > kMostClusterTokens && bags * per_bag >= 32 * rows * blocks;
@@ -1571,7 +1582,7 @@ void launch_token_order(const TokenView &t, const TokenOrder &o, void *scratch, 
 namespace {
 
 // shares a row's runs are divided into: one run a share where they fit shared memory, else as many
-// shares as it takes to fill the device
+// shares as it takes to fill the device, but no more than there are runs
 int splits_of(const TokenOrder &o, int64_t dim) {
   if (dim <= 3) return o.blocks;
   const int64_t lanes = std::max<int64_t>(1, o.rows * ((dim + 7) / 8));
@@ -1619,7 +1630,7 @@ void blocked_grad(const LookupGradLaunch &a, const TokenOrder &o, int vec, float
   if (a.dim == 1) narrow_grad_with<T, 1>(a, o, partial, s);
   else if (a.dim == 2) narrow_grad_with<T, 2>(a, o, partial, s);
   else if (a.dim == 3) narrow_grad_with<T, 3>(a, o, partial, s);
-  else if (vec * sizeof(T) == 16) blocked_grad_with<T, 16 / sizeof(T)>(a, o, splits, partial, s);
+  else if (vec >= 4) blocked_grad_with<T, 4>(a, o, splits, partial, s);
   else if (vec * sizeof(T) >= 4) blocked_grad_with<T, 4 / sizeof(T)>(a, o, splits, partial, s);
   else blocked_grad_with<T, 1>(a, o, splits, partial, s);
   launch_overlapped(blocked_join_kernel<O>, dim3(grid_of(o.rows * a.dim, 32, 32)), dim3(kGradThreads), 0, s, a,

@@ -1027,3 +1027,26 @@ def test_leaf_tokens_on_the_models_device():
     if torch.cuda.device_count() > 1:
         with pytest.raises(ValueError, match="the model works on"):
             model.leaf_tokens(data, out=out.to("cuda:%d" % (1 - device.value)))
+
+
+@pytest.mark.parametrize("bags,per_bag,rows,dim", [(200000, 2, 3, 8), (100003, 3, 1, 40), (300007, 2, 600, 256), (70001, 5, 2, 7),
+                                                   (70001, 5, 2, 1), (65536, 4, 2, 3)])
+def test_sums_of_equal_values_do_not_drift(bags, per_bag, rows, dim):
+    """Sums of one sign over an order kept by runs, where every rounding can go the same way: the limit
+    follows from the longest chain of additions, not from the number of terms."""
+    gen = _rng(bags, rows)
+    tok = torch.randint(0, rows, (bags, per_bag), generator=gen)
+    tok[:, 0] = 0  # a row that every bag names
+    count = torch.bincount(tok.view(-1), minlength=rows).double()[:, None]
+    if dim > 3:
+        # eight bags: seven additions; sums of eights in 64 bits, rounded a share; their join in 64 bits, rounded, times scale
+        chain = 7 + 1 + 2
+    else:
+        # eight bags: seven; a warp's 32 vectors: five; what the 32 before them carry on: one for every 256
+        # bags of a row in a run of 16383 bags; the join as above
+        chain = 7 + 5 + -(-16383 * per_bag // 256) + 1 + 2
+    for dtype in (F32, BF16):
+        value = torch.tensor(0.1).to(dtype)
+        got = arb.embedding_grad(value.expand(bags, dim).contiguous().cuda(), tok.cuda(), rows, scale=0.3, pooled=True, out_dtype=F32)
+        want = count * value.double() * float(np.float32(0.3))
+        assert ((got.double().cpu() - want).abs() <= (chain + 1) * U * want).all(), float(((got.double().cpu() - want) / want).abs().max() / U)
