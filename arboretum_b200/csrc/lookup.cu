@@ -36,20 +36,25 @@ struct LaneShape {
 
 constexpr int kLookupThreads = 256;
 
-// A thread's vector of the sum over the tokens k0, k0 + ly, .. of bag b, K rows in flight.
+// Rows a lane adds up in fp32 before the sum is set aside and begun anew: a bag of a million tokens would
+// drift by thousands of half steps in one chain.
+constexpr int kChain = 1024;
+
+// A thread's vector of the sum over the tokens begin + slice, begin + slice + ly, .. below `end` of bag b,
+// K rows in flight.
 // TOGETHER: the lanes of a group (at least eight) fetch a token each and hand them around, so that a
 // bag's tokens cost one access and empty slots cost nothing.
 template <typename T, int VEC, int K, bool TOGETHER>
-__device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, int slice, int ly, int tx, int c, int vecs,
-                                           float (&sum)[VEC]) {
+__device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, long long begin, long long end, int slice, int ly, int tx,
+                                           int c, int vecs, float (&sum)[VEC]) {
   const T *table = static_cast<const T *>(a.table) + (long long)c * VEC;
-  const long long per_bag = b < a.tokens.bags ? a.tokens.per_bag : 0;
+  const long long mine = b < a.tokens.bags ? end : begin;
   if (TOGETHER) {
     const int width = min(tx, 32), lane = threadIdx.x & 31, group0 = lane & ~(width - 1);
     // every lane of the warp makes as many rounds as a whole bag needs: the shuffles want them all
-    for (long long k0 = 0; k0 < a.tokens.per_bag; k0 += (long long)ly * width) {
+    for (long long k0 = begin; k0 < end; k0 += (long long)ly * width) {
       const long long k = k0 + slice + (long long)(lane - group0) * ly;
-      const long long row = k < per_bag ? row_at(a.tokens, a.rows, b, k) : -1;
+      const long long row = k < mine ? row_at(a.tokens, a.rows, b, k) : -1;
       const int index = int(row);  // rows fit 31 bits
       unsigned todo = (__ballot_sync(0xffffffffu, row >= 0) >> group0) & (width == 32 ? 0xffffffffu : (1u << width) - 1u);
       while (__any_sync(0xffffffffu, todo != 0)) {
@@ -67,10 +72,10 @@ __device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, i
       }
     }
   } else {
-    for (long long k0 = slice; k0 < per_bag; k0 += (long long)ly * K) {
+    for (long long k0 = begin + slice; k0 < mine; k0 += (long long)ly * K) {
       long long row[K];
 #pragma unroll
-      for (int i = 0; i < K; ++i) row[i] = k0 + i * ly < per_bag ? row_at(a.tokens, a.rows, b, k0 + i * ly) : -1;
+      for (int i = 0; i < K; ++i) row[i] = k0 + i * ly < mine ? row_at(a.tokens, a.rows, b, k0 + i * ly) : -1;
       Vec<T, VEC> v[K];
 #pragma unroll
       for (int i = 0; i < K; ++i) {
@@ -89,7 +94,9 @@ __device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, i
 // their sums through shared memory in a fixed order.  20011 bags of up to 12 rows of 100 fp16 columns, a
 // table that the second-level cache holds: 14.3 us, bound by the two accesses' latency (six CTAs an SM;
 // 16.6 with the five that fit without a limit on registers).
-template <typename T, typename O, int VEC, bool TOGETHER>
+// LONG: bags of more than kChain rows a lane, whose sums are set aside; apart from the others, which would
+// pay for it with registers (a million bags of 128 rows of one column: 294 us, 329 in one kernel).
+template <typename T, typename O, int VEC, bool TOGETHER, bool LONG>
 __global__ void __launch_bounds__(kLookupThreads, 6) lookup_kernel(LookupLaunch a, LaneShape sh, int vecs, int chunks) {
   __shared__ float part[kLookupThreads * VEC];
   const int tx = 1 << sh.tx_bits, ly = 1 << sh.ly_bits;
@@ -99,9 +106,24 @@ __global__ void __launch_bounds__(kLookupThreads, 6) lookup_kernel(LookupLaunch 
   for (int chunk = blockIdx.y; chunk < chunks; chunk += gridDim.y) {
     const int c = chunk * tx + lane;
     float sum[VEC];
+    if constexpr (!LONG) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
-    sum_tokens<T, VEC, 8, TOGETHER>(a, b, slice, ly, tx, c, vecs, sum);
+      for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+      sum_tokens<T, VEC, 8, TOGETHER>(a, b, 0, a.tokens.per_bag, slice, ly, tx, c, vecs, sum);
+    } else {
+      __syncthreads();  // others may still read what they join of the columns before
+      for (long long k = 0; k < a.tokens.per_bag; k += (long long)kChain * ly) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sum[j] = 0.0f;
+        sum_tokens<T, VEC, 8, TOGETHER>(a, b, k, min(k + (long long)kChain * ly, (long long)a.tokens.per_bag), slice, ly, tx, c, vecs, sum);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          float &total = part[j * kLookupThreads + threadIdx.x];
+          if (k != 0) sum[j] += total;
+          total = sum[j];
+        }
+      }
+    }
     if (ly > 1) {
       __syncthreads();
 #pragma unroll
@@ -1352,13 +1374,20 @@ void lookup_with(const LookupLaunch &a, cudaStream_t s) {
   const int groups = kLookupThreads >> (sh.tx_bits + sh.ly_bits);
   const int chunks = int((vecs + (int64_t(u) << sh.tx_bits) - 1) / (int64_t(u) << sh.tx_bits));
   const dim3 grid(unsigned((a.tokens.bags + groups - 1) / groups), unsigned(std::min(chunks, 65535)));
-  if (pooled && sh.tx_bits >= 3) lookup_kernel<T, O, VEC, true><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
-  else if (pooled) lookup_kernel<T, O, VEC, false><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  const bool together = sh.tx_bits >= 3, long_bags = a.tokens.per_bag > int64_t(kChain) << sh.ly_bits;
+  if (long_bags && together) lookup_kernel<T, O, VEC, true, true><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  else if (long_bags) lookup_kernel<T, O, VEC, false, true><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  else if (pooled && together) lookup_kernel<T, O, VEC, true, false><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
+  else if (pooled) lookup_kernel<T, O, VEC, false, false><<<grid, kLookupThreads, 0, s>>>(a, sh, int(vecs), chunks);
   else if (u > 1) lookup_rows_kernel<T, O, VEC, kWide><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
   else lookup_rows_kernel<T, O, VEC, 1><<<grid, kLookupThreads, 0, s>>>(a, sh.tx_bits, int(vecs), chunks);
 }
 
 constexpr size_t kMostTableBytes = 200 << 10;  // of shared memory, one CTA an SM
+// Tokens of a bag that one thread adds up in fp32.  Setting sums aside like lookup_kernel costs the usual
+// bags 5 % here (122 us instead of 115 for a million of 128 tokens), and a table of more trees that fits
+// has no more than a dozen leaves a tree.
+constexpr int64_t kMostTableTokens = 4 * kChain;
 
 template <typename T, typename O, typename I, int DIM>
 void lookup_table_with(const LookupLaunch &a, cudaStream_t s) {
@@ -1381,10 +1410,10 @@ void lookup_table_with(const LookupLaunch &a, cudaStream_t s) {
 
 template <typename T, typename O>
 bool lookup_table(const LookupLaunch &a, cudaStream_t s) {
-  // Only where the bags of one slot lie next to one another, the table fits, and the lookups are
-  // many times the words every SM has to copy first.
+  // Only where the bags of one slot lie next to one another, the table fits, the lookups are many times
+  // the words every SM has to copy first, and a thread's chain of additions is not too long.
   const TokenView &t = a.tokens;
-  if (a.dim > 3 || t.per_bag < 2 || std::abs(t.bag_stride) >= std::abs(t.token_stride) ||
+  if (a.dim > 3 || t.per_bag < 2 || t.per_bag > kMostTableTokens || std::abs(t.bag_stride) >= std::abs(t.token_stride) ||
       size_t(a.rows + 1) * size_t(a.dim) * sizeof(float) > kMostTableBytes ||
       t.count() < 4 * a.rows * device_sm_count())
     return false;

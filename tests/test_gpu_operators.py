@@ -1050,3 +1050,27 @@ def test_sums_of_equal_values_do_not_drift(bags, per_bag, rows, dim):
         got = arb.embedding_grad(value.expand(bags, dim).contiguous().cuda(), tok.cuda(), rows, scale=0.3, pooled=True, out_dtype=F32)
         want = count * value.double() * float(np.float32(0.3))
         assert ((got.double().cpu() - want).abs() <= (chain + 1) * U * want).all(), float(((got.double().cpu() - want) / want).abs().max() / U)
+
+
+@pytest.mark.parametrize("bags,per_bag,dim", [(1, 1 << 20, 1), (1, 1 << 20, 64), (3, 300000, 257), (300, 65536, 1), (2000, 4097, 2), (2000, 4096, 2),
+                                              (2, 1025, 1030), (64, 2500, 2048)])
+def test_long_bags_do_not_drift(bags, per_bag, dim):
+    """Equal values, where every rounding can go the same way: at most 4096 rows are added in one chain, and
+    the sums of 1024 rows after one another; a whole CTA's lanes may share a bag."""
+    chain = max(4096, 1024 + per_bag // 1024 + 1) + 8 + 1
+    for dtype in (F32, F16):
+        table = torch.full((3, dim), 0.1, dtype=dtype, device="cuda")
+        want = per_bag * table[0, 0].double().cpu() * float(np.float32(0.3))
+        rows = torch.randint(0, 3, (per_bag, bags), generator=_rng(bags, per_bag), dtype=torch.int32).cuda()
+        for tok in (rows.t(), rows.t().contiguous()):
+            got = arb.embedding(tok, table, scale=0.3, pooled=True, out_dtype=F32)
+            assert got.shape == (bags, dim) and ((got.double().cpu() - want).abs() <= chain * U * want).all()
+    # and the sums themselves: integers, exact in any order
+    table = torch.randint(-3, 4, (500, dim), generator=_rng(dim)).float()
+    tok = torch.randint(-1, 500, (per_bag, bags), generator=_rng(per_bag), dtype=torch.int32)
+    total = torch.zeros(bags, dim, dtype=torch.float64)
+    for b in range(min(bags, 8)):
+        n = torch.bincount(tok[:, b].long() + 1, minlength=501)[1:].double()
+        total[b] = n @ table.double()
+    for view in (tok.cuda().t(), tok.cuda().t().contiguous()):
+        assert torch.equal(arb.embedding(view, table.cuda(), pooled=True).cpu().double()[:8], total[:8])
