@@ -17,7 +17,7 @@ LIB = os.path.join(HERE, "libarboretum.so")
 SOURCES = ["abi.cu", "garden.cu", "hist.cu", "split.cu", "partition.cu", "objective.cu", "quantize.cu", "exchange.cu",
            "lookup.cu", "adamw.cu", "operators_abi.cu"]
 HEADERS = ["common.cuh", "config.h", "gain.cuh", "garden.h", "json.h", "kernels.cuh", "exchange.h", "abi.h", "operators.h",
-           "vec.cuh"]
+           "vec.cuh", "root.cuh"]
 BINDINGS = os.path.join(HERE, "_tensors.so")  # the operators on torch tensors
 NVCC = os.environ.get("NVCC", "nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

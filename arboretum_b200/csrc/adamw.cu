@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "operators.h"
+#include "root.cuh"
 #include "vec.cuh"
 
 namespace arb {
@@ -58,25 +59,6 @@ __device__ __forceinline__ unsigned upper_bytes(unsigned a, unsigned b, unsigned
   return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
-// two float operations in one instruction, each rounded like the single one
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mul.rn.f32x2 z, x, y; mov.b64 {%0, %1}, z;}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{.reg .b64 x, y, z, w; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7}; fma.rn.f32x2 w, x, y, z; "
-      "mov.b64 {%0, %1}, w;}"
-      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
-}
-// a + b as a * one + b: of a packed product and a packed sum the assembler makes one operation with one
-// rounding, whatever it is told; `one` is 1 that it does not know of
-__device__ __forceinline__ float2 add2(float2 a, float2 b, float one) { return fma2(a, make_float2(one, one), b); }
-__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
-
 // exponent field of the scale of a block whose largest magnitude has these bits: the largest code
 // stands for 448 = 1.75 * 2^8.  255: the block holds a value that is not finite
 __device__ __forceinline__ unsigned scale_field(unsigned top_bits) {
@@ -110,19 +92,6 @@ __device__ __forceinline__ Scalars scalars_of(const AdamWLaunch &a) {
   return c;
 }
 
-// Root of v >= 0, rounded to the nearest like sqrtf: one Newton step on the hardware's reciprocal root
-// with the residual in a fused multiply-add (Markstein's correction), a third of sqrtf's instructions.
-// Exhaustively equal to sqrtf on all of [2^-100, 2^126]; the others take sqrtf.
-__device__ __forceinline__ float2 root_of(float2 v) {
-  float2 q;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q.x) : "f"(v.x));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(q.y) : "f"(v.y));
-  const float2 s = mul2(v, q);
-  return fma2(fma2(mul2(s, both(-1.0f)), s, v), mul2(q, both(0.5f)), s);
-}
-__device__ __forceinline__ bool root_is_plain(unsigned largest, unsigned smallest) {
-  return largest <= 0x7E800000u && smallest >= 0x0D800000u;  // 2^126, 2^-100
-}
 // larger magnitude; a NaN stays
 __device__ __forceinline__ float larger(float a, float b) {
   float r;
