@@ -1074,3 +1074,62 @@ def test_long_bags_do_not_drift(bags, per_bag, dim):
         total[b] = n @ table.double()
     for view in (tok.cuda().t(), tok.cuda().t().contiguous()):
         assert torch.equal(arb.embedding(view, table.cuda(), pooled=True).cpu().double()[:8], total[:8])
+
+
+@pytest.mark.parametrize("bags,per_bag,rows,dim", [(40000, 1, 3000, 24), (33000, 1, 40000 * 17, 3), (40000, 5, 90, 2), (40000, 5, 90, 7), (1000, 3, 50, 70),
+                                                   (9, 1, 300000, 5), (0, 2, 40, 4)])
+def test_orders_in_graphs_and_on_other_streams(bags, per_bag, rows, dim):
+    """Every sort captured and replayed on new tokens; an order made on one stream and used on another
+    after its owner let it go."""
+    gen = _rng(bags, rows, dim)
+    make = lambda: (_tokens(bags, per_bag, rows, torch.int32, gen).cuda(), torch.randn(bags, dim, generator=gen).cuda())  # noqa: E731
+    tok, g = make()
+    want = arb.embedding_grad(g, tok, rows, pooled=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = arb.embedding_grad(g, tok, rows, pooled=True)
+        order = arb.token_order(tok, rows, pooled=True)
+        kept = arb.embedding_grad(g, order, rows)
+        bags_out = arb.embedding(tok, kept, pooled=True)
+    for _ in range(3):
+        out.fill_(7)
+        kept.fill_(7)
+        graph.replay()
+        assert torch.equal(out, want) and torch.equal(kept, want) and torch.equal(bags_out, arb.embedding(tok, want, pooled=True))
+        new = make()
+        tok.copy_(new[0])
+        g.copy_(new[1])
+        want = arb.embedding_grad(g, tok, rows, pooled=True)
+    side = torch.cuda.Stream()
+    order = arb.token_order(tok, rows, pooled=True)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = arb.embedding_grad(g, order, rows)
+    size = order._order[0].numel()
+    del order
+    torch.full((size,), 255, dtype=torch.uint8, device="cuda")  # would take the order's memory, were it free already
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows,trees", [(1, 1), (33, 3), (20011, 70)])
+def test_leaf_tokens_of_other_sizes(rows, trees):
+    """Against a walk of the dumped trees."""
+    import json
+    model, data, X, _ = _grown(0, rounds=trees)
+    rng = np.random.default_rng(rows)
+    Z = rng.normal(size=(rows, 6)).astype(np.float32)
+    Z[rng.random(Z.shape) < 0.05] = np.nan
+    tok = model.leaf_tokens(arb.DMatrix(Z))
+    dumped = json.loads(model.dump())["model"]
+    leaves = len(dumped[0]["weights"])
+    assert tok.shape == (rows, trees)
+    for t, tree in enumerate(dumped):
+        nodes = {n["id"]: n for n in tree["nodes"]}
+        at = np.zeros(rows, int)
+        for _ in range(tree["depth"] - 1):
+            fid = np.array([nodes[i]["fid"] for i in range(leaves - 1)])
+            thr = np.array([np.inf if nodes[i]["threshold"] is None else nodes[i]["threshold"] for i in range(leaves - 1)], np.float32)
+            left = Z[np.arange(rows), fid[at]] < thr[at]  # NaN goes right
+            at = 2 * at + np.where(left, 1, 2)
+        assert np.array_equal(tok[:, t], t * leaves + at - (leaves - 1))
