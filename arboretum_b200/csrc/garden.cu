@@ -1780,6 +1780,7 @@ void Garden::RefineLeaves(DataMatrix *data, const Refinement &r) {
   for (size_t t = 0; t < T; ++t) ARB_CHECK(size_t(trees[t].label) == t % K, "the trees are not in the order of their classes");
   ARB_CHECK(shards.world == 1, "leaf refinement does not work on row shards");
   const bool softmax = cfg.objective == kSoftMaxOneVsAll;
+  ARB_CHECK(softmax || K == 1, "leaf refinement of a regression wants labels_count 1: its loss has one output");
   ARB_CHECK(softmax ? data->has_labels() : data->has_y(), "the matrix has no targets");
   const int64_t per_class = int64_t(T / K);
   ARB_CHECK(int64_t(n) <= ((int64_t(1) << 31) - 2) / per_class, "more than 2^31 - 2 leaf tokens of a class");

@@ -182,10 +182,10 @@ const char *AModelDevice(VoidPointer garden, int *device);
  * model's device. */
 const char *ALeafTokens(VoidPointer garden, VoidPointer data, int n_rounds, int *out);
 /* `steps` AdamW steps on the leaf values of all trees together, on the gradient of the mean loss over
- * `data` (its targets; the garden's objective): lookup, gradient by sorted tokens and AdamW step as
- * below, one tensor a tree.  The trees' tests stay.  Training can go on afterwards; predictions that
- * AAppendLastTree has accumulated follow the new values in the next AGetY or AAppendLastTree (an
- * error when another model has added to the same matrix). */
+ * `data` (its targets; the garden's objective, with labels_count 1 unless it is multi:softmax): lookup,
+ * gradient by sorted tokens and AdamW step as below, one tensor a tree.  The trees' tests stay.
+ * Training can go on afterwards; predictions that AAppendLastTree has accumulated follow the new values
+ * in the next AGetY or AAppendLastTree (an error when another model has added to the same matrix). */
 const char *ARefineLeaves(VoidPointer garden, VoidPointer data, int steps, double lr, double beta1, double beta2, double eps,
                           double weight_decay, int state_bits);
 

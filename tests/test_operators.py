@@ -255,3 +255,16 @@ def test_leaf_tokens_refuse_another_device(monkeypatch):
     monkeypatch.setattr(arb.Garden, "_device", lambda self: 1, raising=False)
     assert isinstance(model.leaf_tokens(data, out=Out()), Out)
     assert "NULL" in _message(LIB.AModelDevice(None, ctypes.byref(ctypes.c_int(0)))) and "NULL" in _message(LIB.AModelDevice(model.handle, None))
+
+
+def test_refinement_refuses_a_regression_of_several_outputs():
+    """Its loss has one output: the trees of the others would move along a gradient that is none."""
+    import json
+    cfg = {"objective": 0, "method": 1, "tree": {"max_depth": 1, "labels_count": 2}}
+    nodes = [{"id": 0, "leaf": False, "left": 1, "right": 2, "threshold": 0.5, "fid": 0}, {"id": 1, "leaf": True, "idx": 0}, {"id": 2, "leaf": True, "idx": 1}]
+    model = arb.Garden(cfg)
+    model.load(json.dumps({"configuration": cfg, "model": [{"depth": 2, "nodes": nodes, "weights": [0.25, -0.25]}] * 2}))
+    before = model.dump()
+    with pytest.raises(arb.ArboretumError, match="labels_count"):
+        model.refine_leaves(arb.DMatrix(np.zeros((3, 2), np.float32), y=np.ones(3, np.float32)), 1)
+    assert model.dump() == before
