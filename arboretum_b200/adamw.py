@@ -132,9 +132,9 @@ class AdamW(object):
             x, y = getattr(self, k), state[k]
             if x.shape != y.shape or x.dtype != y.dtype:
                 raise ValueError("%s must be %d elements of %s" % (k, x.numel(), x.dtype))
+        _tensors.adamw_count(self._optimizer, int(state["step"]))  # refuses a bad count before anything is copied
         for k in mine:
             getattr(self, k).copy_(state[k])
-        _tensors.adamw_count(self._optimizer, int(state["step"]))
 
     def moments(self, k):
         """First and second moment of parameter ``k`` as float32 tensors of its shape."""

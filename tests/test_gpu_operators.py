@@ -1133,3 +1133,17 @@ def test_leaf_tokens_of_other_sizes(rows, trees):
             left = Z[np.arange(rows), fid[at]] < thr[at]  # NaN goes right
             at = 2 * at + np.where(left, 1, 2)
         assert np.array_equal(tok[:, t], t * leaves + at - (leaves - 1))
+
+
+def test_a_state_that_is_refused_changes_nothing():
+    p = torch.ones(200, device="cuda")
+    o = arb.AdamW([p])
+    o.step([torch.ones(200, device="cuda")])
+    kept = {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in o.state_dict().items()}
+    zeros = torch.zeros(256, device="cuda")
+    for bad in (dict(step=-1), dict(step="x"), dict(step=None), dict(moment1=zeros[:200]), dict(moment2=zeros.half())):
+        state = dict(step=5, moment1=zeros, moment2=zeros)
+        state.update(bad)
+        with pytest.raises((ValueError, TypeError, arb.ArboretumError)):
+            o.load_state_dict(state)
+        assert o.steps == 1 and torch.equal(o.moment1, kept["moment1"]) and torch.equal(o.moment2, kept["moment2"])
