@@ -61,7 +61,8 @@ TokenView check_tokens(const void *tokens, int bytes, int64_t bags, int64_t per_
                        int64_t token_stride, int64_t rows) {
   ARB_CHECK(bytes == 4 || bytes == 8, "tokens are int32 or int64");
   check_counts(bags, per_bag, rows);
-  ARB_CHECK(std::abs(bag_stride) <= kMostElements && std::abs(token_stride) <= kMostElements, "token stride out of range");
+  for (int64_t stride : {bag_stride, token_stride})  // (the least int64 has no absolute value)
+    ARB_CHECK(stride >= -kMostElements && stride <= kMostElements, "token stride out of range");
   if (bags * per_bag > 0) {
     ARB_CHECK(tokens != nullptr, "tokens is NULL");
     check_aligned(tokens, size_t(bytes), "tokens");

@@ -268,3 +268,10 @@ def test_refinement_refuses_a_regression_of_several_outputs():
     with pytest.raises(arb.ArboretumError, match="labels_count"):
         model.refine_leaves(arb.DMatrix(np.zeros((3, 2), np.float32), y=np.ones(3, np.float32)), 1)
     assert model.dump() == before
+
+
+@pytest.mark.parametrize("stride", [-2 ** 63, 2 ** 63 - 1, -2 ** 46 - 1, 2 ** 46 + 1])
+def test_token_strides_are_bounded_both_ways(stride):
+    assert "stride" in _message(_embedding(bag_stride=stride)) and "stride" in _message(_embedding(token_stride=stride))
+    for strides in ((stride, 1), (1, stride)):
+        assert "stride" in _message(LIB.ATokenOrder(P, 4, 3, 2, strides[0], strides[1], 10, P, P, 0, None))
