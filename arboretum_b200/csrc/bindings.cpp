@@ -184,6 +184,11 @@ double number(PyObject *o) {
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;
 }
+bool truth(PyObject *o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw python_error();
+  return v != 0;
+}
 int64_t whole_number(PyObject *o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw python_error();
@@ -200,7 +205,7 @@ PyObject *embedding(PyObject *, PyObject *const *args, Py_ssize_t n) {
   TORCH_CHECK_VALUE(table.dim() == 2, "table must have two dimensions: rows x columns");
   TORCH_CHECK_VALUE(table.numel() == 0 || table.size(1) <= 1 || table.stride(1) == 1, "the columns of table must be contiguous");
   no_grad(table, "table");
-  const bool pooled = PyObject_IsTrue(args[3]) == 1;
+  const bool pooled = truth(args[3]);
   const Bags b = bags_of(args[0], pooled);
   const int device = cuda_index(table);
   on_device(b.tokens, "tokens", table.device());
@@ -236,7 +241,7 @@ PyObject *token_order(PyObject *, PyObject *const *args, Py_ssize_t n) {
   ARB_BEGIN
   need(n, 3);
   not_traced();
-  const Bags b = bags_of(args[0], PyObject_IsTrue(args[2]) == 1);
+  const Bags b = bags_of(args[0], truth(args[2]));
   const int64_t rows = whole_number(args[1]);
   int64_t order_bytes = 0, scratch_bytes = 0;
   call(ATokenOrderBytes(b.bags, b.per_bag, rows, &order_bytes, &scratch_bytes));
@@ -259,7 +264,7 @@ PyObject *embedding_grad(PyObject *, PyObject *const *args, Py_ssize_t n) {
   at::Tensor grad = tensor(args[0], "grad");
   const int type = float_type(grad, "grad");
   no_grad(grad, "grad");
-  const bool pooled = PyObject_IsTrue(args[4]) == 1, accumulate = PyObject_IsTrue(args[7]) == 1;
+  const bool pooled = truth(args[4]), accumulate = truth(args[7]);
   const int64_t rows = whole_number(args[2]);
   const bool sorted = args[8] != Py_None;
   Bags b{};

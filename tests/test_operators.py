@@ -275,3 +275,13 @@ def test_token_strides_are_bounded_both_ways(stride):
     assert "stride" in _message(_embedding(bag_stride=stride)) and "stride" in _message(_embedding(token_stride=stride))
     for strides in ((stride, 1), (1, stride)):
         assert "stride" in _message(LIB.ATokenOrder(P, 4, 3, 2, strides[0], strides[1], 10, P, P, 0, None))
+
+
+def test_a_flag_without_a_truth_value():
+    """Its own error comes out, not a result with an error behind it."""
+    i, t, both = torch.zeros(3, dtype=torch.int64), torch.zeros(3, 4), np.ones(2)
+    for call in (lambda: arb.embedding(i, t, pooled=both), lambda: arb.embedding_grad(t, i, 5, pooled=both), lambda: arb.embedding_grad(t, i, 5, out=t, accumulate=both)):
+        with pytest.raises(ValueError, match="ambiguous"):
+            call()
+    with pytest.raises(ValueError, match="ambiguous"):
+        arb.lookup._tensors.token_order(i, 5, both)
