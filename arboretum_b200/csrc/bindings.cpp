@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
@@ -77,8 +78,11 @@ int float_type(const at::Tensor &t, const char *name) {
 }
 
 // Nothing here is recorded for derivatives: a tensor that carries one is refused, not stripped of it.
-void no_tangent(const at::Tensor &t, const char *name) {
-  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), name, " carries a tangent, which is not followed here: pass its primal");
+// Tangents live in the dual level that is entered; without one no tensor is asked (20 ns each, more than
+// the rest of a gradient's checks).
+bool tangents() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+void no_tangent(const at::Tensor &t, const char *name, bool any = tangents()) {
+  TORCH_CHECK_VALUE(!any || !t._fw_grad(0).defined(), name, " carries a tangent, which is not followed here: pass its primal");
 }
 void no_grad(const at::Tensor &t, const char *name) {
   TORCH_CHECK_VALUE(!(t.requires_grad() && at::GradMode::is_enabled()), name,
@@ -86,9 +90,10 @@ void no_grad(const at::Tensor &t, const char *name) {
   no_tangent(t, name);
 }
 
-// autograd has to see that this was written in place.  An inference tensor has no version.
+// autograd has to see that this was written in place; an inference tensor has no version
 void written(const at::Tensor &t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  c10::TensorImpl *impl = t.unsafeGetTensorImpl();
+  if (impl->version_counter().enabled()) impl->bump_version();
 }
 
 void on_device(const at::Tensor &t, const char *name, c10::Device device) {
@@ -174,7 +179,8 @@ void *stream_of(int device) { return c10::cuda::getCurrentCUDAStream(device).str
 // A trace would not see the call: the result would stand in it as a constant, or as memory nobody filled.
 void not_traced() {
   const bool traced = at::tracer::impl::is_dispatch_enabled() ||
-                      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+                      (c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                       c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
   TORCH_CHECK_VALUE(!traced, "the operators on learned tables cannot be traced");
 }
 
@@ -345,6 +351,10 @@ Optimizer &optimizer(PyObject *o) {
   return *static_cast<Optimizer *>(p);
 }
 
+void stays(const Optimizer &o, size_t i) {
+  TORCH_CHECK_VALUE(o.params[i].unsafeGetTensorImpl()->data() == o.at[i], "a parameter's memory has moved since the optimizer was made");
+}
+
 // addresses of one gradient, or None, for every parameter; whether all are float32 (else each has its
 // parameter's type)
 bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at, std::vector<at::Tensor> *keep) {
@@ -354,9 +364,11 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
   TORCH_CHECK_VALUE(size_t(n) == o.params.size(), n, " gradients for ", o.params.size(), " parameters");
   at.resize(size_t(n));
   bool same = true, single = true;
+  const bool dual = tangents();
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject *item = PySequence_Fast_GET_ITEM(fast.get(), i);
     const at::Tensor &p = o.params[size_t(i)];
+    stays(o, size_t(i));
     at[size_t(i)] = nullptr;
     if (keep) keep->emplace_back();
     if (item == Py_None) continue;
@@ -368,7 +380,7 @@ bool addresses(const Optimizer &o, PyObject *list, std::vector<const void *> &at
     TORCH_CHECK_VALUE(gi->numel() == 0 || (gi->storage_offset() + gi->numel()) * int64_t(gi->itemsize()) <= int64_t(gi->unsafe_storage().nbytes()),
                       "a gradient lies outside its memory");
     TORCH_CHECK_VALUE(!g.is_neg(), "a gradient is a view to be negated: pass its resolve_neg()");
-    no_tangent(g, "a gradient");
+    no_tangent(g, "a gradient", dual);
     single = single && gi->dtype() == caffe2::TypeMeta::Make<float>();
     same = same && gi->dtype() == pi->dtype();
     at[size_t(i)] = gi->data();
@@ -439,9 +451,7 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   need(n, 4);
   not_traced();
   Optimizer &o = optimizer(args[0]);
-  // one look at every parameter: 500 of them are further apart than the first-level cache is large
-  for (size_t i = 0; i < o.params.size(); ++i)
-    TORCH_CHECK_VALUE(o.params[i].unsafeGetTensorImpl()->data() == o.at[i], "a parameter's memory has moved since the optimizer was made");
+  // one look at every parameter and its gradient: 500 of them are further apart than the first-level cache is large
   std::vector<const void *> given;
   const std::vector<const void *> *grads = &o.grads;
   bool fp32 = o.bound_fp32;
@@ -450,9 +460,11 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
     grads = &given;
   } else {
     TORCH_CHECK_VALUE(o.has_bound, "no gradients: pass grads to step() or to the constructor");
-    for (size_t i = 0; i < o.grads.size(); ++i)
+    for (size_t i = 0; i < o.grads.size(); ++i) {
+      stays(o, i);
       TORCH_CHECK_VALUE(!o.bound[i].defined() || o.bound[i].unsafeGetTensorImpl()->data() == o.grads[i],
                         "a gradient's memory has moved since the optimizer was made");
+    }
   }
   double lr = 0.0;
   const float *lr_device = nullptr;
@@ -463,7 +475,8 @@ PyObject *adamw_step(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (stream.stream() != o.stream)  // the optimizer's memory must not be handed out again before that stream is done with it
     for (const at::Tensor &b : o.buffers) b.record_stream(stream);
   call(AAdamWStep(o.handle, grads->data(), int(grads->size()), fp32, lr, lr_device, grad_scale, stream.stream()));
-  for (size_t i = 0; i < o.params.size(); ++i)  // also a parameter that was passed detached: it shares its counter
+  // also a parameter that was passed detached: it shares its counter (6 ns each, a locked addition)
+  for (size_t i = 0; i < o.params.size(); ++i)
     if ((*grads)[i] != nullptr) written(o.params[i]);
   Py_RETURN_NONE;
   ARB_END
