@@ -295,9 +295,10 @@ __device__ __forceinline__ void step_chunk(const AdamWLaunch &a, const Scalars &
   }
 }
 
-// Many small CTAs: with moments in 8 bits the step is bound by issued instructions (71 an element) and
-// wants as many warps as 40 registers allow: 128 M elements take 308 us with 12 CTAs of 128 threads an
-// SM, 354 with 5 of 256.  Moments in 32 bits are bound by memory: 64 M elements with a copy take 276 us.
+// Many small CTAs: with moments in 8 bits the step issues 69 instructions an element, three quarters of the
+// time, and waits for a tile's loads the rest; it wants as many warps as 40 registers allow: one bf16
+// tensor of 128 M elements takes 309 us with 12 CTAs of 128 threads an SM, 354 with 5 of 256.  Moments in
+// 32 bits are bound by memory: 64 M elements with a copy take 279 us.
 template <int BITS, bool MASTER, int N>
 __global__ void __launch_bounds__(kThreads<BITS>, BITS == 8 ? 12 : 4) adamw_kernel(AdamWLaunch a, const __grid_constant__ GradPointers<N> grads,
                                                             int first_tensor, int first_chunk, int n_chunks, bool last) {

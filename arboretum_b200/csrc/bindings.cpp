@@ -1,6 +1,7 @@
 // The Python side of the operators on torch tensors: arguments are checked and turned into a call of
 // the C entry points here rather than in Python, whose share of a small call was four times the
-// launch's (16.6 us for a lookup, 333 us for the addresses of 500 gradients).
+// launch's (16.6 us for a lookup, 4.8 here; 333 us for the addresses of 500 gradients, 15 here with the
+// whole step, 11 where the gradients are given once).
 #include <Python.h>
 
 #include <ATen/ATen.h>

@@ -92,8 +92,9 @@ __device__ __forceinline__ void sum_tokens(const LookupLaunch &a, long long b, l
 // rows are read once and the result written once; a thread has the loads of K rows in flight before it
 // adds the first.  With few bags the tokens of a bag are split over ly groups of lanes, which join
 // their sums through shared memory in a fixed order.  20011 bags of up to 12 rows of 100 fp16 columns, a
-// table that the second-level cache holds: 14.3 us, bound by the two accesses' latency (six CTAs an SM;
-// 16.6 with the five that fit without a limit on registers).
+// table that the second-level cache holds: 14.3 us (six CTAs an SM; 16.6 with the five that fit without a
+// limit on registers).  Issue is busy half of that time and warps wait for a turn more than for a load:
+// all eight slots of a round are executed, whatever is left of a bag.
 // LONG: bags of more than kChain rows a lane, whose sums are set aside; apart from the others, which would
 // pay for it with registers (a million bags of 128 rows of one column: 294 us, 329 in one kernel).
 template <typename T, typename O, int VEC, bool TOGETHER, bool LONG>
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_rows_kernel(LookupLaunc
 // The same for 16-bit rows that begin on any two bytes (an odd number of columns): four-byte accesses all
 // the same.  A row's elements are taken as they share aligned words where they lie; where the output's
 // words pair them differently, a word's halves come from two neighbouring lanes.  10608 rows of 4545
-// bf16: 51 us, 66 with an access an element (32 at 4546).
+// bf16: 51 us, 66 with an access an element (32 at 4546, 23 at 4544); bound by issued instructions.
 template <typename T>
 __device__ __forceinline__ unsigned load_pair(const T *row, long long e, long long dim) {  // elements e, e + 1; row + e on four bytes
   if (e >= 0 && e + 1 < dim) return *reinterpret_cast<const unsigned *>(row + e);

@@ -61,8 +61,10 @@ def embedding_grad(grad, tokens, rows, scale=1.0, pooled=False, out=None, out_dt
     place, other layouts whose columns are not contiguous are copied).  tokens: the same tokens, or
     a ``TokenOrder`` of them.  The result has grad's type or float32 (``out`` / ``out_dtype``);
     rows that no token names are zero, or stay as they are with ``accumulate=True``, which adds to
-    ``out``.  Sums are held in float32, in an order that only the tokens decide: equal inputs give
-    equal bits.
+    ``out``.  Sums are held in float32 or more, in an order that only the tokens decide: equal inputs
+    give equal bits.  Tokens are sorted in every call, which takes many times as long as the sums where
+    bags are long (128 tokens for each of a million bags: 6.9 ms, the sums 0.1): tokens that come again
+    are worth a ``token_order``.
     """
     if isinstance(tokens, TokenOrder):
         if tokens.rows != rows:

@@ -163,10 +163,11 @@ const char *ASharedAtomicPeak(int steps, double *pair_updates_per_s);
  * tables of any width: lookup, its gradient, and the AdamW step on what is learned.
  *
  * All pointers below are device memory of `device` (an ordinal) unless said otherwise, `stream`
- * is a cudaStream_t of that device (NULL = its default stream).  The calls only enqueue: no
- * synchronisation, no allocation, so they can be captured into a CUDA graph; outputs and scratch
- * memory belong to the caller and must live until the work is done.  Two calls that may overlap
- * need scratch of their own.  Strides are in elements.
+ * is a cudaStream_t of that device (NULL = its default stream).  AEmbedding, ATokenOrder,
+ * AEmbeddingGrad and AAdamWStep only enqueue: no synchronisation, no allocation, so they can be
+ * captured into a CUDA graph; the other calls may allocate and wait.  Outputs and scratch memory
+ * belong to the caller and must live until the work is done.  Two calls that may overlap need
+ * scratch of their own.  Strides are in elements.
  * Element types: 0 = fp32, 1 = bf16, 2 = fp16; an output has the input's type or fp32.
  * Tokens are int32 (token_bytes 4) or int64 (8): token t of bag b is
  * tokens[b * bag_stride + t * token_stride].  A token outside [0, rows) is an empty slot: it adds
@@ -205,7 +206,7 @@ const char *AEmbeddingGradBytes(int64_t bags, int64_t per_bag, int64_t rows, int
                                 int64_t *scratch_bytes);
 /* out[v][:] = scale * sum of grad[b][:] over all (b, t) whose token is v (accumulate: added to out,
  * rows no token names stay untouched; else they become zero).  `order` of the same bags, tokens a
- * bag and rows.  Summed in fp32 in a fixed order: the same inputs give the same bits on the same
+ * bag and rows.  Summed in fp32 or more in a fixed order: the same inputs give the same bits on the same
  * device.  grad_stride 0: one row for all bags. */
 const char *AEmbeddingGrad(const void *grad, int type, int64_t bags, int64_t dim, int64_t grad_stride,
                            const void *order, int64_t per_bag, int64_t rows, double scale, void *out, int out_type,
