@@ -1411,7 +1411,8 @@ void lookup_table_with(const LookupLaunch &a, cudaStream_t s) {
 
 template <typename T, typename O>
 bool lookup_table(const LookupLaunch &a, cudaStream_t s) {
-  // Only where the bags of one slot lie next to one another, the table fits, the lookups are many times
+  // Instances are there for one to three columns (a leaf's values for a few classes); wider rows go through
+  // the cache.  Only where the bags of one slot lie next to one another, the table fits, the lookups are many times
   // the words every SM has to copy first, and a thread's chain of additions is not too long.
   const TokenView &t = a.tokens;
   if (a.dim > 3 || t.per_bag < 2 || t.per_bag > kMostTableTokens || std::abs(t.bag_stride) >= std::abs(t.token_stride) ||
